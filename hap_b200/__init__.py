@@ -14,8 +14,12 @@ from .linear import linear
 from . import plan, spmd, attention, fxpass, profiler, dropout
 from .einsum import einsum
 from .loss import nll_log_softmax_sum
-from .norm import layer_norm
+from . import block8
+from .block8 import Block8
+from .linear8 import linear8
+from .norm import layer_norm, layer_norm8
 from .optim import ClipAdam
 
 __all__ = ["Comm", "init_process_comm", "local_comm", "single_comm", "collectives", "LocalCollectives",
-           "sharding_round", "sharding_round_", "linear", "linear_ops", "plan", "spmd", "attention", "einsum"]
+           "sharding_round", "sharding_round_", "linear", "linear_ops", "plan", "spmd", "attention", "einsum", "block8",
+           "Block8", "linear8", "layer_norm8"]

@@ -22,6 +22,7 @@ from . import _native as N
 from . import dropout as _dropout
 from .comm import _on_device, _stream
 from .linear import linear
+from .linear8 import linear8
 
 FUSED_HEAD_DIM = 64
 
@@ -174,6 +175,27 @@ def multi_head_attention_forward(query, key, value, embed_dim_to_check, num_head
         raise NotImplementedError("attention: bias_k / bias_v / add_zero_attn / key_padding_mask / separate weights are not emitted by the planner")
     if query.shape[-1] != embed_dim_to_check:
         raise ValueError("attention: embedding dimension mismatch")
-    qkv = linear(query, in_proj_weight, in_proj_bias)
-    out = attention(qkv, num_heads, attn_mask, float(dropout_p) if training else 0.0)
-    return linear(out, out_proj_weight, out_proj_bias), None
+    return _project_attend_project(linear, query, num_heads, in_proj_weight, in_proj_bias, attn_mask, float(dropout_p) if training else 0.0,
+                                   out_proj_weight, out_proj_bias)
+
+
+def _project_attend_project(project, x, num_heads, in_w, in_b, attn_mask, dropout_p, out_w, out_b):
+    qkv = project(x, in_w, in_b)
+    out = attention(qkv, num_heads, attn_mask, dropout_p)
+    return project(out, out_w, out_b), None
+
+
+def multi_head_attention_forward8(query, key, value, embed_dim_to_check, num_heads, in_proj_weight, in_proj_bias,
+                                  bias_k=None, bias_v=None, add_zero_attn=False, dropout_p=0.0, out_proj_weight=None,
+                                  out_proj_bias=None, training=True, key_padding_mask=None, need_weights=True, attn_mask=None,
+                                  use_separate_proj_weight=False, **unsupported):
+    """:func:`multi_head_attention_forward` with the two projections on :func:`hap_b200.linear8.linear8` (their products
+    in 8-bit floating point); the attention core between them is the same."""
+    if not (query is key and key is value):
+        raise NotImplementedError("attention: only self-attention (query is key is value) is emitted by the planner")
+    if bias_k is not None or bias_v is not None or add_zero_attn or key_padding_mask is not None or use_separate_proj_weight:
+        raise NotImplementedError("attention: bias_k / bias_v / add_zero_attn / key_padding_mask / separate weights are not emitted by the planner")
+    if query.shape[-1] != embed_dim_to_check:
+        raise ValueError("attention: embedding dimension mismatch")
+    return _project_attend_project(linear8, query, num_heads, in_proj_weight, in_proj_bias, attn_mask, float(dropout_p) if training else 0.0,
+                                   out_proj_weight, out_proj_bias)

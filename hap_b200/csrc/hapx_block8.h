@@ -1,0 +1,87 @@
+// 8-bit blocks: e4m3 values with one power-of-two scale per block of 128 elements, shared by the quantiser, the
+// block-scaled product and the operators that keep their input for the backward pass in 8 bits.
+//
+// A block's scale is 2^e with the smallest integer e >= -126 for which the block's largest magnitude is at most
+// 448 * 2^e (448 = 1.75 * 2^8 is the largest e4m3 number); a block of zeros has e = 0.  Scaling by a power of two is
+// exact, so the stored value is the correctly rounded (to nearest, ties to even) e4m3 number of x * 2^-e and the
+// only error of a block is that one rounding: half a step of 3 fraction bits, 2^-4 relative, for magnitudes down to
+// 2^-14 of the block's largest one.  e4m3 has no infinity: infinities and NaN become NaN and do not enter the maximum.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+namespace hapx {
+namespace block8 {
+
+constexpr int kBlock = 128;
+
+// Exponent of the scale of a block whose largest finite magnitude is `big` (>= 0).
+__device__ __forceinline__ int scale_exponent(float big) {
+  const unsigned b = __float_as_uint(big);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);   // 0x600000: the fraction of 1.75
+  return b == 0u ? 0 : max(e, -126);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
+
+// Infinities become NaN; fmaxf then leaves both out of a block's maximum.
+__device__ __forceinline__ float finite_or_nan(float v) {
+  return (__float_as_uint(v) & 0x7fffffffu) >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : v;
+}
+
+// Two values, already scaled, as two e4m3 bytes (the first in the low byte); NaN stays NaN.
+__device__ __forceinline__ unsigned pack2(float lo, float hi) {
+  return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) { return pack2(a, b) | (pack2(c, d) << 16); }
+__device__ __forceinline__ float2 unpack2(unsigned two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+__device__ __forceinline__ float warp_max(float v) {   // v >= 0 and not NaN: the bit patterns order like the numbers
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Four consecutive elements; `vec` says that p is aligned to all four.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool vec, int valid, float (&f)[4]) {
+  if (vec && valid >= 4) {
+    if constexpr (sizeof(T) == 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      f[0] = __uint_as_float(w.x << 16); f[1] = __uint_as_float(w.x & 0xffff0000u);
+      f[2] = __uint_as_float(w.y << 16); f[3] = __uint_as_float(w.y & 0xffff0000u);
+    } else {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = j < valid ? to_f(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, bool vec, int valid, const float (&f)[4]) {
+  if (vec && valid >= 4) {
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+    } else {
+      *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) p[j] = from_f<T>(f[j]);
+  }
+}
+
+}  // namespace block8
+}  // namespace hapx

@@ -13,6 +13,7 @@ draws fresh masks on every replay.  Call ids number the dropout sites in program
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .comm import _on_device, _stream
@@ -173,6 +174,52 @@ def act_dropout(x: torch.Tensor, act: str, p: float, training: bool = True) -> t
     _check(x, "act_dropout", p)
     p = float(p) if training else 0.0
     return _ActDropout.apply(x, _ACTS[act], p, new_call_id() if p > 0.0 else 0)
+
+
+class _ActDropout8(torch.autograd.Function):
+    """What is kept for the backward pass: gelu its input as e4m3 values with one scale per 128 consecutive elements,
+    relu one bit per element (active and kept)."""
+
+    @staticmethod
+    def forward(ctx, x, act, p, call_id, keep):
+        (x,) = _dense(x)
+        n = x.numel()
+        y = torch.empty_like(x)
+        saved = scales = None
+        if keep and ctx.needs_input_grad[0]:
+            saved = torch.empty((n + 7) // 8 if act == 1 else (n + 3) // 4 * 4, dtype=torch.uint8, device=x.device)
+            scales = torch.empty((n + 127) // 128, dtype=torch.float32, device=x.device) if act == 2 else None
+        with _on_device(x.device):
+            N.check(N.lib.hapx_act_dropout8(y.data_ptr(), saved.data_ptr() if saved is not None else None,
+                                            scales.data_ptr() if scales is not None else None, x.data_ptr(), _code(x), n, act, float(p),
+                                            call_id, _stream(x.device)))
+        ctx.save_for_backward(saved, scales)
+        ctx.meta = (act, p, call_id, y.stride())
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        saved, scales = ctx.saved_tensors
+        act, p, call_id, strides = ctx.meta
+        grad = _in_layout(grad, strides)              # the layout the forward pass walked
+        dx = torch.empty_strided(grad.shape, strides, dtype=grad.dtype, device=grad.device)
+        with _on_device(grad.device):
+            N.check(N.lib.hapx_act_dropout8_backward(dx.data_ptr(), grad.data_ptr(), saved.data_ptr(),
+                                                     scales.data_ptr() if scales is not None else None, _code(grad), grad.numel(), act,
+                                                     float(p), call_id, _stream(grad.device)))
+        return dx, None, None, None, None
+
+
+def act_dropout8(x: torch.Tensor, act: str, p: float, training: bool = True) -> torch.Tensor:
+    """:func:`act_dropout` that keeps one byte (gelu) or one bit (relu) per element for the backward pass instead of a
+    whole tensor.  The result is the same; relu's gradient too, gelu's slope is taken at the input rounded to e4m3
+    (blocks of 128 consecutive elements, :mod:`hap_b200.block8`)."""
+    _check(x, "act_dropout8", p)
+    if act not in _ACTS:
+        raise ValueError(f"act_dropout8: the activation is \"relu\" or \"gelu\", got {act!r}")
+    p = float(p) if training else 0.0
+    return _ActDropout8.apply(x, _ACTS[act], p, new_call_id() if p > 0.0 else 0, torch.is_grad_enabled())
 
 
 def keep_mask(n: int, p: float, call_id: int, device=None) -> torch.Tensor:

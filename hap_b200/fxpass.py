@@ -268,6 +268,41 @@ def fuse_residual_norm(graph: torch.fx.Graph) -> int:
     return changed
 
 
+def use_block8(graph: torch.fx.Graph, products: bool = True, saved: bool = True, skip=None) -> Dict[str, int]:
+    """Move a program onto the 8-bit operators; rewrites ``graph`` in place and returns how many nodes of each kind
+    were changed.  Run it last, after the passes that fuse nodes.
+
+    * ``products``: ``linear`` -> :func:`hap_b200.linear8.linear8`, ``multi_head_attention_forward`` ->
+      :func:`hap_b200.attention.multi_head_attention_forward8` (its two projections): products in 8-bit floating point,
+      inputs kept for the backward pass in 8 bits;
+    * ``saved``: ``act_dropout`` -> :func:`hap_b200.dropout.act_dropout8`, ``layer_norm`` / ``layer_norm_fork`` ->
+      :func:`hap_b200.norm.layer_norm8` / ``layer_norm_fork8``: the same forward results, inputs kept in 8 bits.
+
+    ``skip(node)``: true for a node to leave as it is (a vocabulary projection, say).  Unlike the other passes this
+    one changes what the program computes: by the rounding of the products' operands and of the kept inputs."""
+    from .attention import multi_head_attention_forward, multi_head_attention_forward8
+    from .dropout import act_dropout, act_dropout8
+    from .linear import linear
+    from .linear8 import linear8
+    from .norm import layer_norm, layer_norm8, layer_norm_fork, layer_norm_fork8
+    moves = []
+    if products:
+        moves += [(linear, linear8), (multi_head_attention_forward, multi_head_attention_forward8)]
+    if saved:
+        moves += [(act_dropout, act_dropout8), (layer_norm, layer_norm8), (layer_norm_fork, layer_norm_fork8)]
+    changed = {old.__name__: 0 for old, _ in moves}
+    for node in graph.nodes:
+        if node.op != "call_function" or (skip is not None and skip(node)):
+            continue
+        for old, new in moves:
+            if _is(node.target, old):
+                node.target = new
+                changed[old.__name__] += 1
+                break
+    graph.lint()
+    return changed
+
+
 def _peel(node, method: str):
     """If ``node`` is ``x.<method>(...)`` return ``x`` else ``node`` itself."""
     if isinstance(node, torch.fx.Node) and node.op == "call_method" and node.target == method:

@@ -424,6 +424,52 @@ int hapx_layer_norm_backward_add(const void* x, const void* dy, const void* gamm
                                  void* dx, void* dgamma, void* dbeta, float* partial, int dtype, int64_t rows, int64_t E,
                                  hapx_stream stream);
 
+/* ---- 8-bit blocks -----------------------------------------------------------------------
+ * No counterpart in the reference: F.linear (hap.rs:1030-1037) with its products in 8-bit floating point, and
+ * operators that keep their input for the backward pass in 8 bits.
+ *
+ * A matrix of rows x cols is held as e4m3 bytes, `ld` bytes from row to row (base and ld multiples of 16), with one
+ * float32 scale per block of 128 columns of a row, at scale[(c / 128) * ld_scale + r], or per 128 x 128 tile
+ * ("square"), at scale[(c / 128) * ld_scale + r / 128].  value = byte * scale; the scale is 2^e with the smallest
+ * e >= -126 for which the block's largest finite magnitude is at most 448 * 2^e (1 for a block of zeros); infinities
+ * and NaN become NaN.
+ *
+ *   quantize: x (rows x cols of `dtype`, ldx elements from row to row) -> q / s as it stands and / or qt / st
+ *             transposed (cols x rows, blocks along x's rows), in one read; either pair may be null.  `colsum` (may be
+ *             null): ceil(rows / 128) x cols floats, the column sums of every 128 rows of x.
+ *   colsum_join: out[c] = sum of `partial` over the ceil(rows / 128) row groups, in their order.
+ *   dequantize: the values back, contiguous.
+ *   matmul: d[m, n] (contiguous) = a (m x k, 1 x 128 blocks) * b (n x k)^T + bias; sums in float32, one rounding.
+ *             bias: n values of out_dtype or null.  `workspace`: matmul_workspace(m, n, k) bytes (may be 0) on the
+ *             current device, 16-byte aligned, free to be reused when the call's kernels have run. */
+int hapx_block8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int square, void* q, int64_t ldq, float* s,
+                         int64_t lds, void* qt, int64_t ldqt, float* st, int64_t ldst, float* colsum, hapx_stream stream);
+int hapx_block8_colsum_join(void* out, int dtype, const float* partial, int64_t rows, int64_t cols, hapx_stream stream);
+int hapx_block8_dequantize(void* out, int dtype, const void* q, int64_t ldq, const float* s, int64_t lds, int square, int64_t rows,
+                           int64_t cols, hapx_stream stream);
+int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k);
+int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const float* a_scale, int64_t lda_scale, const void* b, int64_t ldb,
+                       const float* b_scale, int64_t ldb_scale, int b_square, const void* bias, int64_t m, int64_t n, int64_t k,
+                       void* workspace, int64_t workspace_bytes, hapx_stream stream);
+/* hapx_act_dropout and its backward pass with less kept in between.  act 2 (gelu): `saved` holds the input as e4m3
+ * bytes (n rounded up to 4, 16-byte aligned), `scales` one float per 128 consecutive elements.  act 1 (relu): `saved`
+ * holds one bit per element, active and kept (bit i % 8 of byte i / 8), `scales` is not used.  saved null: nothing is
+ * kept. */
+int hapx_act_dropout8(void* y, void* saved, float* scales, const void* x, int dtype, int64_t n, int act, double p, uint64_t call_id,
+                      hapx_stream stream);
+int hapx_act_dropout8_backward(void* dx, const void* dy, const void* saved, const float* scales, int dtype, int64_t n, int act, double p,
+                               uint64_t call_id, hapx_stream stream);
+/* layer_norm over the last dimension of any extent E in [1, 2^20], its input kept as e4m3 bytes (rows x ld_saved) with
+ * scales[row * ceil(E / 128) + c / 128]; gamma, beta and add may be null; saved null: nothing is kept and mean, rstd
+ * and scales are not written.  backward: dx = the normalisation's gradient at the kept input (+ add); dgamma, dbeta
+ * may be null, else `workspace` holds backward_workspace(rows, E) bytes; summed in a fixed order. */
+int hapx_layer_norm8_forward(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, void* saved, int64_t ld_saved,
+                             float* scales, int dtype, int64_t rows, int64_t E, double eps, hapx_stream stream);
+int64_t hapx_layer_norm8_backward_workspace(int64_t rows, int64_t E);
+int hapx_layer_norm8_backward(const void* saved, int64_t ld_saved, const float* scales, const void* dy, const void* gamma, const float* mean,
+                              const float* rstd, const void* add, void* dx, void* dgamma, void* dbeta, float* workspace, int dtype, int64_t rows,
+                              int64_t E, hapx_stream stream);
+
 /* ---- diagnostics ----------------------------------------------------------------
  * No counterpart in the reference.  Walks the kernels' tiling of ONE rank's pull over
  * HOST buffers (op: 0 gather, 1 all-to-all, 2 slice, 3 slice-backward), bounds-checking
