@@ -136,26 +136,6 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned char* __
   }
 }
 
-// The product, one thread per output: block sums in float32, joined with the scales in float32.
-template <typename T>
-__global__ void __launch_bounds__(256) matmul_kernel(T* __restrict__ d, const unsigned char* __restrict__ a, long long lda,
-                                                     const float* __restrict__ as, long long ldas, const unsigned char* __restrict__ b,
-                                                     long long ldb, const float* __restrict__ bs, long long ldbs, int b_shift,
-                                                     const T* __restrict__ bias, long long M, long long N, long long K) {
-  const long long n = (long long)blockIdx.x * 16 + (threadIdx.x & 15);
-  for (long long m = (long long)blockIdx.y * 16 + (threadIdx.x >> 4); m < M; m += (long long)gridDim.y * 16) {
-    if (n >= N) continue;
-    float acc = 0.f;
-    for (long long k0 = 0; k0 < K; k0 += kBlock) {
-      float part = 0.f;
-      for (long long k = k0; k < min(k0 + kBlock, K); ++k) part = fmaf(unpack2(a[m * lda + k]).x, unpack2(b[n * ldb + k]).x, part);
-      const long long kb = k0 / kBlock;
-      acc = fmaf(part * bs[kb * ldbs + (n >> b_shift)], as[kb * ldas + m], acc);
-    }
-    d[m * N + n] = from_f<T>(bias ? acc + to_f(bias[n]) : acc);
-  }
-}
-
 static int sms(int* out) {
   int device = 0;
   HAPX_CUDA(cudaGetDevice(&device));
@@ -229,36 +209,6 @@ int hapx_block8_dequantize(void* out, int dtype, const void* q, int64_t ldq, con
   const unsigned char* v = static_cast<const unsigned char*>(q);
   if (dtype == HAPX_BF16) dequantize_kernel<<<grid, 256, 0, stream>>>(v, ldq, s, lds, square ? 7 : 0, static_cast<__nv_bfloat16*>(out), rows, cols);
   else dequantize_kernel<<<grid, 256, 0, stream>>>(v, ldq, s, lds, square ? 7 : 0, static_cast<float*>(out), rows, cols);
-  HAPX_CUDA(cudaGetLastError());
-  count_launch();
-  return HAPX_OK;
-}
-
-int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k) { (void)m; (void)n; (void)k; return 0; }
-
-int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const float* a_scale, int64_t lda_scale, const void* b, int64_t ldb,
-                       const float* b_scale, int64_t ldb_scale, int b_square, const void* bias, int64_t m, int64_t n, int64_t k,
-                       void* workspace, int64_t workspace_bytes, hapx_stream stream_) {
-  if (out_dtype != HAPX_F32 && out_dtype != HAPX_BF16) return fail(HAPX_ERR_DTYPE, "block8_matmul: the output is float32 or bfloat16");
-  if (m < 0 || n < 0 || k < 0 || m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff)
-    return fail(HAPX_ERR_EXTENT, "block8_matmul: extents must lie in [0, 2^31)");
-  if (m == 0 || n == 0) return HAPX_OK;
-  if (!d || (k > 0 && (!a || !a_scale || !b || !b_scale))) return fail(HAPX_ERR_ARGUMENT, "block8_matmul: null pointer");
-  if (k > 0 && (lda % 16 != 0 || ldb % 16 != 0 || lda < k || ldb < k || ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u)))
-    return fail(HAPX_ERR_EXTENT, "block8_matmul: operands need a 16-byte aligned base and pitch, and a pitch that covers a row");
-  if (k > 0 && (lda_scale < m || ldb_scale < (b_square ? (n + kBlock - 1) / kBlock : n)))
-    return fail(HAPX_ERR_EXTENT, "block8_matmul: a scale pitch does not cover its rows");
-  if (workspace_bytes < hapx_block8_matmul_workspace(m, n, k) || (workspace_bytes > 0 && !workspace))
-    return fail(HAPX_ERR_ARGUMENT, "block8_matmul: the workspace is smaller than hapx_block8_matmul_workspace says");
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const dim3 grid((unsigned)((n + 15) / 16), (unsigned)std::min<int64_t>((m + 15) / 16, 65535));
-  const unsigned char *av = static_cast<const unsigned char*>(a), *bv = static_cast<const unsigned char*>(b);
-  if (out_dtype == HAPX_BF16)
-    matmul_kernel<<<grid, 256, 0, stream>>>(static_cast<__nv_bfloat16*>(d), av, lda, a_scale, lda_scale, bv, ldb, b_scale, ldb_scale,
-                                            b_square ? 7 : 0, static_cast<const __nv_bfloat16*>(bias), m, n, k);
-  else
-    matmul_kernel<<<grid, 256, 0, stream>>>(static_cast<float*>(d), av, lda, a_scale, lda_scale, bv, ldb, b_scale, ldb_scale, b_square ? 7 : 0,
-                                            static_cast<const float*>(bias), m, n, k);
   HAPX_CUDA(cudaGetLastError());
   count_launch();
   return HAPX_OK;

@@ -161,6 +161,11 @@ __device__ __forceinline__ unsigned map_to_cta(unsigned smem_addr, unsigned cta)
 __device__ __forceinline__ void mbar_arrive_cluster(unsigned cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same without a release at cluster scope (which waits for the thread's earlier memory traffic to be visible in the
+// whole cluster, about a microsecond): for arrivals that only say that tensor memory has been read.
+__device__ __forceinline__ void mbar_arrive_cluster_light(unsigned cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -440,6 +440,7 @@ int hapx_layer_norm_backward_add(const void* x, const void* dy, const void* gamm
  *   colsum_join: out[c] = sum of `partial` over the ceil(rows / 128) row groups, in their order.
  *   dequantize: the values back, contiguous.
  *   matmul: d[m, n] (contiguous) = a (m x k, 1 x 128 blocks) * b (n x k)^T + bias; sums in float32, one rounding.
+ *             The scales of 1 x 128 blocks of b need a 16-byte aligned base and a pitch that is a multiple of 4.
  *             bias: n values of out_dtype or null.  `workspace`: matmul_workspace(m, n, k) bytes (may be 0) on the
  *             current device, 16-byte aligned, free to be reused when the call's kernels have run. */
 int hapx_block8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int square, void* q, int64_t ldq, float* s,
