@@ -32,16 +32,15 @@ def _blocks(n: int) -> int:
 
 
 class Block8:
-    """``rows x cols`` e4m3 values (``values``, float8_e4m3fn, rows padded to a multiple of 16 bytes) and their
-    scales (``scales``, float32).  The scale of element (r, c) is ``scales[c // 128, r]``, or
-    ``scales[c // 128, r // 128]`` when ``square``.  ``transposed`` is the same matrix with rows and columns
-    exchanged, where the maker was asked for both."""
+    """``rows x cols`` e4m3 values (``values``, float8_e4m3fn, rows padded to a multiple of 16 bytes) and one
+    power-of-two scale per 128 columns of a row (``scales``, bytes in the order the tensor cores read them;
+    :meth:`scale_matrix` decodes them).  ``transposed`` is the same matrix with rows and columns exchanged, where the
+    maker was asked for both."""
 
-    __slots__ = ("values", "scales", "rows", "cols", "square", "transposed")
+    __slots__ = ("values", "scales", "rows", "cols", "transposed")
 
-    def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, square: bool,
-                 transposed: Optional["Block8"] = None):
-        self.values, self.scales, self.rows, self.cols, self.square, self.transposed = values, scales, rows, cols, square, transposed
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, transposed: Optional["Block8"] = None):
+        self.values, self.scales, self.rows, self.cols, self.transposed = values, scales, rows, cols, transposed
 
     @property
     def shape(self):
@@ -53,7 +52,13 @@ class Block8:
 
     @property
     def nbytes(self) -> int:
-        return self.values.numel() + 4 * self.scales.numel()
+        return self.values.numel() + self.scales.numel()
+
+    def scale_matrix(self) -> torch.Tensor:
+        """The scales as float32, (rows, blocks of 128 columns)."""
+        s = self.scales.view(_up(self.cols, 512) // 512, _blocks(self.rows), 32, 4, 4).permute(1, 3, 2, 0, 4)       # [row / 128][row / 32][row % 32][block / 4][block % 4]
+        s = s.reshape(_blocks(self.rows) * BLOCK, _up(self.cols, 512) // 128)[:self.rows, :_blocks(self.cols)]
+        return torch.ldexp(torch.ones(s.shape, device=s.device), s.to(torch.int32) - 127)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The matrix as it is represented (exact in bfloat16 too: e4m3 has four significant bits)."""
@@ -62,12 +67,11 @@ class Block8:
         out = torch.empty((self.rows, self.cols), dtype=dtype, device=self.device)
         with _on_device(self.device):
             N.check(N.lib.hapx_block8_dequantize(out.data_ptr(), _CODES[dtype], self.values.data_ptr(), self.values.shape[1],
-                                                 self.scales.data_ptr(), self.scales.shape[1], int(self.square), self.rows, self.cols,
-                                                 _stream(self.device)))
+                                                 self.scales.data_ptr(), self.rows, self.cols, _stream(self.device)))
         return out
 
     def __repr__(self):
-        return f"Block8({self.rows} x {self.cols}, {'128 x 128' if self.square else '1 x 128'} blocks, {self.device})"
+        return f"Block8({self.rows} x {self.cols}, {self.device})"
 
 
 def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -85,18 +89,18 @@ def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     return x
 
 
-def _empty(rows: int, cols: int, square: bool, device) -> Block8:
+def _empty(rows: int, cols: int, device) -> Block8:
     values = torch.empty((rows, _up(cols, 16)), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty((_blocks(cols), _up(_blocks(rows) if square else rows, 4)), dtype=torch.float32, device=device)
-    return Block8(values, scales, rows, cols, square)
+    scales = torch.empty(_up(cols, 512) // 512 * _blocks(rows) * 512, dtype=torch.uint8, device=device)
+    return Block8(values, scales, rows, cols)
 
 
 def _run(x: torch.Tensor, square: bool, q: Optional[Block8], qt: Optional[Block8], colsum: Optional[torch.Tensor] = None) -> None:
     """One pass of the quantiser over ``x`` into ``q`` (as it stands) and / or ``qt`` (transposed)."""
     rows, cols = x.shape
     ldx = x.stride(0) if rows > 1 else cols
-    a = (q.values.data_ptr(), q.values.shape[1], q.scales.data_ptr(), q.scales.shape[1]) if q is not None else (None, 0, None, 0)
-    b = (qt.values.data_ptr(), qt.values.shape[1], qt.scales.data_ptr(), qt.scales.shape[1]) if qt is not None else (None, 0, None, 0)
+    a = (q.values.data_ptr(), q.values.shape[1], q.scales.data_ptr()) if q is not None else (None, 0, None)
+    b = (qt.values.data_ptr(), qt.values.shape[1], qt.scales.data_ptr()) if qt is not None else (None, 0, None)
     with _on_device(x.device):
         N.check(N.lib.hapx_block8_quantize(x.data_ptr(), _CODES[x.dtype], rows, cols, ldx, int(square), *a, *b,
                                            colsum.data_ptr() if colsum is not None else None, _stream(x.device)))
@@ -111,8 +115,8 @@ def quantize(x: torch.Tensor, rows: bool = True, columns: bool = False):
     x = _matrix(x, "block8.quantize")
     if columns and x.shape[0] < 1:
         raise ValueError("block8.quantize: the columns of an empty matrix have no blocks")
-    q = _empty(x.shape[0], x.shape[1], False, x.device) if rows else None
-    qt = _empty(x.shape[1], x.shape[0], False, x.device) if columns else None
+    q = _empty(x.shape[0], x.shape[1], x.device) if rows else None
+    qt = _empty(x.shape[1], x.shape[0], x.device) if columns else None
     _run(x, False, q, qt)
     return (q, qt) if rows and columns else (q if rows else qt)
 
@@ -124,19 +128,16 @@ def quantize_weight(w: torch.Tensor, transposed: bool = False) -> Block8:
     w = _matrix(w, "block8.quantize_weight")
     if w.shape[0] < 1:
         raise ValueError("block8.quantize_weight: rows of at least one element are expected")
-    q = _empty(w.shape[0], w.shape[1], True, w.device)
-    qt = _empty(w.shape[1], w.shape[0], True, w.device) if transposed else None
+    q = _empty(w.shape[0], w.shape[1], w.device)
+    qt = _empty(w.shape[1], w.shape[0], w.device) if transposed else None
     _run(w, True, q, qt)
     q.transposed = qt
     return q
 
 
 def matmul(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``a @ b.T (+ bias)``: a (m x k) in 1 x 128 blocks, b (n x k) in 1 x 128 or 128 x 128 blocks, m x n out.  Every
-    block's products are summed on the tensor cores in float32 and the blocks joined with their scales in float32;
-    one rounding to ``out_dtype``.  ``bias``: n values of ``out_dtype``.  Not differentiable."""
-    if a.square:
-        raise ValueError("block8.matmul: the first operand is expected in 1 x 128 blocks (block8.quantize)")
+    """``a @ b.T (+ bias)``: a (m x k), b (n x k), m x n out.  Products and scales are multiplied on the tensor cores and
+    summed there in float32; one rounding to ``out_dtype``.  ``bias``: n values of ``out_dtype``.  Not differentiable."""
     if a.cols != b.cols:
         raise ValueError(f"block8.matmul: contraction lengths differ ({a.cols} and {b.cols})")
     if a.device != b.device:
@@ -155,7 +156,7 @@ def matmul(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype:
         need = N.lib.hapx_block8_matmul_workspace(m, n, k)
         ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
         N.check(N.lib.hapx_block8_matmul(out.data_ptr(), _CODES[out_dtype], a.values.data_ptr(), a.values.shape[1], a.scales.data_ptr(),
-                                         a.scales.shape[1], b.values.data_ptr(), b.values.shape[1], b.scales.data_ptr(), b.scales.shape[1],
-                                         int(b.square), bias.data_ptr() if bias is not None else None, m, n, k,
-                                         ws.data_ptr() if need else None, need, _stream(a.device)))
+                                         b.values.data_ptr(), b.values.shape[1], b.scales.data_ptr(),
+                                         bias.data_ptr() if bias is not None else None, m, n, k, ws.data_ptr() if need else None, need,
+                                         _stream(a.device)))
     return out

@@ -6,6 +6,9 @@
 // exact, so the stored value is the correctly rounded (to nearest, ties to even) e4m3 number of x * 2^-e and the
 // only error of a block is that one rounding: half a step of 3 fraction bits, 2^-4 relative, for magnitudes down to
 // 2^-14 of the block's largest one.  e4m3 has no infinity: infinities and NaN become NaN and do not enter the maximum.
+//
+// A matrix's scales are kept as the bytes e + 127 in the order the tensor cores take them: 512 bytes for every 128 rows
+// and 4 blocks of columns, in them 16 bytes for each of 32 lanes (row % 32), 4 for each row / 32, one per block.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -24,6 +27,14 @@ __device__ __forceinline__ int scale_exponent(float big) {
   return b == 0u ? 0 : max(e, -126);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
+
+__host__ __device__ __forceinline__ long long scale_bytes(long long rows, long long cols) {
+  return ((cols + 511) / 512) * ((rows + 127) / 128) * 512;
+}
+// Where the scale of row r and column block kb is; `groups` = ceil(rows / 128).
+__device__ __forceinline__ long long scale_at(long long r, long long kb, long long groups) {
+  return ((kb >> 2) * groups + (r >> 7)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (kb & 3);
+}
 
 // Infinities become NaN; fmaxf then leaves both out of a block's maximum.
 __device__ __forceinline__ float finite_or_nan(float v) {

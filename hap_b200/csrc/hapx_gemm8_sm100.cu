@@ -1,18 +1,21 @@
-// The block-scaled product on the tensor cores: D[M, N] = sum over blocks kb of 128 along the contraction of
-//     a_scale[kb][m] * b_scale[kb][n] * sum_{k in kb} A[m, k] B[n, k]   (+ bias)
-// with e4m3 operands, both with the contraction contiguous in memory (hapx_block8.h).
+// The block-scaled product on the tensor cores: D[M, N] = sum over k of (a_scale A)[m, k] (b_scale B)[n, k]  (+ bias)
+// with e4m3 operands, both with the contraction contiguous in memory, and one power-of-two scale per block of 128 along
+// the contraction (hapx_block8.h).
 //
-// Persistent and warp-specialised like the bfloat16 product (hapx_gemm_sm100.cu), with one difference that shapes it:
-// an accumulator lives for ONE block of 128 only.  Its scales differ from the next block's, so tensor memory holds
-// block products, and the epilogue warps keep the running float32 sums of the output tile in registers, adding each
-// block product with its scales while the tensor cores work on the next one (two accumulators, used alternately).
-//   warp 0      : TMA producer (128 x 128 byte tiles, 128-byte swizzle; with 1 x 128 blocks of B also their scales)
-//   warp 1      : allocates TMEM; one thread issues tcgen05.mma kind::f8f6f4, four of 32 deep per block
-//   warps 4 ... : epilogue; a warp owns 32 rows x CW columns of the tile, a thread one row: CW float32 sums
+// The scales are applied by the tensor cores (tcgen05.mma kind::mxf8f6f4, which multiplies every 32 products by the two
+// scales of their row and column before adding them): the four 32-deep instructions of a block of 128 name the same
+// scale bytes.  So an accumulator runs over the whole contraction, as in the bfloat16 product (hapx_gemm_sm100.cu),
+// whose structure this kernel has: persistent, warp-specialised, two accumulators used alternately.
+//   warp 0      : TMA producer (128 x 128 byte tiles, 128-byte swizzle; every fourth block also the scales of four blocks)
+//   warp 1      : allocates TMEM; one thread copies scales to tensor memory (tcgen05.cp) and issues tcgen05.mma
+//   warps 2 - 9 : epilogue, two warps per 32 rows: bias, one rounding, bulk stores through a staging tile
+// (An earlier form kept one accumulator per block and the running sums in registers, adding block products with their
+// scales in the epilogue warps; it was bound by the chain commit -> wait -> read -> arrive of its two accumulators.)
 //
-// Pair kernel (M > 128): clusters of two CTAs, 256 x 256 tiles, cta_group::2; each CTA stages its 128 rows of A and half
-// of B's rows and sums its 128 x 256 half of the tile with eight epilogue warps (128 sums per thread).  Single kernel
-// (M <= 128): 128 x 64 tiles, so that a narrow product still spreads over the SMs.
+// Pair kernel (M > 128): clusters of two CTAs, 256 x 192 tiles, cta_group::2; each CTA stages its 128 rows of A and half
+// of B's rows.  192 columns, because two accumulators of 192 leave tensor memory for the scales, and the model widths
+// (768, 2304) are whole numbers of such tiles.  Single kernel (M <= 128): 128 x 64 tiles, so that a narrow product still
+// spreads over the SMs.
 //
 // Every mbarrier wait is bounded; on expiry a role raises the error word and leaves, the others follow as their own
 // waits run out, TMEM is freed and the kernel returns.
@@ -36,78 +39,68 @@ using namespace tc;
 constexpr int BM = 128;      // rows of the tile per CTA
 constexpr int BK = 128;      // one block of the contraction: one 128-byte swizzle row
 constexpr int UMMA_K = 32;
+constexpr unsigned kAtom = 512;      // scales of 128 rows x 4 blocks
 
 struct Params {
   int M, N, k_blocks;
-  const float* a_scale; long long lda_scale;
-  const float* b_scale; long long ldb_scale;   // square: [k block][block of 128 rows]
   void* D; long long ldd;
   const void* bias;          // N values of D's type, or null
-  int out_f32, tma_store;
+  int out_f32, tma_store, bias_vec;
   int m_tiles, n_tiles;
   int splits, kb_per_split;  // > 1: the blocks are cut into ranges; each writes a float32 partial tile to rows [split * m_pad, ...)
   long long m_pad;
   unsigned* error;
 };
 
-__device__ __forceinline__ void umma8(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void umma8(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned sfa, unsigned sfb,
+                                      unsigned accumulate) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
 }
-__device__ __forceinline__ void umma8_pair(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Two float32 lanes per instruction.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair2(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 pair2u(unsigned a, unsigned b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
+// One atom of scales (32 lanes x 16 bytes, lane by lane in shared memory) to 4 columns of tensor memory, in all four
+// lane quarters; with a pair, in each CTA from its own shared memory.
+template <bool PAIR>
+__device__ __forceinline__ void copy_scales(unsigned taddr, unsigned smem) {
+  // no swizzle; 8 lanes x 16 bytes are a core matrix, the next 8 lanes follow 128 bytes later
+  const unsigned long long desc = (unsigned long long)((smem & 0x3ffffu) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46);
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-template <bool PAIR, bool SQUARE>
+template <bool PAIR>
 struct Cfg {
-  static constexpr int BN = PAIR ? 256 : 64;                 // columns of the tile
-  static constexpr int EPI_WARPS = PAIR ? 8 : 4;
-  static constexpr int CW = BN / (EPI_WARPS / 4);            // columns per epilogue warp
-  static constexpr int THREADS = 128 + 32 * EPI_WARPS;      // warps 2 and 3 only complete the first warpgroup
-  static constexpr int STAGES = PAIR ? 5 : 7;
-  static constexpr int RING = STAGES + 4;                    // slots of B's scales; see the producer
+  static constexpr int BN = PAIR ? 192 : 64;                 // columns of the tile
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int STAGES = PAIR ? 6 : 7;
+  static constexpr int B_ATOMS = PAIR ? 2 : 1;               // 192 columns from a multiple of 64 on lie in two groups of 128
   static constexpr unsigned A_BYTES = BM * BK;
   static constexpr unsigned B_BYTES = (PAIR ? BN / 2 : BN) * BK;
   static constexpr unsigned STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr unsigned SCALE_BYTES = SQUARE ? 0 : BN * 4;
+  static constexpr unsigned SCALE_BYTES = (1 + B_ATOMS) * kAtom;
   static constexpr unsigned STORE_BYTES = EPI_WARPS * 32 * 128;  // one 32-row x 128-byte staging tile per epilogue warp
-  static constexpr unsigned TMEM_COLS = 2 * BN;
-  static constexpr unsigned SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STORE_BYTES + RING * SCALE_BYTES + 256;
-  // float32 accumulator, e4m3 x e4m3 (format 0), K-major operands, N >> 3, M >> 4
-  static constexpr unsigned IDESC = (1u << 4) | ((unsigned)(BN >> 3) << 17) | ((unsigned)((PAIR ? 2 * BM : BM) >> 4) << 24);
+  static constexpr unsigned SF_COL = 2 * BN;                 // scales behind the accumulators, one set per stage
+  static constexpr unsigned SF_SET = 4 * (1 + B_ATOMS);
+  static constexpr unsigned TMEM_COLS = PAIR ? 512 : 256;
+  static_assert(SF_COL + STAGES * SF_SET <= TMEM_COLS, "tensor memory");
+  static constexpr unsigned SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STORE_BYTES + STAGES * SCALE_BYTES + 256;
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+  // e4m3 x e4m3 (format 0), K-major operands, N >> 3 at bit 17, scales of type ue8m0 (bit 23), M >> 7 at bit 27; the
+  // bytes of the scale words that an instruction uses at bits 4 (B) and 29 (A)
+  static constexpr unsigned IDESC = ((unsigned)(BN >> 3) << 17) | (1u << 23) | ((unsigned)((PAIR ? 2 * BM : BM) >> 7) << 27);
 };
 
 // One 128-byte row piece per thread, swizzled within the warp's staging tile (chunk ^ row % 8).
@@ -130,15 +123,43 @@ __device__ __forceinline__ void stage_row(unsigned char* row, int sw, const floa
   }
 }
 
-template <bool PAIR, bool SQUARE>
-__global__ void __launch_bounds__(Cfg<PAIR, SQUARE>::THREADS, 1)
-gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmS,
-             const __grid_constant__ CUtensorMap tmD, const Params p) {
-  using C = Cfg<PAIR, SQUARE>;
+// v[j] += bias[n + j] for the columns inside the matrix.
+template <bool OUT_F32, int W>
+__device__ __forceinline__ void add_bias(const Params& p, int n, float (&v)[W]) {
+  if (p.bias_vec && n + W <= p.N) {            // 16-byte loads, the same address in every lane
+    if constexpr (OUT_F32) {
+      const float4* b = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + n);
+#pragma unroll
+      for (int j = 0; j < W / 4; ++j) {
+        const float4 x = __ldg(b + j);
+        v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+      }
+    } else {
+      const uint4* b = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + n);
+#pragma unroll
+      for (int j = 0; j < W / 8; ++j) {
+        const uint4 x = __ldg(b + j);
+        const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[8 * j + 2 * e] += __uint_as_float(w[e] << 16); v[8 * j + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u); }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if (n + j < p.N) v[j] += OUT_F32 ? static_cast<const float*>(p.bias)[n + j] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n + j]);
+  }
+}
+
+template <bool PAIR>
+__global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
+gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
+             const __grid_constant__ CUtensorMap tmSB, const __grid_constant__ CUtensorMap tmD, const Params p) {
+  using C = Cfg<PAIR>;
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* gen_base = smem_raw + (base - smem_u32(smem_raw));
-  constexpr unsigned kStore = C::STAGES * C::STAGE_BYTES, kScales = kStore + C::STORE_BYTES, kBars = kScales + C::RING * C::SCALE_BYTES;
+  constexpr unsigned kStore = C::STAGES * C::STAGE_BYTES, kScales = kStore + C::STORE_BYTES, kBars = kScales + C::STAGES * C::SCALE_BYTES;
   const unsigned bars = base + kBars;
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (C::STAGES + s); };
@@ -169,6 +190,8 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     fence_barrier_init();
     prefetch_tensormap(&tmA);
     prefetch_tensormap(&tmB);
+    prefetch_tensormap(&tmSA);
+    prefetch_tensormap(&tmSB);
   }
   if (warp == 1) {
     if (PAIR) { tmem_alloc2(tmem_slot, C::TMEM_COLS); tmem_relinquish2(); }
@@ -180,14 +203,10 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
   tc_fence_after();
   const unsigned tmem_base = *tmem_slot_gen;
 
-  // 384 threads start with 168 registers each; the epilogue's 128 sums and two buffers of 32 need more, the first
-  // warpgroup far fewer: 128 x 40 + 256 x 232 = 64,512, the block's all.
-  if (warp < 4) {
-    if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0) {
+  if (warp == 0) {
     // ---------------- TMA producer (one per CTA) ----------------
     if (lane == 0) {
-      int stage = 0, slot = 0;
+      int stage = 0;
       unsigned phase = 0;
       bool ok = true;
       for (int unit = worker; unit < units && ok; unit += workers) {
@@ -195,28 +214,34 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u)) { ok = false; break; }
           const unsigned sa = base + stage * C::STAGE_BYTES, sb = sa + C::A_BYTES;
-          // This stage's block products are done, so the sums of the two blocks before it are too: the accumulator they
-          // came from was needed.  A slot of B's scales is therefore free STAGES + 2 blocks after it was filled.
-          const unsigned ss = base + kScales + slot * C::SCALE_BYTES;
+          // the scales of four blocks come with the first of them that the unit needs, in the stage's own slot
+          const bool scales = kb == u.kb0 || (kb & 3) == 0;
+          const unsigned ss = base + kScales + stage * C::SCALE_BYTES;
+          const unsigned bytes = C::STAGE_BYTES + (scales ? C::SCALE_BYTES : 0u);
           if (PAIR) {
             const unsigned bar = map_to_cta(full_bar(stage), 0);
-            if (cta == 0) mbar_expect_tx(full_bar(stage), 2 * (C::STAGE_BYTES + C::SCALE_BYTES));     // the bytes of both CTAs
+            if (cta == 0) mbar_expect_tx(full_bar(stage), 2 * bytes);     // the bytes of both CTAs
             tma_load_4d_pair(sa, &tmA, kb * BK, u.m0, 0, 0, bar);
             tma_load_4d_pair(sb, &tmB, kb * BK, u.n0 + cta * (C::BN / 2), 0, 0, bar);
-            if (!SQUARE) tma_load_4d_pair(ss, &tmS, u.n0, kb, 0, 0, bar);
+            if (scales) {
+              tma_load_4d_pair(ss, &tmSA, 0, u.m0 >> 7, kb >> 2, 0, bar);
+              tma_load_4d_pair(ss + kAtom, &tmSB, 0, u.n0 >> 7, kb >> 2, 0, bar);
+            }
           } else {
-            mbar_expect_tx(full_bar(stage), C::STAGE_BYTES + C::SCALE_BYTES);
+            mbar_expect_tx(full_bar(stage), bytes);
             tma_load_4d(sa, &tmA, kb * BK, u.m0, 0, 0, full_bar(stage));
             tma_load_4d(sb, &tmB, kb * BK, u.n0, 0, 0, full_bar(stage));
-            if (!SQUARE) tma_load_4d(ss, &tmS, u.n0, kb, 0, 0, full_bar(stage));
+            if (scales) {
+              tma_load_4d(ss, &tmSA, 0, u.m0 >> 7, kb >> 2, 0, full_bar(stage));
+              tma_load_4d(ss + kAtom, &tmSB, 0, u.n0 >> 7, kb >> 2, 0, full_bar(stage));
+            }
           }
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-          if (++slot == C::RING) slot = 0;
         }
       }
       if (!ok) atomicCAS(p.error, 0u, 1u);
     }
-    } else if (warp == 1) {
+  } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
     if (lane == 0 && cta == 0) {
       int stage = 0, acc = 0;
@@ -224,145 +249,110 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
       bool ok = true;
       for (int unit = worker; unit < units && ok; unit += workers) {
         const Unit u = decode(unit);
+        const unsigned d = tmem_base + (unsigned)(acc * C::BN), shift = (unsigned)(u.n0 >> 5) & 3u;   // B's rows start inside a group of 128
+        unsigned sfa = 0, sfb = 0;
+        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u)) { ok = false; break; }
         for (int kb = u.kb0; kb < u.kb1; ++kb) {
-          if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u) || !mbar_wait(full_bar(stage), phase)) { ok = false; break; }
+          if (!mbar_wait(full_bar(stage), phase)) { ok = false; break; }
           tc_fence_after();
-          const unsigned sa = base + stage * C::STAGE_BYTES, sb = sa + C::A_BYTES, d = tmem_base + (unsigned)(acc * C::BN);
+          if (kb == u.kb0 || (kb & 3) == 0) {
+            // tcgen05.cp and tcgen05.mma run in the order of their issue, and a set is not written again before the
+            // stages have gone round
+            const unsigned ss = base + kScales + stage * C::SCALE_BYTES;
+            sfa = tmem_base + C::SF_COL + stage * C::SF_SET;
+            sfb = sfa + 4;
+            copy_scales<PAIR>(sfa, ss);
 #pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k) {
-            const unsigned long long da = make_desc(sa + k * 32u, 16u, 1024u), db = make_desc(sb + k * 32u, 16u, 1024u);
-            if (PAIR) umma8_pair(d, da, db, C::IDESC, k != 0);
-            else umma8(d, da, db, C::IDESC, k != 0);
+            for (int i = 0; i < C::B_ATOMS; ++i) copy_scales<PAIR>(sfb + 4 * i, ss + (1 + i) * kAtom);
           }
-          if (PAIR) { umma2_commit_both(empty_bar(stage)); umma2_commit_both(tfull_bar(acc)); }
-          else { umma_commit(empty_bar(stage)); umma_commit(tfull_bar(acc)); }
+          const unsigned sa = base + stage * C::STAGE_BYTES, sb = sa + C::A_BYTES;
+          const unsigned idesc = C::IDESC | ((unsigned)(kb & 3) << 4) | ((unsigned)(kb & 3) << 29);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma8<PAIR>(d, make_desc(sa + k * 32u, 16u, 1024u), make_desc(sb + k * 32u, 16u, 1024u), idesc, sfa, sfb + shift, kb != u.kb0 || k != 0);
+          if (PAIR) umma2_commit_both(empty_bar(stage));
+          else umma_commit(empty_bar(stage));
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
+        if (!ok) break;
+        if (PAIR) umma2_commit_both(tfull_bar(acc));
+        else umma_commit(tfull_bar(acc));
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
       if (!ok) atomicCAS(p.error, 0u, 2u);
     }
-    }
   } else {
-    // ---------------- epilogue: 32 rows x CW columns per warp ----------------
-    if (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    const int q = warp & 3, half = (warp - 4) >> 2;          // q: the TMEM lane quarter this warp may read
-    const unsigned t_warp = tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(half * C::CW);
-    unsigned char* tile_gen = gen_base + kStore + (warp - 4) * 4096;
-    const unsigned tile_u32 = base + kStore + (warp - 4) * 4096;
-    int acc = 0, slot = 0;
+    // ---------------- epilogue: 32 rows per warp, every other piece of 128 bytes per row ----------------
+    const int q = warp & 3, half = (warp - 2) >> 2;          // q: the TMEM lane quarter this warp may read
+    unsigned char* tile_gen = gen_base + kStore + (warp - 2) * 4096;
+    const unsigned tile_u32 = base + kStore + (warp - 2) * 4096;
+    int acc = 0;
     unsigned acc_phase = 0;
     bool ok = true;
-    for (int unit = worker; unit < units && ok; unit += workers) {
+    for (int unit = worker; unit < units; unit += workers) {
       const Unit u = decode(unit);
-      const int row = u.m0 + q * 32 + lane, c0 = u.n0 + half * C::CW;
-      f32x2 sum[C::CW / 2];
-#pragma unroll
-      for (int j = 0; j < C::CW / 2; ++j) sum[j] = 0ull;
-      const float* as = p.a_scale + (row < p.M ? row : 0);
-      const float* bs = p.b_scale + (SQUARE && c0 < p.N ? c0 >> 7 : 0);
-      float sa = as[u.kb0 * p.lda_scale], sb = SQUARE ? bs[u.kb0 * p.ldb_scale] : 1.f;
-      for (int kb = u.kb0; kb < u.kb1; ++kb) {
-        const f32x2 s2 = SQUARE ? pair2(sa * sb, sa * sb) : pair2(sa, sa);
-        const int nx = min(kb + 1, u.kb1 - 1);               // the next block's scales travel during the wait
-        sa = as[nx * p.lda_scale];
-        if (SQUARE) sb = bs[nx * p.ldb_scale];
-        ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
-        if (!ok) break;
-        tc_fence_after();
-        const unsigned t = t_warp + (unsigned)(acc * C::BN);
-        const float* sb_row = reinterpret_cast<const float*>(gen_base + kScales + slot * C::SCALE_BYTES) + half * C::CW;
-        // 32 columns per load, two loads in flight; the accumulator goes back as soon as the last ones have landed
-        auto add = [&](const unsigned (&v)[32], int c) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            f32x2 x0 = pair2u(v[4 * j], v[4 * j + 1]), x1 = pair2u(v[4 * j + 2], v[4 * j + 3]);
-            if (!SQUARE) {
-              const float4 b4 = *reinterpret_cast<const float4*>(sb_row + c + 4 * j);
-              x0 = mul2(x0, pair2(b4.x, b4.y));
-              x1 = mul2(x1, pair2(b4.z, b4.w));
-            }
-            sum[c / 2 + 2 * j] = fma2(x0, s2, sum[c / 2 + 2 * j]);
-            sum[c / 2 + 2 * j + 1] = fma2(x1, s2, sum[c / 2 + 2 * j + 1]);
-          }
-        };
-        unsigned r0[32], r1[32];
-        tmem_ld_32x32(t, r0);
-        tmem_ld_32x32(t + 32, r1);
-#pragma unroll
-        for (int c = 0; c < C::CW; c += 64) {
-          tmem_ld_wait();
-          if (c + 64 >= C::CW) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (PAIR) mbar_arrive_cluster_light(map_to_cta(tempty_bar(acc), 0));
-              else mbar_arrive(tempty_bar(acc));
-            }
-          }
-          add(r0, c);
-          if (c + 64 < C::CW) tmem_ld_32x32(t + c + 64, r0);
-          add(r1, c + 32);
-          if (c + 64 < C::CW) tmem_ld_32x32(t + c + 96, r1);
-        }
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
-        if (++slot == C::RING) slot = 0;
-      }
+      ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
       if (!ok) break;
-      // the finished rows: bias, one rounding, out through the staging tile in pieces of 128 bytes per row
+      tc_fence_after();
+      const unsigned t = tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(acc * C::BN);
       const long long out_row0 = (long long)u.split * p.m_pad + u.m0 + q * 32;
-      auto piece = [&](auto f32_tag, int c) {                // columns c0 + c .. of this warp
-        constexpr bool OUT_F32 = decltype(f32_tag)::value;
-        constexpr int W = OUT_F32 ? 32 : 64;
-        float v[W];
-#pragma unroll
-        for (int j = 0; j < W / 2; ++j) {
-          // `c` is a constant after unrolling
-          unpair2(sum[c / 2 + j], v[2 * j], v[2 * j + 1]);
-        }
-        if (p.bias) {
-#pragma unroll
-          for (int j = 0; j < W; ++j) {
-            const int n = min(c0 + c + j, p.N - 1);
-            v[j] += OUT_F32 ? static_cast<const float*>(p.bias)[n] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]);
-          }
-        }
-        if (lane == 0) bulk_wait_read_0();                   // the previous piece has left the staging tile
+      const int width = min(C::BN, p.N - u.n0);              // columns of the tile inside the matrix
+      auto drained = [&] {                                   // this warp has read its part of the accumulator
+        tc_fence_before();
         __syncwarp();
-        stage_row<OUT_F32>(tile_gen + lane * 128, lane & 7, v);
-        if (p.tma_store) {
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_4d(&tmD, tile_u32, c0 + c, (int)out_row0, 0, 0);
-            bulk_commit_group();
-          }
-        } else {                                             // any pitch: rows of the tile one after another, coalesced
-          __syncwarp();
-          for (int r = 0; r < 32; ++r) {
-            if (u.m0 + q * 32 + r >= p.M) break;
-#pragma unroll
-            for (int h = 0; h < W / 32; ++h) {
-              const int col = lane + 32 * h, byte = col * (OUT_F32 ? 4 : 2);
-              const unsigned char* src = tile_gen + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15);
-              if (c0 + c + col < p.N) {
-                if (OUT_F32) static_cast<float*>(p.D)[(out_row0 + r) * p.ldd + c0 + c + col] = *reinterpret_cast<const float*>(src);
-                else static_cast<__nv_bfloat16*>(p.D)[(out_row0 + r) * p.ldd + c0 + c + col] = *reinterpret_cast<const __nv_bfloat16*>(src);
-              }
-            }
-          }
-          __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster_light(map_to_cta(tempty_bar(acc), 0));
+          else mbar_arrive(tempty_bar(acc));
         }
       };
-      if (p.out_f32) {
+      auto drain = [&](auto f32_tag) {
+        constexpr bool OUT_F32 = decltype(f32_tag)::value;
+        constexpr int W = OUT_F32 ? 32 : 64;
+        bool told = false;
+#pragma unroll 1
+        for (int c = half * W; c < width; c += 2 * W) {
+          unsigned r[W];
+          tmem_ld_32x32(t + (unsigned)c, reinterpret_cast<unsigned(&)[32]>(r[0]));
+          if (!OUT_F32) tmem_ld_32x32(t + (unsigned)c + 32, reinterpret_cast<unsigned(&)[32]>(r[W - 32]));
+          tmem_ld_wait();
+          if (c + 2 * W >= width) { drained(); told = true; }
+          float v[W];
 #pragma unroll
-        for (int c = 0; c < C::CW; c += 32)
-          if (c0 + c < p.N) piece(std::true_type{}, c);
-      } else {
+          for (int j = 0; j < W; ++j) v[j] = __uint_as_float(r[j]);
+          if (p.bias) add_bias<OUT_F32, W>(p, u.n0 + c, v);
+          if (lane == 0) bulk_wait_read_0();                 // the previous piece has left the staging tile
+          __syncwarp();
+          stage_row<OUT_F32>(tile_gen + lane * 128, lane & 7, v);
+          if (p.tma_store) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_4d(&tmD, tile_u32, u.n0 + c, (int)out_row0, 0, 0);
+              bulk_commit_group();
+            }
+          } else {                                           // any pitch: rows of the tile one after another, coalesced
+            __syncwarp();
+            const int rows = min(32, p.M - (u.m0 + q * 32));
+            for (int i = 0; i < rows; ++i) {
 #pragma unroll
-        for (int c = 0; c < C::CW; c += 64)
-          if (c0 + c < p.N) piece(std::false_type{}, c);
-      }
+              for (int h = 0; h < W / 32; ++h) {
+                const int col = lane + 32 * h, byte = col * (OUT_F32 ? 4 : 2);
+                const unsigned char* src = tile_gen + i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15);
+                if (c + col < width) {
+                  const long long at = (out_row0 + i) * p.ldd + u.n0 + c + col;
+                  if (OUT_F32) static_cast<float*>(p.D)[at] = *reinterpret_cast<const float*>(src);
+                  else static_cast<__nv_bfloat16*>(p.D)[at] = *reinterpret_cast<const __nv_bfloat16*>(src);
+                }
+              }
+            }
+            __syncwarp();
+          }
+        }
+        if (!told) drained();                                // no column for this warp in a narrow tile
+      };
+      if (p.out_f32) drain(std::true_type{});
+      else drain(std::false_type{});
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) bulk_wait_all();
     if (!ok) atomicCAS(p.error, 0u, 3u);
@@ -433,14 +423,14 @@ struct Plan { bool pair; int splits, kb_per_split; long long m_pad; int n_pad; }
 static Plan plan_of(long long M, long long N, long long K, int sm_count) {
   Plan pl;
   pl.pair = M > BM;
-  const long long bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true, true>::BN : Cfg<false, true>::BN;
+  const long long bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true>::BN : Cfg<false>::BN;
   const long long m_tiles = (M + bm - 1) / bm, tiles = m_tiles * ((N + bn - 1) / bn);
   const int blocks = (int)((K + BK - 1) / BK), workers = pl.pair ? sm_count / 2 : sm_count;
   pl.splits = 1; pl.kb_per_split = blocks; pl.m_pad = m_tiles * bm; pl.n_pad = (int)((N + 3) / 4 * 4);
   // A long contraction over few tiles leaves SMs idle, or the last round of tiles nearly empty: cut the blocks into
   // ranges whose float32 partial tiles a second kernel adds in a fixed order.  In microseconds: rounds x blocks x the
   // time of one block, and for a split the partial tiles written and read back at about 4 TB/s plus a launch.
-  const double block_us = pl.pair ? 0.30 : 0.15, partial = 8.0 * (double)pl.m_pad * pl.n_pad / 4e6;
+  const double block_us = pl.pair ? 0.25 : 0.15, partial = 8.0 * (double)pl.m_pad * pl.n_pad / 4e6;
   auto rounds = [&](long long units) { return (double)((units + workers - 1) / workers); };
   double best = rounds(tiles) * blocks * block_us;
   for (int sp = 2; sp <= 16 && sp * 4 <= blocks; ++sp) {
@@ -460,11 +450,11 @@ static int sm_count_of(int* out) {
   return HAPX_OK;
 }
 
-template <bool PAIR, bool SQUARE>
-static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmS, const CUtensorMap& tmD, const Params& p, int sm_count,
-                  cudaStream_t stream) {
-  using C = Cfg<PAIR, SQUARE>;
-  auto kernel = gemm8_kernel<PAIR, SQUARE>;
+template <bool PAIR>
+static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmSA, const CUtensorMap& tmSB, const CUtensorMap& tmD,
+                  const Params& p, int sm_count, cudaStream_t stream) {
+  using C = Cfg<PAIR>;
+  auto kernel = gemm8_kernel<PAIR>;
   static int limit_of[64] = {};             // per device: function attributes and occupancy belong to one
   static std::mutex mutex;
   int device = 0;
@@ -497,45 +487,55 @@ static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensor
   const long long units = (long long)p.m_tiles * p.n_tiles * p.splits;
   if (units > 0x7fffffff) return fail(HAPX_ERR_EXTENT, "block8_matmul: too many tiles");
   cfg.gridDim = dim3((unsigned)std::min<long long>(units, limit) * (PAIR ? 2 : 1));
-  HAPX_CUDA(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmS, tmD, p));
+  HAPX_CUDA(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmSA, tmSB, tmD, p));
   count_launch();
   return HAPX_OK;
 }
 
-static int run(void* d, int out_f32, const void* a, long long lda, const float* as, long long ldas, const void* b, long long ldb, const float* bs,
-               long long ldbs, bool square, const void* bias, long long M, long long N, long long K, void* workspace, cudaStream_t stream) {
+// The scales as (128 words of an atom, group of 128 rows, four blocks).
+static int make_scale_map(CUtensorMap* map, const void* ptr, long long rows, int k_blocks, int box_groups) {
+  gemm::EncodeTiledFn fn = gemm::encode_fn();
+  if (!fn) return fail(HAPX_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t groups = (cuuint64_t)((rows + 127) / 128);
+  cuuint64_t dims[4] = {kAtom / 4, groups, (cuuint64_t)((k_blocks + 3) / 4), 1};
+  cuuint64_t strides[3] = {kAtom, kAtom * groups, kAtom * groups};
+  cuuint32_t box[4] = {kAtom / 4, (cuuint32_t)box_groups, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HAPX_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed with code " + std::to_string((int)r));
+  return HAPX_OK;
+}
+
+static int run(void* d, int out_f32, const void* a, long long lda, const void* as, const void* b, long long ldb, const void* bs, const void* bias,
+               long long M, long long N, long long K, void* workspace, cudaStream_t stream) {
   unsigned* error = nullptr;
   int sm_count = 0;
   if (int e = gemm::error_word(&error, &sm_count)) return e;
   const Plan pl = plan_of(M, N, K, sm_count);
   Params p = Params();
   p.M = (int)M; p.N = (int)N; p.k_blocks = (int)((K + BK - 1) / BK);
-  p.a_scale = as; p.lda_scale = ldas; p.b_scale = bs; p.ldb_scale = ldbs;
   p.splits = pl.splits; p.kb_per_split = pl.kb_per_split; p.m_pad = pl.m_pad;
   p.error = error;
-  const int bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true, true>::BN : Cfg<false, true>::BN;
+  const int bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true>::BN : Cfg<false>::BN;
   p.m_tiles = (p.M + bm - 1) / bm; p.n_tiles = (p.N + bn - 1) / bn;
   long long out_rows = M;
   if (pl.splits > 1) { p.D = workspace; p.ldd = pl.n_pad; p.out_f32 = 1; p.bias = nullptr; out_rows = pl.splits * pl.m_pad; }
   else { p.D = d; p.ldd = N; p.out_f32 = out_f32; p.bias = bias; }
+  p.bias_vec = (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
   const int es = p.out_f32 ? 4 : 2;
-  CUtensorMap tmA, tmB, tmS, tmD;
-  std::memset(&tmS, 0, sizeof(tmS));
+  CUtensorMap tmA, tmB, tmSA, tmSB, tmD;
   std::memset(&tmD, 0, sizeof(tmD));
   if (int e = make_map(&tmA, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
   if (int e = make_map(&tmB, b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, ldb, BK, pl.pair ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
-  if (!square)
-    if (int e = make_map(&tmS, bs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, N, p.k_blocks, ldbs, bn, 1, CU_TENSOR_MAP_SWIZZLE_NONE,
-                         CU_TENSOR_MAP_L2_PROMOTION_NONE)) return e;
+  if (int e = make_scale_map(&tmSA, as, M, p.k_blocks, 1)) return e;
+  if (int e = make_scale_map(&tmSB, bs, N, p.k_blocks, pl.pair ? Cfg<true>::B_ATOMS : Cfg<false>::B_ATOMS)) return e;
   p.tma_store = (reinterpret_cast<uintptr_t>(p.D) & 15u) == 0 && (p.ldd * es) % 16 == 0;
   if (p.tma_store)
     if (int e = make_map(&tmD, p.D, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, pl.splits > 1 ? pl.n_pad : N,
                          out_rows, p.ldd, 128 / es, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE)) return e;
-  int e;
-  if (pl.pair) e = square ? launch<true, true>(tmA, tmB, tmS, tmD, p, sm_count, stream) : launch<true, false>(tmA, tmB, tmS, tmD, p, sm_count, stream);
-  else e = square ? launch<false, true>(tmA, tmB, tmS, tmD, p, sm_count, stream) : launch<false, false>(tmA, tmB, tmS, tmD, p, sm_count, stream);
-  if (e) return e;
+  if (int e = pl.pair ? launch<true>(tmA, tmB, tmSA, tmSB, tmD, p, sm_count, stream) : launch<false>(tmA, tmB, tmSA, tmSB, tmD, p, sm_count, stream)) return e;
   if (pl.splits > 1) {
     const int grid = (int)std::min<long long>((M * (pl.n_pad / 4) + 255) / 256, (long long)sm_count * 8);
     const float* ws = static_cast<const float*>(workspace);
@@ -563,9 +563,8 @@ int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
   return pl.splits > 1 ? (int64_t)pl.splits * pl.m_pad * pl.n_pad * 4 : 0;
 }
 
-int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const float* a_scale, int64_t lda_scale, const void* b, int64_t ldb,
-                       const float* b_scale, int64_t ldb_scale, int b_square, const void* bias, int64_t m, int64_t n, int64_t k,
-                       void* workspace, int64_t workspace_bytes, hapx_stream stream) {
+int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const void* a_scale, const void* b, int64_t ldb, const void* b_scale,
+                       const void* bias, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, hapx_stream stream) {
   if (out_dtype != HAPX_F32 && out_dtype != HAPX_BF16) return fail(HAPX_ERR_DTYPE, "block8_matmul: the output is float32 or bfloat16");
   if (m < 0 || n < 0 || k < 1 || m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff)
     return fail(HAPX_ERR_EXTENT, "block8_matmul: extents must lie below 2^31, the contraction at 1 or above");
@@ -573,15 +572,12 @@ int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const
   if (!d || !a || !a_scale || !b || !b_scale) return fail(HAPX_ERR_ARGUMENT, "block8_matmul: null pointer");
   if (lda % 16 != 0 || ldb % 16 != 0 || lda < k || ldb < k || ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u))
     return fail(HAPX_ERR_EXTENT, "block8_matmul: operands need a 16-byte aligned base and pitch, and a pitch that covers a row");
-  if (lda_scale < m || ldb_scale < (b_square ? (n + 127) / 128 : n))
-    return fail(HAPX_ERR_EXTENT, "block8_matmul: a scale pitch does not cover its rows");
-  if (!b_square && (ldb_scale % 4 != 0 || (reinterpret_cast<uintptr_t>(b_scale) & 15u)))
-    return fail(HAPX_ERR_EXTENT, "block8_matmul: the scales of 1 x 128 blocks of b need a 16-byte aligned base and pitch");
+  if ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale)) & 15u)
+    return fail(HAPX_ERR_EXTENT, "block8_matmul: the scales need a 16-byte aligned base");
   const int64_t need = hapx_block8_matmul_workspace(m, n, k);
   if (workspace_bytes < need || (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))))
     return fail(HAPX_ERR_ARGUMENT, "block8_matmul: the workspace must be 16-byte aligned and as large as hapx_block8_matmul_workspace says");
-  return gemm8::run(d, out_dtype == HAPX_F32, a, lda, a_scale, lda_scale, b, ldb, b_scale, ldb_scale, b_square != 0, bias, m, n, k, workspace,
-                    static_cast<cudaStream_t>(stream));
+  return gemm8::run(d, out_dtype == HAPX_F32, a, lda, a_scale, b, ldb, b_scale, bias, m, n, k, workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

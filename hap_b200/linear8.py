@@ -9,7 +9,7 @@ Same call shape as :func:`hap_b200.linear.linear` (the ``torch.nn.functional.lin
     dW = g8t^T x8t         g and x in 128 x 1 blocks along the tokens
     db = sum g             from g itself
 
-x8t is written by the pass that makes x8 and is all the forward pass keeps of x: one byte per element and 4 bytes
+x8t is written by the pass that makes x8 and is all the forward pass keeps of x: one byte per element and one
 per 128 instead of two or four bytes per element.  The weight's 8-bit transposed form is kept too (one byte per
 weight).  A weight that does not change (evaluation, frozen layers) is quantised once with
 :func:`hap_b200.block8.quantize_weight` and passed as it is.
@@ -36,7 +36,7 @@ def _pack(*forms):
             meta.append(None)
         else:
             tensors += [f.values, f.scales]
-            meta.append((f.rows, f.cols, f.square))
+            meta.append((f.rows, f.cols))
     return tensors, meta
 
 
@@ -64,8 +64,8 @@ class _Linear8(torch.autograd.Function):
             w8 = prepared
         x8t = None
         if rows:
-            x8 = _empty(rows, fin, False, x.device)
-            x8t = _empty(fin, rows, False, x.device) if need_w else None
+            x8 = _empty(rows, fin, x.device)
+            x8t = _empty(fin, rows, x.device) if need_w else None
             _run(x2, False, x8, x8t)
             y = block8.matmul(x8, w8, bias, x.dtype)
         else:
@@ -94,8 +94,8 @@ class _Linear8(torch.autograd.Function):
             return dx, dw, db, None, None
         g2 = block8._matrix(g.reshape(rows, fout), "linear8 backward")
         # one read of g: its rows for dx, its columns for dW, partial column sums for db
-        g8 = _empty(rows, fout, False, g.device) if need_x or not need_w else None
-        g8t = _empty(fout, rows, False, g.device) if need_w else None
+        g8 = _empty(rows, fout, g.device) if need_x or not need_w else None
+        g8t = _empty(fout, rows, g.device) if need_w else None
         partial = torch.empty((block8._blocks(rows), fout), dtype=torch.float32, device=g.device) if need_b else None
         _run(g2, False, g8, g8t, partial)
         if need_x:
@@ -120,8 +120,6 @@ def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Opti
         raise ValueError(f"linear8: at least one input feature is expected, got shape {tuple(input.shape)}")
     prepared = weight if isinstance(weight, Block8) else None
     if prepared is not None:
-        if not prepared.square:
-            raise ValueError("linear8: a prepared weight comes in 128 x 128 blocks (block8.quantize_weight)")
         if input.requires_grad and torch.is_grad_enabled() and prepared.transposed is None:
             raise ValueError("linear8: the input's gradient needs the weight's transposed form: block8.quantize_weight(w, transposed=True)")
         fout, fin, device = prepared.rows, prepared.cols, prepared.device

@@ -429,29 +429,28 @@ int hapx_layer_norm_backward_add(const void* x, const void* dy, const void* gamm
  * operators that keep their input for the backward pass in 8 bits.
  *
  * A matrix of rows x cols is held as e4m3 bytes, `ld` bytes from row to row (base and ld multiples of 16), with one
- * float32 scale per block of 128 columns of a row, at scale[(c / 128) * ld_scale + r], or per 128 x 128 tile
- * ("square"), at scale[(c / 128) * ld_scale + r / 128].  value = byte * scale; the scale is 2^e with the smallest
- * e >= -126 for which the block's largest finite magnitude is at most 448 * 2^e (1 for a block of zeros); infinities
- * and NaN become NaN.
+ * power-of-two scale per block of 128 columns of a row: value = byte * 2^e with the smallest e >= -126 for which the
+ * block's largest finite magnitude is at most 448 * 2^e (0 for a block of zeros); infinities and NaN become NaN.  The
+ * scales are bytes e + 127, scale_bytes(rows, cols) of them (16-byte aligned): the scale of row r and block kb = c / 128 is byte
+ *     ((kb / 4) * ceil(rows / 128) + r / 128) * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + kb % 4.
  *
  *   quantize: x (rows x cols of `dtype`, ldx elements from row to row) -> q / s as it stands and / or qt / st
- *             transposed (cols x rows, blocks along x's rows), in one read; either pair may be null.  `colsum` (may be
- *             null): ceil(rows / 128) x cols floats, the column sums of every 128 rows of x.
- *   colsum_join: out[c] = sum of `partial` over the ceil(rows / 128) row groups, in their order.
+ *             transposed (cols x rows, blocks along x's rows), in one read; either pair may be null.  square: every
+ *             128 x 128 tile of x shares one scale, so that q and qt hold the same values.  `colsum` (may be null):
+ *             ceil(rows / 128) x cols floats, the column sums of every 128 rows of x.
+ *   colsum_join: out[c] = sum of `partial` over the ceil(rows / 128) row groups, in a fixed order.
  *   dequantize: the values back, contiguous.
- *   matmul: d[m, n] (contiguous) = a (m x k, 1 x 128 blocks) * b (n x k)^T + bias; sums in float32, one rounding.
- *             The scales of 1 x 128 blocks of b need a 16-byte aligned base and a pitch that is a multiple of 4.
- *             bias: n values of out_dtype or null.  `workspace`: matmul_workspace(m, n, k) bytes (may be 0) on the
- *             current device, 16-byte aligned, free to be reused when the call's kernels have run. */
-int hapx_block8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int square, void* q, int64_t ldq, float* s,
-                         int64_t lds, void* qt, int64_t ldqt, float* st, int64_t ldst, float* colsum, hapx_stream stream);
+ *   matmul: d[m, n] (contiguous) = a (m x k) * b (n x k)^T + bias; sums in float32, one rounding.  bias: n values of
+ *             out_dtype or null.  `workspace`: matmul_workspace(m, n, k) bytes (may be 0) on the current device,
+ *             16-byte aligned, free to be reused when the call's kernels have run. */
+int64_t hapx_block8_scale_bytes(int64_t rows, int64_t cols);
+int hapx_block8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int square, void* q, int64_t ldq, void* s,
+                         void* qt, int64_t ldqt, void* st, float* colsum, hapx_stream stream);
 int hapx_block8_colsum_join(void* out, int dtype, const float* partial, int64_t rows, int64_t cols, hapx_stream stream);
-int hapx_block8_dequantize(void* out, int dtype, const void* q, int64_t ldq, const float* s, int64_t lds, int square, int64_t rows,
-                           int64_t cols, hapx_stream stream);
+int hapx_block8_dequantize(void* out, int dtype, const void* q, int64_t ldq, const void* s, int64_t rows, int64_t cols, hapx_stream stream);
 int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k);
-int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const float* a_scale, int64_t lda_scale, const void* b, int64_t ldb,
-                       const float* b_scale, int64_t ldb_scale, int b_square, const void* bias, int64_t m, int64_t n, int64_t k,
-                       void* workspace, int64_t workspace_bytes, hapx_stream stream);
+int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const void* a_scale, const void* b, int64_t ldb, const void* b_scale,
+                       const void* bias, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, hapx_stream stream);
 /* hapx_act_dropout and its backward pass with less kept in between.  act 2 (gelu): `saved` holds the input as e4m3
  * bytes (n rounded up to 4, 16-byte aligned), `scales` one float per 128 consecutive elements.  act 1 (relu): `saved`
  * holds one bit per element, active and kept (bit i % 8 of byte i / 8), `scales` is not used.  saved null: nothing is

@@ -44,16 +44,25 @@ def test_quantize_with_nothing_to_do_is_refused():
         block8.quantize(torch.ones(2, 8), rows=False)
 
 
-def _block8(rows, cols, square=False):
-    step = 128 if square else 1
+def _block8(rows, cols):
     return block8.Block8(torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.uint8).view(torch.float8_e4m3fn),
-                         torch.ones(-(-cols // 128), -(-rows // step)), rows, cols, square)
+                         torch.full((-(-cols // 512) * -(-rows // 128) * 512,), 127, dtype=torch.uint8), rows, cols)
+
+
+def test_scale_matrix_decodes_the_order_of_the_tensor_cores():
+    b = _block8(300, 700)                                               # 3 groups of rows, 6 blocks of columns in 2 groups of 4
+    assert b.scales.numel() == N.lib.hapx_block8_scale_bytes(300, 700) == 2 * 3 * 512 and b.nbytes == 300 * 704 + 3072
+    for r, kb in ((0, 0), (31, 1), (32, 2), (127, 3), (128, 4), (299, 5), (170, 3)):
+        b.scales.fill_(127)
+        b.scales[((kb // 4) * 3 + r // 128) * 512 + (r % 32) * 16 + (r // 32 % 4) * 4 + kb % 4] = 130
+        want = torch.ones(300, 6)
+        want[r, kb] = 8.0
+        assert torch.equal(b.scale_matrix(), want)
+    assert _block8(0, 40).scale_matrix().shape == (0, 1) and N.lib.hapx_block8_scale_bytes(0, 40) == 0
 
 
 def test_matmul_refusals():
     a, b = _block8(3, 40), _block8(5, 40)
-    with pytest.raises(ValueError, match="1 x 128"):
-        block8.matmul(_block8(3, 40, True), b)
     with pytest.raises(ValueError, match="contraction"):
         block8.matmul(a, _block8(5, 41))
     with pytest.raises(TypeError, match="output"):
@@ -68,34 +77,34 @@ def test_c_entries_refuse_before_any_launch():
     """Pointers below are never dereferenced: every call is answered by the checks of its arguments."""
     p, q = 4096, 4097                                                    # a 16-byte aligned and an odd address
     quant = N.lib.hapx_block8_quantize
-    assert quant(p, N.F16, 4, 8, 8, 0, p, 16, p, 4, None, 0, None, 0, None, None) == N.ERR_DTYPE
-    assert quant(p, N.BF16, 4, 8, 7, 0, p, 16, p, 4, None, 0, None, 0, None, None) == N.ERR_EXTENT      # pitch below the row
-    assert quant(p, N.BF16, -1, 8, 8, 0, p, 16, p, 4, None, 0, None, 0, None, None) == N.ERR_EXTENT
-    assert quant(p, N.BF16, 4, 8, 8, 0, p, 8, p, 4, None, 0, None, 0, None, None) == N.ERR_EXTENT       # pitch not of 16 bytes
-    assert quant(p, N.BF16, 4, 8, 8, 0, q, 16, p, 4, None, 0, None, 0, None, None) == N.ERR_EXTENT
-    assert quant(p, N.BF16, 4, 8, 8, 0, p, 16, p, 3, None, 0, None, 0, None, None) == N.ERR_EXTENT      # too few scales
-    assert quant(p, N.BF16, 4, 8, 8, 0, None, 0, None, 0, p, 16, p, 7, None, None) == N.ERR_EXTENT
-    assert quant(p, N.BF16, 4, 8, 8, 0, None, 0, None, 0, None, 0, None, 0, None, None) == N.ERR_ARGUMENT
-    assert quant(p, N.BF16, 4, 8, 8, 0, p, 16, None, 4, None, 0, None, 0, None, None) == N.ERR_ARGUMENT
-    assert quant(None, N.BF16, 4, 8, 8, 0, p, 16, p, 4, None, 0, None, 0, None, None) == N.ERR_ARGUMENT
-    assert quant(p, N.BF16, 1 << 40, 1 << 40, 1 << 40, 0, p, 1 << 40, p, 1 << 40, None, 0, None, 0, None, None) == N.ERR_EXTENT
-    assert quant(None, N.BF16, 0, 8, 8, 0, None, 0, None, 0, None, 0, None, 0, None, None) == N.OK      # an empty matrix
-    assert N.lib.hapx_block8_dequantize(p, N.F64, p, 16, p, 4, 0, 4, 8, None) == N.ERR_DTYPE
-    assert N.lib.hapx_block8_dequantize(p, N.F32, p, 4, p, 4, 0, 4, 8, None) == N.ERR_EXTENT
-    assert N.lib.hapx_block8_dequantize(None, N.F32, p, 16, p, 4, 0, 4, 8, None) == N.ERR_ARGUMENT
+    assert quant(p, N.F16, 4, 8, 8, 0, p, 16, p, None, 0, None, None, None) == N.ERR_DTYPE
+    assert quant(p, N.BF16, 4, 8, 7, 0, p, 16, p, None, 0, None, None, None) == N.ERR_EXTENT      # pitch below the row
+    assert quant(p, N.BF16, -1, 8, 8, 0, p, 16, p, None, 0, None, None, None) == N.ERR_EXTENT
+    assert quant(p, N.BF16, 4, 8, 8, 0, p, 8, p, None, 0, None, None, None) == N.ERR_EXTENT       # pitch not of 16 bytes
+    assert quant(p, N.BF16, 4, 8, 8, 0, q, 16, p, None, 0, None, None, None) == N.ERR_EXTENT
+    assert quant(p, N.BF16, 40, 8, 8, 0, None, 0, None, p, 32, p, None, None) == N.ERR_EXTENT     # pitch below the column
+    assert quant(p, N.BF16, 4, 8, 8, 0, None, 0, None, q, 16, p, None, None) == N.ERR_EXTENT
+    assert quant(p, N.BF16, 4, 8, 8, 0, None, 0, None, None, 0, None, None, None) == N.ERR_ARGUMENT
+    assert quant(p, N.BF16, 4, 8, 8, 0, p, 16, None, None, 0, None, None, None) == N.ERR_ARGUMENT
+    assert quant(None, N.BF16, 4, 8, 8, 0, p, 16, p, None, 0, None, None, None) == N.ERR_ARGUMENT
+    assert quant(p, N.BF16, 1 << 40, 1 << 40, 1 << 40, 0, p, 1 << 40, p, None, 0, None, None, None) == N.ERR_EXTENT
+    assert quant(None, N.BF16, 0, 8, 8, 0, None, 0, None, None, 0, None, None, None) == N.OK      # an empty matrix
+    assert N.lib.hapx_block8_dequantize(p, N.F64, p, 16, p, 4, 8, None) == N.ERR_DTYPE
+    assert N.lib.hapx_block8_dequantize(p, N.F32, p, 4, p, 4, 8, None) == N.ERR_EXTENT
+    assert N.lib.hapx_block8_dequantize(None, N.F32, p, 16, p, 4, 8, None) == N.ERR_ARGUMENT
     assert N.lib.hapx_block8_colsum_join(p, N.F16, p, 4, 8, None) == N.ERR_DTYPE
     assert N.lib.hapx_block8_colsum_join(None, N.F32, p, 4, 8, None) == N.ERR_ARGUMENT
     mm = N.lib.hapx_block8_matmul
-    assert mm(p, N.F16, p, 16, p, 4, p, 16, p, 4, 0, None, 4, 4, 8, None, 0, None) == N.ERR_DTYPE
-    assert mm(p, N.BF16, p, 16, p, 4, p, 16, p, 4, 0, None, 4, 4, -8, None, 0, None) == N.ERR_EXTENT
-    assert mm(p, N.BF16, p, 16, p, 4, p, 16, p, 4, 0, None, 1 << 31, 4, 8, None, 0, None) == N.ERR_EXTENT
-    assert mm(p, N.BF16, p, 16, p, 4, p, 12, p, 4, 0, None, 4, 4, 8, None, 0, None) == N.ERR_EXTENT
-    assert mm(p, N.BF16, q, 16, p, 4, p, 16, p, 4, 0, None, 4, 4, 8, None, 0, None) == N.ERR_EXTENT
-    assert mm(p, N.BF16, p, 16, p, 3, p, 16, p, 4, 0, None, 4, 4, 8, None, 0, None) == N.ERR_EXTENT
-    assert mm(p, N.BF16, p, 16, p, 4, p, 16, p, 3, 0, None, 4, 4, 8, None, 0, None) == N.ERR_EXTENT
-    assert mm(None, N.BF16, p, 16, p, 4, p, 16, p, 4, 0, None, 4, 4, 8, None, 0, None) == N.ERR_ARGUMENT
-    assert mm(p, N.BF16, None, 16, p, 4, p, 16, p, 4, 0, None, 4, 4, 8, None, 0, None) == N.ERR_ARGUMENT
-    assert mm(None, N.BF16, None, 0, None, 0, None, 0, None, 0, 0, None, 0, 4, 8, None, 0, None) == N.OK
+    assert mm(p, N.F16, p, 16, p, p, 16, p, None, 4, 4, 8, None, 0, None) == N.ERR_DTYPE
+    assert mm(p, N.BF16, p, 16, p, p, 16, p, None, 4, 4, -8, None, 0, None) == N.ERR_EXTENT
+    assert mm(p, N.BF16, p, 16, p, p, 16, p, None, 4, 4, 0, None, 0, None) == N.ERR_EXTENT
+    assert mm(p, N.BF16, p, 16, p, p, 16, p, None, 1 << 31, 4, 8, None, 0, None) == N.ERR_EXTENT
+    assert mm(p, N.BF16, p, 16, p, p, 12, p, None, 4, 4, 8, None, 0, None) == N.ERR_EXTENT
+    assert mm(p, N.BF16, q, 16, p, p, 16, p, None, 4, 4, 8, None, 0, None) == N.ERR_EXTENT
+    assert mm(p, N.BF16, p, 16, q, p, 16, p, None, 4, 4, 8, None, 0, None) == N.ERR_EXTENT
+    assert mm(None, N.BF16, p, 16, p, p, 16, p, None, 4, 4, 8, None, 0, None) == N.ERR_ARGUMENT
+    assert mm(p, N.BF16, None, 16, p, p, 16, p, None, 4, 4, 8, None, 0, None) == N.ERR_ARGUMENT
+    assert mm(None, N.BF16, None, 0, None, None, 0, None, None, 0, 4, 8, None, 0, None) == N.OK
     act = N.lib.hapx_act_dropout8
     assert act(p, p, p, p, N.F16, 8, 2, 0.0, 0, None) == N.ERR_DTYPE
     assert act(p, p, p, p, N.F32, -1, 2, 0.0, 0, None) == N.ERR_EXTENT

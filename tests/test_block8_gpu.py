@@ -34,6 +34,11 @@ def sum_slack(magnitudes, n):
     return magnitudes * (n + 4) * 2.0 ** -23
 
 
+def per_row(scales, rows):
+    """The oracle's scales [column block, row or row block] as (rows, column blocks)."""
+    return (scales if scales.shape[1] == rows else scales.repeat_interleave(128, 1)[:, :rows]).t()
+
+
 # ---- quantiser ----------------------------------------------------------------------------------------
 SHAPES = [(1, 1), (1, 128), (3, 129), (128, 128), (129, 127), (300, 515), (17, 1000), (257, 64), (1000, 33)]
 
@@ -50,7 +55,7 @@ def test_quantize_is_exact(dtype, shape):
         values, scales = want
         assert torch.equal(got.dequantize(F32).cpu().double(), values)
         assert torch.equal(got.dequantize(BF).cpu().double(), values)
-        assert torch.equal(got.scales.cpu().double()[:, :scales.shape[1]], scales)
+        assert torch.equal(got.scale_matrix().cpu().double(), per_row(scales, got.rows))
     # one form at a time gives the same
     assert torch.equal(block8.quantize(x.to(DEV)).dequantize(), rows.dequantize())
     assert torch.equal(block8.quantize(x.to(DEV), rows=False, columns=True).dequantize(), cols.dequantize())
@@ -74,7 +79,7 @@ def test_quantize_special_values():
         # dequantize rounds to float32: 3.3e38 / 2^120 = 248.3 is nearest to 256 on its grid (steps of 16), and 256 * 2^120 = 2^128
         # is above float32's largest number, an infinity there
         torch.testing.assert_close(got.dequantize().cpu(), values.float(), rtol=0, atol=0, equal_nan=True)
-        assert torch.equal(got.scales.cpu().double()[:, :scales.shape[1]], scales)
+        assert torch.equal(got.scale_matrix().cpu().double(), per_row(scales, got.rows))
     assert torch.equal(torch.isnan(rows.dequantize().cpu()), ~torch.isfinite(x))
 
 
@@ -235,7 +240,7 @@ def test_linear8_refusals():
     for args, err in (((x.half(), w.half()), TypeError), ((x, w.to(BF)), TypeError), ((x, w[:, :7]), ValueError), ((x, w, w[0]), ValueError),
                       ((x, w, torch.ones(5, device=DEV, dtype=BF)), TypeError), ((x, w, torch.ones(5)), ValueError), ((x, w.cpu()), ValueError),
                       ((x, w[0]), ValueError), ((x[:, :0], w[:, :0]), ValueError), ((x, w[:0]), ValueError), ((x[0, 0], w), ValueError),
-                      ((x, block8.quantize(w)), ValueError)):
+                      ((x, block8.quantize(w[:, :7])), ValueError)):
         with pytest.raises(err):
             hap_b200.linear8(*args)
     for bad in (x[0], x[:, :0]):
@@ -269,8 +274,8 @@ def test_what_is_kept_for_the_backward_pass():
     rows, fin, fout = 512, 1024, 256
     x, w = leaf(torch.randn(rows, fin).to(BF)), torch.randn(fout, fin).to(BF).to(DEV)
     n = rows * fin
-    assert saved_bytes(lambda: hap_b200.linear8(x.detach(), leaf(w))) == n + 4 * n // 128                      # the input, 8 bits
-    assert saved_bytes(lambda: hap_b200.linear8(x, w)) == fin * fout + 4 * (fout // 128) * (fin // 128)      # the weight
+    assert saved_bytes(lambda: hap_b200.linear8(x.detach(), leaf(w))) == n + n // 128                          # the input, 8 bits
+    assert saved_bytes(lambda: hap_b200.linear8(x, w)) == fin * fout + fin * 4                  # the weight: out_features 256 are two blocks of four
     assert saved_bytes(lambda: hap_b200.dropout.act_dropout8(x, "gelu", 0.1)) == n + 4 * n // 128
     assert saved_bytes(lambda: hap_b200.dropout.act_dropout8(x, "relu", 0.1)) == n // 8
     assert saved_bytes(lambda: hap_b200.layer_norm8(x, (fin,))) == n + 4 * n // 128 + 8 * rows
