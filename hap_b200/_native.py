@@ -92,6 +92,10 @@ SIGNATURES = {
     "hapx_block8_colsum_join": (_int, [_vp, _int, _vp, _i64, _i64, _vp]),
     "hapx_block8_matmul_workspace": (_i64, [_i64, _i64, _i64]),
     "hapx_block8_matmul": (_int, [_vp, _int, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "hapx_linear8_forward_workspace": (_i64, [_i64, _i64, _i64, _int, _int]),
+    "hapx_linear8_forward": (_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "hapx_linear8_backward_workspace": (_i64, [_i64, _i64, _i64, _int, _int, _int]),
+    "hapx_linear8_backward": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "hapx_act_dropout8": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _int, _dbl, _u64, _vp]),
     "hapx_act_dropout8_backward": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _int, _dbl, _u64, _vp]),
     "hapx_layer_norm8_forward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _int, _i64, _i64, _dbl, _vp]),

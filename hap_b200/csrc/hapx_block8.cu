@@ -13,14 +13,7 @@
 namespace hapx {
 namespace block8 {
 
-struct QuantParams {
-  const void* x;
-  long long rows, cols, ldx;
-  unsigned char* q;  long long ldq;  unsigned char* s;     // as it stands: rows x cols
-  unsigned char* qt; long long ldqt; unsigned char* st;    // transposed: cols x rows
-  float* colsum;                                           // [row tile][cols] partial column sums, or null
-  int row_tiles, col_tiles;
-};
+struct QuantJobs { QuantJob job[2]; long long tiles0, tiles; };     // tiles of the first matrix, of both
 
 // Four consecutive elements as they are in memory.
 template <typename T> struct Raw4;
@@ -88,19 +81,22 @@ template <> struct Max4<float> {
   }
 };
 
-// SQUARE: one scale per 128 x 128 tile, stored for each of its rows (and columns).
+// square: one scale per 128 x 128 tile, stored for each of its rows (and columns).
 //
 // The elements stay in their own type in registers (32 of them for bfloat16), so that three blocks fit an SM; the
 // transposed bytes go through shared memory and leave as whole 128-byte rows.
-template <typename T, bool SQUARE>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const QuantParams p) {
+template <typename T>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const __grid_constant__ QuantJobs jobs) {
   __shared__ float s_col[8][kBlock];
   __shared__ uint4 s_t[kBlock * 8];
   __shared__ int s_odd;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const T* x = static_cast<const T*>(p.x);
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0 && (p.ldx & 3) == 0;
-  for (long long tile = blockIdx.x; tile < (long long)p.row_tiles * p.col_tiles; tile += gridDim.x) {
+  for (long long both = blockIdx.x; both < jobs.tiles; both += gridDim.x) {
+    const QuantJob& p = jobs.job[both >= jobs.tiles0];
+    const long long tile = both >= jobs.tiles0 ? both - jobs.tiles0 : both;
+    const T* x = static_cast<const T*>(p.x);
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0 && (p.ldx & 3) == 0;
+    const bool square = p.square != 0;
     const int rt = (int)(tile / p.col_tiles), ct = (int)(tile % p.col_tiles);
     const long long r0 = (long long)rt * kBlock + 16 * warp, c0 = (long long)ct * kBlock + 4 * lane;
     const int valid = (int)max(0ll, min(4ll, p.cols - c0)), live = (int)max(0ll, min(16ll, p.rows - r0));   // columns, rows of this thread
@@ -169,7 +165,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(c
       cm.get(colbig);
     }
     int ecol[4];
-    if (SQUARE) {
+    if (square) {
       const float mine = warp_max(fmaxf(fmaxf(colbig[0], colbig[1]), fmaxf(colbig[2], colbig[3])));
       if (lane == 0) s_col[0][warp] = mine;
       __syncthreads();
@@ -202,15 +198,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(c
       unsigned char* dst = p.q + r0 * p.ldq + c0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int e = SQUARE ? ecol[0] : scale_exponent(warp_max(Max4<T>::of(v[i])));
-        if (!SQUARE && lane == i) mine = e;
+        const int e = square ? ecol[0] : scale_exponent(warp_max(Max4<T>::of(v[i])));
+        if (!square && lane == i) mine = e;
         const float inv = pow2(-e);
         float f[4];
         v[i].get(f);
         if (i < live && valid > 0)     // the pitch is a multiple of 16: a partial group of 4 stays inside it
           *reinterpret_cast<unsigned*>(dst + i * p.ldq) = pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
       }
-      if (!SQUARE && lane < live) p.s[scale_at(r0 + lane, ct, p.row_tiles)] = (unsigned char)(mine + 127);
+      if (!square && lane < live) p.s[scale_at(r0 + lane, ct, p.row_tiles)] = (unsigned char)(mine + 127);
     }
     if (p.qt) {
 #pragma unroll
@@ -262,10 +258,22 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned char* __
   }
 }
 
-static int sms(int* out) {
-  int device = 0;
-  HAPX_CUDA(cudaGetDevice(&device));
-  HAPX_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, device));
+int quantize(QuantJob* job, int n_jobs, int dtype, cudaStream_t stream) {
+  int n_sm = 0;
+  if (int e = sm_count(&n_sm)) return e;
+  QuantJobs jobs;
+  for (int i = 0; i < n_jobs; ++i) {
+    job[i].row_tiles = (int)((job[i].rows + kBlock - 1) / kBlock);
+    job[i].col_tiles = (int)((job[i].cols + kBlock - 1) / kBlock);
+    jobs.job[i] = job[i];
+    jobs.tiles = (i ? jobs.tiles0 : 0) + (long long)job[i].row_tiles * job[i].col_tiles;
+    if (i == 0) jobs.tiles0 = jobs.tiles;
+  }
+  const int grid = (int)std::min<long long>(jobs.tiles, (long long)n_sm * 16);
+  if (dtype == HAPX_BF16) quantize_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(jobs);
+  else quantize_kernel<float><<<grid, 256, 0, stream>>>(jobs);
+  HAPX_CUDA(cudaGetLastError());
+  count_launch();
   return HAPX_OK;
 }
 
@@ -291,22 +299,12 @@ int hapx_block8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, i
     return fail(HAPX_ERR_EXTENT, "block8_quantize: values need a 16-byte aligned base and pitch, and a pitch that covers a row");
   if (qt && (ldqt % 16 != 0 || ldqt < rows || (reinterpret_cast<uintptr_t>(qt) & 15u)))
     return fail(HAPX_ERR_EXTENT, "block8_quantize: transposed values need a 16-byte aligned base and pitch, and a pitch that covers a column");
-  int n_sm = 0;
-  if (int e = sms(&n_sm)) return e;
-  QuantParams p = {x, rows, cols, ldx, static_cast<unsigned char*>(q), ldq, static_cast<unsigned char*>(s), static_cast<unsigned char*>(qt), ldqt,
-                   static_cast<unsigned char*>(st), colsum, (int)row_tiles, (int)col_tiles};
-  const int grid = (int)std::min<int64_t>(row_tiles * col_tiles, (int64_t)n_sm * 16);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (dtype == HAPX_BF16) {
-    if (square) quantize_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(p);
-    else quantize_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(p);
-  } else {
-    if (square) quantize_kernel<float, true><<<grid, 256, 0, stream>>>(p);
-    else quantize_kernel<float, false><<<grid, 256, 0, stream>>>(p);
-  }
-  HAPX_CUDA(cudaGetLastError());
-  count_launch();
-  return HAPX_OK;
+  QuantJob job;
+  job.x = x; job.rows = rows; job.cols = cols; job.ldx = ldx; job.square = square;
+  job.q = static_cast<unsigned char*>(q); job.ldq = ldq; job.s = static_cast<unsigned char*>(s);
+  job.qt = static_cast<unsigned char*>(qt); job.ldqt = ldqt; job.st = static_cast<unsigned char*>(st);
+  job.colsum = colsum;
+  return quantize(&job, 1, dtype, static_cast<cudaStream_t>(stream_));
 }
 
 int hapx_block8_colsum_join(void* out, int dtype, const float* partial, int64_t rows, int64_t cols, hapx_stream stream_) {
@@ -330,7 +328,7 @@ int hapx_block8_dequantize(void* out, int dtype, const void* q, int64_t ldq, con
   if (rows == 0 || cols == 0) return HAPX_OK;
   if (!out || !q || !s) return fail(HAPX_ERR_ARGUMENT, "block8_dequantize: null pointer");
   int n_sm = 0;
-  if (int e = sms(&n_sm)) return e;
+  if (int e = sm_count(&n_sm)) return e;
   const int grid = (int)std::min<int64_t>((rows * cols + 255) / 256, (int64_t)n_sm * 16);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const unsigned char *v = static_cast<const unsigned char*>(q), *sc = static_cast<const unsigned char*>(s);

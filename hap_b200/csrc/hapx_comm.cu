@@ -23,6 +23,19 @@ int fail(int code, const std::string& msg) {
 }
 void count_launch(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
+int sm_count(int* out) {
+  static std::atomic<int> known[64];
+  int device = 0;
+  HAPX_CUDA(cudaGetDevice(&device));
+  int n = device >= 0 && device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    HAPX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
+    if (device >= 0 && device < 64) known[device].store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return HAPX_OK;
+}
+
 static int check_sizes(int world, size_t heap_bytes, size_t stage_bytes) {
   if (world < 1 || world > HAPX_MAX_WORLD)
     return fail(HAPX_ERR_ARGUMENT, "world must be in [1, " + std::to_string(HAPX_MAX_WORLD) + "]");

@@ -443,13 +443,6 @@ static Plan plan_of(long long M, long long N, long long K, int sm_count) {
   return pl;
 }
 
-static int sm_count_of(int* out) {
-  int device = 0;
-  HAPX_CUDA(cudaGetDevice(&device));
-  HAPX_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, device));
-  return HAPX_OK;
-}
-
 template <bool PAIR>
 static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmSA, const CUtensorMap& tmSB, const CUtensorMap& tmD,
                   const Params& p, int sm_count, cudaStream_t stream) {
@@ -507,11 +500,15 @@ static int make_scale_map(CUtensorMap* map, const void* ptr, long long rows, int
   return HAPX_OK;
 }
 
-static int run(void* d, int out_f32, const void* a, long long lda, const void* as, const void* b, long long ldb, const void* bs, const void* bias,
-               long long M, long long N, long long K, void* workspace, cudaStream_t stream) {
+long long workspace_bytes(long long m, long long n, long long k, int sm_count) {
+  const Plan pl = plan_of(m, n, k, sm_count);
+  return pl.splits > 1 ? pl.splits * pl.m_pad * pl.n_pad * 4 : 0;
+}
+
+int run(const Product& pr, int sm_count, cudaStream_t stream) {
   unsigned* error = nullptr;
-  int sm_count = 0;
-  if (int e = gemm::error_word(&error, &sm_count)) return e;
+  if (int e = gemm::error_word(&error, nullptr)) return e;
+  const long long M = pr.m, N = pr.n, K = pr.k;
   const Plan pl = plan_of(M, N, K, sm_count);
   Params p = Params();
   p.M = (int)M; p.N = (int)N; p.k_blocks = (int)((K + BK - 1) / BK);
@@ -520,17 +517,17 @@ static int run(void* d, int out_f32, const void* a, long long lda, const void* a
   const int bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true>::BN : Cfg<false>::BN;
   p.m_tiles = (p.M + bm - 1) / bm; p.n_tiles = (p.N + bn - 1) / bn;
   long long out_rows = M;
-  if (pl.splits > 1) { p.D = workspace; p.ldd = pl.n_pad; p.out_f32 = 1; p.bias = nullptr; out_rows = pl.splits * pl.m_pad; }
-  else { p.D = d; p.ldd = N; p.out_f32 = out_f32; p.bias = bias; }
+  if (pl.splits > 1) { p.D = pr.workspace; p.ldd = pl.n_pad; p.out_f32 = 1; p.bias = nullptr; out_rows = pl.splits * pl.m_pad; }
+  else { p.D = pr.d; p.ldd = N; p.out_f32 = pr.out_f32; p.bias = pr.bias; }
   p.bias_vec = (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
   const int es = p.out_f32 ? 4 : 2;
   CUtensorMap tmA, tmB, tmSA, tmSB, tmD;
   std::memset(&tmD, 0, sizeof(tmD));
-  if (int e = make_map(&tmA, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
-  if (int e = make_map(&tmB, b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, ldb, BK, pl.pair ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
+  if (int e = make_map(&tmA, pr.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, pr.lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
+  if (int e = make_map(&tmB, pr.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, pr.ldb, BK, pl.pair ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
-  if (int e = make_scale_map(&tmSA, as, M, p.k_blocks, 1)) return e;
-  if (int e = make_scale_map(&tmSB, bs, N, p.k_blocks, pl.pair ? Cfg<true>::B_ATOMS : Cfg<false>::B_ATOMS)) return e;
+  if (int e = make_scale_map(&tmSA, pr.a_scale, M, p.k_blocks, 1)) return e;
+  if (int e = make_scale_map(&tmSB, pr.b_scale, N, p.k_blocks, pl.pair ? Cfg<true>::B_ATOMS : Cfg<false>::B_ATOMS)) return e;
   p.tma_store = (reinterpret_cast<uintptr_t>(p.D) & 15u) == 0 && (p.ldd * es) % 16 == 0;
   if (p.tma_store)
     if (int e = make_map(&tmD, p.D, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, pl.splits > 1 ? pl.n_pad : N,
@@ -538,10 +535,10 @@ static int run(void* d, int out_f32, const void* a, long long lda, const void* a
   if (int e = pl.pair ? launch<true>(tmA, tmB, tmSA, tmSB, tmD, p, sm_count, stream) : launch<false>(tmA, tmB, tmSA, tmSB, tmD, p, sm_count, stream)) return e;
   if (pl.splits > 1) {
     const int grid = (int)std::min<long long>((M * (pl.n_pad / 4) + 255) / 256, (long long)sm_count * 8);
-    const float* ws = static_cast<const float*>(workspace);
-    if (out_f32) gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, M, p.N, pl.m_pad, pl.n_pad, static_cast<const float*>(bias), static_cast<float*>(d));
-    else gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, M, p.N, pl.m_pad, pl.n_pad, static_cast<const __nv_bfloat16*>(bias),
-                                                     static_cast<__nv_bfloat16*>(d));
+    const float* ws = static_cast<const float*>(pr.workspace);
+    if (pr.out_f32) gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, M, p.N, pl.m_pad, pl.n_pad, static_cast<const float*>(pr.bias), static_cast<float*>(pr.d));
+    else gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, M, p.N, pl.m_pad, pl.n_pad, static_cast<const __nv_bfloat16*>(pr.bias),
+                                                     static_cast<__nv_bfloat16*>(pr.d));
     HAPX_CUDA(cudaGetLastError());
     count_launch();
   }
@@ -557,10 +554,8 @@ extern "C" {
 
 int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0 || m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff) return 0;
-  int sm_count = 0;
-  if (gemm8::sm_count_of(&sm_count)) return 0;
-  const gemm8::Plan pl = gemm8::plan_of(m, n, k, sm_count);
-  return pl.splits > 1 ? (int64_t)pl.splits * pl.m_pad * pl.n_pad * 4 : 0;
+  int n_sm = 0;
+  return sm_count(&n_sm) ? 0 : gemm8::workspace_bytes(m, n, k, n_sm);
 }
 
 int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const void* a_scale, const void* b, int64_t ldb, const void* b_scale,
@@ -574,10 +569,15 @@ int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const
     return fail(HAPX_ERR_EXTENT, "block8_matmul: operands need a 16-byte aligned base and pitch, and a pitch that covers a row");
   if ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale)) & 15u)
     return fail(HAPX_ERR_EXTENT, "block8_matmul: the scales need a 16-byte aligned base");
-  const int64_t need = hapx_block8_matmul_workspace(m, n, k);
+  int n_sm = 0;
+  if (int e = sm_count(&n_sm)) return e;
+  const long long need = gemm8::workspace_bytes(m, n, k, n_sm);
   if (workspace_bytes < need || (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))))
     return fail(HAPX_ERR_ARGUMENT, "block8_matmul: the workspace must be 16-byte aligned and as large as hapx_block8_matmul_workspace says");
-  return gemm8::run(d, out_dtype == HAPX_F32, a, lda, a_scale, b, ldb, b_scale, bias, m, n, k, workspace, static_cast<cudaStream_t>(stream));
+  gemm8::Product pr;
+  pr.d = d; pr.out_f32 = out_dtype == HAPX_F32; pr.a = a; pr.lda = lda; pr.a_scale = a_scale; pr.b = b; pr.ldb = ldb; pr.b_scale = b_scale;
+  pr.bias = bias; pr.m = m; pr.n = n; pr.k = k; pr.workspace = workspace;
+  return gemm8::run(pr, n_sm, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -62,6 +62,39 @@ int gemm_bf16(const Operand& D, int out_f32, const Operand& A, const Operand& B,
               long long M, long long N, long long Kc, int batch_in, int batch_out, cudaStream_t stream);
 }  // namespace gemm
 
+namespace block8 {
+// One matrix to quantise; see hapx_block8_quantize for the fields.
+struct QuantJob {
+  const void* x = nullptr;
+  long long rows = 0, cols = 0, ldx = 0;
+  int square = 0;
+  unsigned char* q = nullptr;  long long ldq = 0;  unsigned char* s = nullptr;
+  unsigned char* qt = nullptr; long long ldqt = 0; unsigned char* st = nullptr;
+  float* colsum = nullptr;
+  int row_tiles = 0, col_tiles = 0;
+};
+// One or two matrices of one type in one launch (arguments checked by the callers).
+int quantize(QuantJob* jobs, int n_jobs, int dtype, cudaStream_t stream);
+}  // namespace block8
+
+namespace gemm8 {
+// d[m, n] = a b^T (+ bias); see hapx_block8_matmul.
+struct Product {
+  void* d = nullptr;
+  int out_f32 = 0;
+  const void* a = nullptr; long long lda = 0; const void* a_scale = nullptr;
+  const void* b = nullptr; long long ldb = 0; const void* b_scale = nullptr;
+  const void* bias = nullptr;
+  long long m = 0, n = 0, k = 0;
+  void* workspace = nullptr;
+};
+long long workspace_bytes(long long m, long long n, long long k, int sm_count);
+int run(const Product& p, int sm_count, cudaStream_t stream);
+}  // namespace gemm8
+
+// Multiprocessors of the current device (asked for once per device).
+int sm_count(int* out);
+
 }  // namespace hapx
 
 struct hapx_comm {

@@ -10,7 +10,10 @@
 //
 // x~ is x to half a step of 3 fraction bits; forward results are those of the operators that keep x.
 #include <algorithm>
+#include <mutex>
+#include <set>
 #include <string>
+#include <utility>
 
 #include "hapx_block8.h"
 #include "hapx_internal.h"
@@ -23,51 +26,119 @@ using namespace block8;
 
 enum Act { ACT_RELU = 1, ACT_GELU = 2 };
 
-// Phi(v) and its density's exponential.
-__device__ __forceinline__ float normal_cdf(float v) { return 0.5f * erfcf(-v * 0.70710678118654752f); }
-__device__ __forceinline__ float gelu_slope(float v) { return fmaf(v * 0.3989422804014327f, __expf(-0.5f * v * v), normal_cdf(v)); }
+// Phi(v) = erfc(-v / sqrt 2) / 2 and e = exp(-v^2 / 2).  erfc(z) = e^{-z^2} t P(t) for z >= 0 with t = 1 / (1 + 0.33 z): P is a
+// least-maximum fit of degree 7 to erfcx(z) / t over 0 <= z <= 9.3, relative error 8.2e-8, so the tail keeps its relative
+// accuracy (which y = v Phi(v) needs for negative v) and shares its exponential with the density.
+__device__ __forceinline__ float normal_cdf(float v, float& e) {
+  const float z = fabsf(v) * 0.70710678118654752f;
+  const float t = __fdividef(1.f, fmaf(0.33f, z, 1.f));
+  e = exp2f(v * v * -0.72134752044448170f);               // log2(e) / 2
+  float q = fmaf(-0.1359295927870348f, t, 0.4626916833556958f);
+  q = fmaf(q, t, -0.3554451549092876f);
+  q = fmaf(q, t, 0.41254758607072767f);
+  q = fmaf(q, t, 0.04500733930570897f);
+  q = fmaf(q, t, 0.20192486623134484f);
+  q = fmaf(q, t, 0.18283706989561532f);
+  q = fmaf(q, t, 0.1863661211613116f);
+  const float tail = 0.5f * q * t * e;
+  return v >= 0.f ? 1.f - tail : tail;
+}
 
-// One warp per run of 128 elements; lane l holds elements 4l .. 4l + 3 of it.
+// Eight consecutive elements; `vec`: p is aligned to 16 bytes.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, int valid, float (&f)[8]) {
+  if (vec && valid >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = j < valid ? to_f(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool vec, int valid, const float (&f)[8]) {
+  if (vec && valid >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      unsigned u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        u[i] = *reinterpret_cast<const unsigned*>(&h);
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+      *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < valid) p[j] = from_f<T>(f[j]);
+  }
+}
+
+// A thread holds eight consecutive elements (one evaluation of the generator), sixteen lanes a block of 128; a warp takes
+// kActUnroll pieces of 256 elements at a time, their loads in flight together.
+constexpr int kActUnroll = 2;
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ x, T* __restrict__ y, unsigned char* __restrict__ saved,
                                                           float* __restrict__ scales, long long n, unsigned threshold, float keep_scale,
                                                           const rng::State* st, unsigned long long call_id) {
   const int lane = threadIdx.x & 31;
-  const bool vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & (4 * sizeof(T) - 1)) == 0;
+  const bool vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0;
   rng::Key key = {0u, 0u, 0u, 0u};
   if (threshold) key = rng::make_key(st, call_id);
-  const long long runs = (n + kBlock - 1) / kBlock;
-  for (long long run = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); run < runs; run += (long long)gridDim.x * 8) {
-    const long long e0 = run * kBlock + 4 * lane;
-    const int valid = (int)max(0ll, min(4ll, n - e0));
-    float v[4], o[4];
-    load4(x + e0, vec, valid, v);
-    unsigned keep = 0xfu;
-    if (threshold) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold) >> (e0 & 4);
-    unsigned bits = 0;
+  constexpr int kPiece = 256 * kActUnroll;
+  const long long pieces = (n + kPiece - 1) / kPiece;
+  for (long long piece = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); piece < pieces; piece += (long long)gridDim.x * 8) {
+    float v[kActUnroll][8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float k = (keep >> j) & 1u ? keep_scale : 0.f;
-      if (ACT == ACT_RELU) {
-        o[j] = (v[j] <= 0.f ? 0.f : v[j]) * k;      // NaN passes
-        bits |= (v[j] > 0.f && k != 0.f && j < valid ? 1u : 0u) << j;
-      } else {
-        o[j] = v[j] * normal_cdf(v[j]) * k;
-      }
+    for (int u = 0; u < kActUnroll; ++u) {
+      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
+      load8(x + e0, vec, (int)max(0ll, min(8ll, n - e0)), v[u]);
     }
-    store4(y + e0, vec, valid, o);
-    if (!saved) continue;                           // nothing asks for a gradient
-    if (ACT == ACT_RELU) {
-      bits |= __shfl_down_sync(0xffffffffu, bits, 1) << 4;
-      if ((lane & 1) == 0 && valid > 0) saved[e0 >> 3] = (unsigned char)bits;
-    } else {
-      float big = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { v[j] = finite_or_nan(v[j]); big = fmaxf(big, fabsf(v[j])); }
-      const int e = scale_exponent(warp_max(big));
-      const float inv = pow2(-e);
-      if (lane == 0) scales[run] = pow2(e);
-      if (valid > 0) *reinterpret_cast<unsigned*>(saved + e0) = pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    for (int u = 0; u < kActUnroll; ++u) {
+      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
+      const int valid = (int)max(0ll, min(8ll, n - e0));
+      unsigned keep = 0xffu, bits = 0u;
+      if (threshold) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float k = (keep >> j) & 1u ? keep_scale : 0.f, w = v[u][j];
+        if (ACT == ACT_RELU) {
+          o[j] = (w <= 0.f ? 0.f : w) * k;          // NaN passes
+          bits |= (w > 0.f && j < valid ? 1u : 0u) << j;
+        } else {
+          float e;
+          o[j] = w * normal_cdf(w, e) * k;
+        }
+      }
+      store8(y + e0, vec, valid, o);
+      if (!saved) continue;                         // nothing asks for a gradient
+      if (ACT == ACT_RELU) {
+        if (valid > 0) saved[e0 >> 3] = (unsigned char)(bits & keep);
+      } else {
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { v[u][j] = finite_or_nan(v[u][j]); big = fmaxf(big, fabsf(v[u][j])); }
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+        const int e = scale_exponent(big);
+        const float inv = pow2(-e);
+        if ((lane & 15) == 0 && valid > 0) scales[e0 / kBlock] = pow2(e);
+        if (valid > 0)        // n rounded up to 8 bytes
+          *reinterpret_cast<uint2*>(saved + e0) = make_uint2(pack4(v[u][0] * inv, v[u][1] * inv, v[u][2] * inv, v[u][3] * inv),
+                                                             pack4(v[u][4] * inv, v[u][5] * inv, v[u][6] * inv, v[u][7] * inv));
+      }
     }
   }
 }
@@ -77,30 +148,50 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
                                                            const float* __restrict__ scales, T* __restrict__ dx, long long n,
                                                            unsigned threshold, float keep_scale, const rng::State* st,
                                                            unsigned long long call_id) {
-  const bool vec = ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx)) & (4 * sizeof(T) - 1)) == 0;
+  const int lane = threadIdx.x & 31;
+  const bool vec = ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx)) & 15u) == 0;
   rng::Key key = {0u, 0u, 0u, 0u};
   if (ACT == ACT_GELU && threshold) key = rng::make_key(st, call_id);
-  const long long groups = (n + 3) / 4;
-  for (long long g = (long long)blockIdx.x * 256 + threadIdx.x; g < groups; g += (long long)gridDim.x * 256) {
-    const long long e0 = 4 * g;
-    const int valid = (int)min(4ll, n - e0);
-    float d[4], o[4];
-    load4(dy + e0, vec, valid, d);
-    if (ACT == ACT_RELU) {
-      const unsigned bits = saved[e0 >> 3] >> (e0 & 4);
+  constexpr int kPiece = 256 * kActUnroll;
+  const long long pieces = (n + kPiece - 1) / kPiece;
+  for (long long piece = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); piece < pieces; piece += (long long)gridDim.x * 8) {
+    float d[kActUnroll][8], s[kActUnroll];
+    uint2 w[kActUnroll];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = (bits >> j) & 1u ? d[j] * keep_scale : 0.f;
-    } else {
-      unsigned keep = 0xfu;
-      if (threshold) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold) >> (e0 & 4);
-      const unsigned w = *reinterpret_cast<const unsigned*>(saved + e0);
-      const float s = scales[e0 / kBlock];
-      const float2 a = unpack2(w & 0xffffu), b = unpack2(w >> 16);
-      const float h[4] = {a.x * s, a.y * s, b.x * s, b.y * s};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = d[j] * ((keep >> j) & 1u ? keep_scale : 0.f) * gelu_slope(h[j]);
+    for (int u = 0; u < kActUnroll; ++u) {
+      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
+      const int valid = (int)max(0ll, min(8ll, n - e0));
+      load8(dy + e0, vec, valid, d[u]);
+      w[u] = make_uint2(0u, 0u);
+      s[u] = 0.f;
+      if (valid > 0) {
+        if (ACT == ACT_RELU) w[u].x = saved[e0 >> 3];
+        else { w[u] = *reinterpret_cast<const uint2*>(saved + e0); s[u] = scales[e0 / kBlock]; }
+      }
     }
-    store4(dx + e0, vec, valid, o);
+#pragma unroll
+    for (int u = 0; u < kActUnroll; ++u) {
+      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
+      const int valid = (int)max(0ll, min(8ll, n - e0));
+      float o[8];
+      if (ACT == ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = (w[u].x >> j) & 1u ? d[u][j] * keep_scale : 0.f;
+      } else {
+        unsigned keep = 0xffu;
+        if (threshold) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
+        const unsigned half[4] = {w[u].x & 0xffffu, w[u].x >> 16, w[u].y & 0xffffu, w[u].y >> 16};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float2 two = unpack2(half[j >> 1]);
+          const float h = (j & 1 ? two.y : two.x) * s[u];
+          float e;
+          const float cdf = normal_cdf(h, e);
+          o[j] = d[u][j] * ((keep >> j) & 1u ? keep_scale : 0.f) * fmaf(h * 0.3989422804014327f, e, cdf);
+        }
+      }
+      store8(dx + e0, vec, valid, o);
+    }
   }
 }
 
@@ -110,7 +201,168 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// One warp per row, blocks of 128 columns one after another; the row is read three times, twice from the caches.
+// ---- layer_norm ---------------------------------------------------------------------------------------
+// A row belongs to a team of W warps; warp w of it holds the blocks of 128 columns w, w + W, ... (NB of them at most) in
+// registers, lane l the columns 4l .. 4l + 3 of each.  A thread block has 8 / W teams.  Rows of up to 8192 columns are read
+// once; longer ones take the kernels below these.
+constexpr int kTeamColumns = 8192;
+
+// Sum over a team (`s`: one float per warp of the block, reused after the next call's other buffer).
+template <int W>
+__device__ __forceinline__ float team_sum(float v, float* s, int warp) {
+  v = warp_sum(v);
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 31) == 0) s[warp] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / W), "n"(32 * W) : "memory");
+    const int first = warp / W * W;
+    v = s[first];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v += s[first + i];
+  }
+  return v;
+}
+
+template <typename T, int W, int NB>
+__global__ void __launch_bounds__(256, NB <= 4 ? 4 : NB <= 6 ? 3 : 2) norm_forward_team_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b,
+                                                                                 T* __restrict__ y, float* __restrict__ mean_out,
+                                                                                 float* __restrict__ rstd_out, unsigned char* __restrict__ q,
+                                                                                 long long ldq, float* __restrict__ s, long long rows, int E, float eps) {
+  __shared__ float s_sum[2][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W, blocks = (E + kBlock - 1) / kBlock;
+  const bool vec = (E & 3) == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(w) |
+                                     reinterpret_cast<uintptr_t>(b)) & (4 * sizeof(T) - 1)) == 0;
+  const float inv_e = 1.f / (float)E;
+  for (long long row = (long long)blockIdx.x * (8 / W) + warp / W; row < rows; row += (long long)gridDim.x * (8 / W)) {
+    const T* xr = x + row * E;
+    float v[NB][4], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int c = (part + k * W) * kBlock + 4 * lane;
+      load4(xr + c, vec, max(0, min(4, E - c)), v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) sum += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
+    const float mean = team_sum<W>(sum, s_sum[0], warp) * inv_e;
+    float sq = 0.f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int valid = E - ((part + k * W) * kBlock + 4 * lane);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float d = j < valid ? v[k][j] - mean : 0.f;
+        sq = fmaf(d, d, sq);
+      }
+    }
+    const float rstd = rsqrtf(team_sum<W>(sq, s_sum[1], warp) * inv_e + eps);
+    float my_scale = 0.f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
+      float g[4] = {1.f, 1.f, 1.f, 1.f}, h[4] = {0.f, 0.f, 0.f, 0.f}, o[4], big = 0.f;
+      if (w) load4(w + c, vec, valid, g);
+      if (b) load4(b + c, vec, valid, h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[j] = fmaf((v[k][j] - mean) * rstd, g[j], h[j]);
+        v[k][j] = finite_or_nan(v[k][j]);
+        big = fmaxf(big, fabsf(v[k][j]));
+      }
+      store4(y + row * E + c, vec, valid, o);
+      if (q) {                                    // a gradient is asked for
+        const int e = scale_exponent(warp_max(big));
+        const float inv = pow2(-e);
+        if (lane == k) my_scale = pow2(e);
+        if (valid > 0) *reinterpret_cast<unsigned*>(q + row * ldq + c) = pack4(v[k][0] * inv, v[k][1] * inv, v[k][2] * inv, v[k][3] * inv);
+      }
+    }
+    if (q) {
+      if (lane < NB && part + lane * W < blocks) s[row * blocks + part + lane * W] = my_scale;
+      if (part == 0 && lane == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
+    }
+  }
+}
+
+// dx of the rows, and partial[block][0][c] = sum dy z, partial[block][1][c] = sum dy over the rows the thread block took.  The
+// running sums of a warp's columns lie in shared memory, owned by the warp (registers would leave a third of the warps).
+template <typename T, int W, int NB>
+__global__ void __launch_bounds__(256, 2) norm_backward_team_kernel(const unsigned char* __restrict__ q, long long ldq, const float* __restrict__ s,
+                                                                    const T* __restrict__ dy, const T* __restrict__ w,
+                                                                    const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                                                                    const T* __restrict__ add, T* __restrict__ dx, float* __restrict__ partial,
+                                                                    long long rows, int E) {
+  extern __shared__ float4 s_acc[];               // [warp][NB][2][32 lanes]
+  __shared__ float s_sum[2][2][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W, blocks = (E + kBlock - 1) / kBlock;
+  const bool vec = (E & 3) == 0 && ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(w) |
+                                     reinterpret_cast<uintptr_t>(add)) & (4 * sizeof(T) - 1)) == 0;
+  float4* acc = s_acc + (long long)warp * NB * 64 + lane;
+  if (partial) {
+#pragma unroll
+    for (int k = 0; k < 2 * NB; ++k) acc[32 * k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const float inv_e = 1.f / (float)E;
+  int flip = 0;
+  for (long long row = (long long)blockIdx.x * (8 / W) + warp / W; row < rows; row += (long long)gridDim.x * (8 / W), flip ^= 1) {
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    const float my_scale = lane < NB && part + lane * W < blocks ? s[row * blocks + part + lane * W] : 0.f;
+    float g[NB][4], z[NB][4], s1 = 0.f, s2 = 0.f;
+    unsigned raw[NB];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
+      load4(dy + row * E + c, vec, valid, g[k]);
+      raw[k] = valid > 0 ? *reinterpret_cast<const unsigned*>(q + row * ldq + c) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
+      const float sc = __shfl_sync(0xffffffffu, my_scale, k);
+      const float2 lo = unpack2(raw[k] & 0xffffu), hi = unpack2(raw[k] >> 16);
+      const float h[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[k][j] = j < valid ? (h[j] * sc - mean) * rstd : 0.f;
+      if (partial) {
+        float4 a = acc[64 * k], d = acc[64 * k + 32];
+        a.x = fmaf(g[k][0], z[k][0], a.x); a.y = fmaf(g[k][1], z[k][1], a.y); a.z = fmaf(g[k][2], z[k][2], a.z); a.w = fmaf(g[k][3], z[k][3], a.w);
+        d.x += g[k][0]; d.y += g[k][1]; d.z += g[k][2]; d.w += g[k][3];
+        acc[64 * k] = a;
+        acc[64 * k + 32] = d;
+      }
+      if (w) {
+        float ww[4];
+        load4(w + c, vec, valid, ww);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[k][j] *= ww[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { s1 += g[k][j]; s2 = fmaf(g[k][j], z[k][j], s2); }
+    }
+    const float m1 = team_sum<W>(s1, s_sum[flip][0], warp) * inv_e, m2 = team_sum<W>(s2, s_sum[flip][1], warp) * inv_e;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
+      float o[4], r[4] = {0.f, 0.f, 0.f, 0.f};
+      if (add) load4(add + row * E + c, vec, valid, r);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(rstd, g[k][j] - m1 - z[k][j] * m2, r[j]);
+      store4(dx + row * E + c, vec, valid, o);
+    }
+  }
+  if (!partial) return;
+  __syncthreads();
+  // the block's teams, in their order
+  float* out = partial + (long long)blockIdx.x * 2 * E;
+  const float* flat = reinterpret_cast<const float*>(s_acc);
+  for (int i = threadIdx.x; i < 2 * E; i += 256) {
+    const int which = i >= E, c = which ? i - E : i, block = c / kBlock, at = c % kBlock;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8 / W; ++t) sum += flat[(((long long)(t * W + block % W) * NB + block / W) * 2 + which) * kBlock + at];
+    out[i] = sum;
+  }
+}
+
+// Rows of more than kTeamColumns: one warp per row, which is read three times, twice from the caches.
 template <typename T>
 __global__ void __launch_bounds__(128) norm_forward_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b,
                                                            T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
@@ -224,21 +476,28 @@ __global__ void __launch_bounds__(128) norm_param_partial_kernel(const unsigned 
   }
 }
 
+// dw[c], db[c]: the partial rows in a fixed order - warp w of 32 takes rows w, w + 32, ..., the 32 sums are added in order.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_param_join_kernel(const float* __restrict__ partial, long long slices, int E, T* __restrict__ dw,
-                                                              T* __restrict__ db) {
-  const int e = blockIdx.x * 256 + threadIdx.x;
-  if (e >= 2 * E) return;
+__global__ void __launch_bounds__(1024) norm_param_join_kernel(const float* __restrict__ partial, long long slices, int E, T* __restrict__ dw,
+                                                               T* __restrict__ db) {
+  __shared__ float s_sum[32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
   float sum = 0.f;
-  for (long long i = 0; i < slices; ++i) sum += partial[i * 2 * E + e];
+  if (e < 2 * E)
+#pragma unroll 4
+    for (long long i = warp; i < slices; i += 32) sum += partial[i * 2 * E + e];
+  s_sum[warp][lane] = sum;
+  __syncthreads();
+  if (warp != 0 || e >= 2 * E) return;
+#pragma unroll
+  for (int w = 1; w < 32; ++w) sum += s_sum[w][lane];
   if (e < E) { if (dw) dw[e] = from_f<T>(sum); }
   else if (db) db[e - E] = from_f<T>(sum);
 }
 
 static int grid_for(long long blocks, int per_sm, int* grid) {
-  int device = 0, n_sm = 0;
-  HAPX_CUDA(cudaGetDevice(&device));
-  HAPX_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
+  int n_sm = 0;
+  if (int e = sm_count(&n_sm)) return e;
   *grid = (int)std::max<long long>(1, std::min<long long>(blocks, (long long)n_sm * per_sm));
   return HAPX_OK;
 }
@@ -254,6 +513,30 @@ static int check_act(const char* who, int dtype, int64_t n, int act, double p) {
 static int check_norm(const char* who, int dtype, int64_t rows, int64_t E) {
   if (dtype != HAPX_F32 && dtype != HAPX_BF16) return fail(HAPX_ERR_DTYPE, std::string(who) + ": float32 or bfloat16 only");
   if (rows < 0 || E < 1 || E > (1 << 20)) return fail(HAPX_ERR_EXTENT, std::string(who) + ": the normalised dimension must lie in [1, 2^20]");
+  return HAPX_OK;
+}
+
+// Warps per row and blocks of 128 columns per warp (at most) for a row of E <= kTeamColumns.
+static int team_warps(long long E) { return E <= 1024 ? 1 : E <= 2048 ? 2 : E <= 4096 ? 4 : 8; }
+#define HAPX_LN8_SWITCH(E)                  \
+  if ((E) <= 256) HAPX_LN8_TEAM(1, 2);      \
+  else if ((E) <= 512) HAPX_LN8_TEAM(1, 4); \
+  else if ((E) <= 768) HAPX_LN8_TEAM(1, 6); \
+  else if ((E) <= 1024) HAPX_LN8_TEAM(1, 8); \
+  else if ((E) <= 2048) HAPX_LN8_TEAM(2, 8); \
+  else if ((E) <= 4096) HAPX_LN8_TEAM(4, 8); \
+  else if ((E) <= kTeamColumns) HAPX_LN8_TEAM(8, 8);
+
+// 64 KiB of dynamic shared memory for a kernel on the current device (asked for once).
+static int allow_shared(const void* kernel) {
+  static std::mutex mutex;
+  static std::set<std::pair<int, const void*>> known;
+  int device = 0;
+  HAPX_CUDA(cudaGetDevice(&device));
+  std::lock_guard<std::mutex> lock(mutex);
+  if (known.count({device, kernel})) return HAPX_OK;
+  HAPX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
+  known.insert({device, kernel});
   return HAPX_OK;
 }
 
@@ -276,7 +559,7 @@ int hapx_act_dropout8(void* y, void* saved, float* scales, const void* x, int dt
   if (thr)
     if (int e = rng_state(&st)) return e;
   int grid = 1;
-  if (int e = grid_for((n + 8 * kBlock - 1) / (8 * kBlock), 8, &grid)) return e;
+  if (int e = grid_for((n + 2048 * kActUnroll - 1) / (2048 * kActUnroll), 8, &grid)) return e;
   const float ks = (float)(1.0 / (1.0 - p));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   unsigned char* sv = static_cast<unsigned char*>(saved);
@@ -302,7 +585,7 @@ int hapx_act_dropout8_backward(void* dx, const void* dy, const void* saved, cons
   if (thr)
     if (int e = rng_state(&st)) return e;
   int grid = 1;
-  if (int e = grid_for((n + 1023) / 1024, 8, &grid)) return e;
+  if (int e = grid_for((n + 2048 * kActUnroll - 1) / (2048 * kActUnroll), 8, &grid)) return e;
   const float ks = (float)(1.0 / (1.0 - p));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const unsigned char* sv = static_cast<const unsigned char*>(saved);
@@ -324,13 +607,24 @@ int hapx_layer_norm8_forward(const void* x, const void* gamma, const void* beta,
   if (saved && (ld_saved < E || ld_saved % 16 != 0 || (reinterpret_cast<uintptr_t>(saved) & 15u)))
     return fail(HAPX_ERR_EXTENT, "layer_norm8_forward: `saved` needs a 16-byte aligned base and pitch, and a pitch that covers a row");
   int grid = 1;
-  if (int e = grid_for((rows + 3) / 4, 16, &grid)) return e;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-#define HAPX_LN8(T)                                                                                                                       \
-  norm_forward_kernel<T><<<grid, 128, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(gamma), static_cast<const T*>(beta),   \
-                                                   static_cast<T*>(y), mean, rstd, static_cast<unsigned char*>(saved), ld_saved, scales, \
-                                                   rows, (int)E, (float)eps)
-  if (dtype == HAPX_BF16) HAPX_LN8(__nv_bfloat16); else HAPX_LN8(float);
+  unsigned char* q = static_cast<unsigned char*>(saved);
+#define HAPX_LN8(T, KERNEL, THREADS) \
+  KERNEL<<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(gamma), static_cast<const T*>(beta), static_cast<T*>(y), mean, \
+                                       rstd, q, ld_saved, scales, rows, (int)E, (float)eps)
+#define HAPX_LN8_TEAM(W, NB)                                                                    \
+  do {                                                                                          \
+    if (int e = grid_for((rows + 8 / W - 1) / (8 / W), NB <= 4 ? 4 : NB <= 6 ? 3 : 2, &grid)) return e; \
+    if (dtype == HAPX_BF16) HAPX_LN8(__nv_bfloat16, (norm_forward_team_kernel<__nv_bfloat16, W, NB>), 256); \
+    else HAPX_LN8(float, (norm_forward_team_kernel<float, W, NB>), 256);                        \
+  } while (0)
+  HAPX_LN8_SWITCH(E)
+  else {
+    if (int e = grid_for((rows + 3) / 4, 16, &grid)) return e;
+    if (dtype == HAPX_BF16) HAPX_LN8(__nv_bfloat16, norm_forward_kernel<__nv_bfloat16>, 128);
+    else HAPX_LN8(float, norm_forward_kernel<float>, 128);
+  }
+#undef HAPX_LN8_TEAM
 #undef HAPX_LN8
   HAPX_CUDA(cudaGetLastError());
   count_launch();
@@ -338,7 +632,14 @@ int hapx_layer_norm8_forward(const void* x, const void* gamma, const void* beta,
 }
 
 int64_t hapx_layer_norm8_backward_workspace(int64_t rows, int64_t E) {
-  return (std::max<int64_t>(1, (rows + kSliceRows - 1) / kSliceRows)) * 2 * E * (int64_t)sizeof(float);
+  int grid = 1;
+  if (E < 1 || rows < 0) return 0;
+  int64_t slices = (rows + kSliceRows - 1) / kSliceRows;
+  if (E <= kTeamColumns) {
+    if (grid_for((rows + 8 / team_warps(E) - 1) / (8 / team_warps(E)), 2, &grid)) return 0;
+    slices = grid;
+  }
+  return std::max<int64_t>(1, slices) * 2 * E * (int64_t)sizeof(float);
 }
 
 int hapx_layer_norm8_backward(const void* saved, int64_t ld_saved, const float* scales, const void* dy, const void* gamma, const float* mean,
@@ -350,31 +651,58 @@ int hapx_layer_norm8_backward(const void* saved, int64_t ld_saved, const float* 
   if (rows > 0 && (ld_saved < E || ld_saved % 16 != 0 || (reinterpret_cast<uintptr_t>(saved) & 15u)))
     return fail(HAPX_ERR_EXTENT, "layer_norm8_backward: `saved` needs a 16-byte aligned base and pitch, and a pitch that covers a row");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const long long slices = (rows + kSliceRows - 1) / kSliceRows;
-  int grid = 1;
-  if (int e = grid_for((rows + 3) / 4, 16, &grid)) return e;
   const unsigned char* q = static_cast<const unsigned char*>(saved);
-#define HAPX_LN8(T)                                                                                                                           \
-  do {                                                                                                                                        \
-    if (rows > 0) {                                                                                                                           \
-      norm_backward_kernel<T><<<grid, 128, 0, stream>>>(q, ld_saved, scales, static_cast<const T*>(dy), static_cast<const T*>(gamma), mean,   \
-                                                        rstd, static_cast<const T*>(add), static_cast<T*>(dx), rows, (int)E);                 \
-      count_launch();                                                                                                                         \
-    }                                                                                                                                         \
-    if (dgamma || dbeta) {                                                                                                                    \
-      if (rows > 0) {                                                                                                                         \
-        const dim3 g2((unsigned)((E + kBlock - 1) / kBlock), (unsigned)std::min<long long>(slices, 65535));                                   \
-        norm_param_partial_kernel<T><<<g2, 128, 0, stream>>>(q, ld_saved, scales, static_cast<const T*>(dy), mean, rstd, workspace, rows, (int)E); \
-        count_launch();                                                                                                                       \
-      }                                                                                                                                       \
-      norm_param_join_kernel<T><<<(unsigned)((2 * E + 255) / 256), 256, 0, stream>>>(workspace, slices, (int)E, static_cast<T*>(dgamma),      \
-                                                                                     static_cast<T*>(dbeta));                                 \
-      count_launch();                                                                                                                         \
-    }                                                                                                                                         \
+  const bool params = dgamma || dbeta;
+  float* partial = params ? workspace : nullptr;
+  long long slices = 0;
+  int grid = 1;
+  if (rows > 0) {
+#define HAPX_LN8_RUN(T, W, NB)                                                                                                              \
+  do {                                                                                                                                      \
+    auto kernel = norm_backward_team_kernel<T, W, NB>;                                                                                      \
+    if (int e = allow_shared(reinterpret_cast<const void*>(kernel))) return e;                                                              \
+    kernel<<<grid, 256, params ? 8 * NB * 1024 : 0, stream>>>(q, ld_saved, scales, static_cast<const T*>(dy), static_cast<const T*>(gamma), mean, \
+                                                              rstd, static_cast<const T*>(add), static_cast<T*>(dx), partial, rows, (int)E); \
   } while (0)
-  if (dtype == HAPX_BF16) HAPX_LN8(__nv_bfloat16); else HAPX_LN8(float);
-#undef HAPX_LN8
-  HAPX_CUDA(cudaGetLastError());
+#define HAPX_LN8_TEAM(W, NB)                                                             \
+  do {                                                                                   \
+    if (int e = grid_for((rows + 8 / W - 1) / (8 / W), 2, &grid)) return e;              \
+    slices = grid;                                                                       \
+    if (dtype == HAPX_BF16) HAPX_LN8_RUN(__nv_bfloat16, W, NB);                          \
+    else HAPX_LN8_RUN(float, W, NB);                                                     \
+  } while (0)
+    HAPX_LN8_SWITCH(E)
+    else {
+      slices = (rows + kSliceRows - 1) / kSliceRows;
+      if (int e = grid_for((rows + 3) / 4, 16, &grid)) return e;
+      const dim3 g2((unsigned)((E + kBlock - 1) / kBlock), (unsigned)std::min<long long>(slices, 65535));
+#define HAPX_LN8_LONG(T)                                                                                                                       \
+  do {                                                                                                                                         \
+    norm_backward_kernel<T><<<grid, 128, 0, stream>>>(q, ld_saved, scales, static_cast<const T*>(dy), static_cast<const T*>(gamma), mean, rstd, \
+                                                      static_cast<const T*>(add), static_cast<T*>(dx), rows, (int)E);                          \
+    if (params)                                                                                                                                \
+      norm_param_partial_kernel<T><<<g2, 128, 0, stream>>>(q, ld_saved, scales, static_cast<const T*>(dy), mean, rstd, workspace, rows, (int)E); \
+  } while (0)
+      if (dtype == HAPX_BF16) HAPX_LN8_LONG(__nv_bfloat16);
+      else HAPX_LN8_LONG(float);
+      if (params) count_launch();
+#undef HAPX_LN8_LONG
+    }
+#undef HAPX_LN8_TEAM
+#undef HAPX_LN8_RUN
+    HAPX_CUDA(cudaGetLastError());
+    count_launch();
+  }
+  if (params) {
+    const unsigned joins = (unsigned)((2 * E + 31) / 32);
+    if (dtype == HAPX_BF16)
+      norm_param_join_kernel<__nv_bfloat16><<<joins, 1024, 0, stream>>>(workspace, slices, (int)E, static_cast<__nv_bfloat16*>(dgamma),
+                                                                        static_cast<__nv_bfloat16*>(dbeta));
+    else
+      norm_param_join_kernel<float><<<joins, 1024, 0, stream>>>(workspace, slices, (int)E, static_cast<float*>(dgamma), static_cast<float*>(dbeta));
+    HAPX_CUDA(cudaGetLastError());
+    count_launch();
+  }
   return HAPX_OK;
 }
 

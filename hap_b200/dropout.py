@@ -13,10 +13,9 @@ draws fresh masks on every replay.  Call ids number the dropout sites in program
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from .comm import _on_device, _stream
+from .comm import _on_device, _once, _stream
 
 _next_call_id = 0
 
@@ -176,39 +175,44 @@ def act_dropout(x: torch.Tensor, act: str, p: float, training: bool = True) -> t
     return _ActDropout.apply(x, _ACTS[act], p, new_call_id() if p > 0.0 else 0)
 
 
-class _ActDropout8(torch.autograd.Function):
-    """What is kept for the backward pass: gelu its input as e4m3 values with one scale per 128 consecutive elements,
-    relu one bit per element (active and kept)."""
+def _act8(x, act, p, call_id, keep):
+    """The activation, and - ``keep`` - what its backward pass needs: gelu its input as e4m3 bytes followed by one float32
+    scale per 128 consecutive elements, relu one bit per element (active and kept)."""
+    (x,) = _dense(x)
+    n = x.numel()
+    y = torch.empty_like(x)
+    kept = saved = scales = None
+    if keep:
+        values = (n + 127) // 128 * 128 if act == 2 else (n + 7) // 8
+        kept = torch.empty(values + (values // 32 if act == 2 else 0), dtype=torch.uint8, device=x.device)
+        saved = kept.data_ptr()
+        scales = saved + values if act == 2 else None
+    with _on_device(x.device):
+        N.check(N.lib.hapx_act_dropout8(y.data_ptr(), saved, scales, x.data_ptr(), _code(x), n, act, p, call_id, _stream(x.device)))
+    return y, kept
 
+
+class _ActDropout8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, act, p, call_id, keep):
-        (x,) = _dense(x)
-        n = x.numel()
-        y = torch.empty_like(x)
-        saved = scales = None
-        if keep and ctx.needs_input_grad[0]:
-            saved = torch.empty((n + 7) // 8 if act == 1 else (n + 3) // 4 * 4, dtype=torch.uint8, device=x.device)
-            scales = torch.empty((n + 127) // 128, dtype=torch.float32, device=x.device) if act == 2 else None
-        with _on_device(x.device):
-            N.check(N.lib.hapx_act_dropout8(y.data_ptr(), saved.data_ptr() if saved is not None else None,
-                                            scales.data_ptr() if scales is not None else None, x.data_ptr(), _code(x), n, act, float(p),
-                                            call_id, _stream(x.device)))
-        ctx.save_for_backward(saved, scales)
+    def forward(ctx, x, act, p, call_id):
+        y, kept = _act8(x, act, p, call_id, True)
+        ctx.save_for_backward(kept)
         ctx.meta = (act, p, call_id, y.stride())
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
-        saved, scales = ctx.saved_tensors
+        (kept,) = ctx.saved_tensors
         act, p, call_id, strides = ctx.meta
         grad = _in_layout(grad, strides)              # the layout the forward pass walked
-        dx = torch.empty_strided(grad.shape, strides, dtype=grad.dtype, device=grad.device)
+        dx = torch.empty_like(grad) if grad.is_contiguous() else torch.empty_strided(grad.shape, strides, dtype=grad.dtype, device=grad.device)
+        n = grad.numel()
+        saved = kept.data_ptr()
         with _on_device(grad.device):
-            N.check(N.lib.hapx_act_dropout8_backward(dx.data_ptr(), grad.data_ptr(), saved.data_ptr(),
-                                                     scales.data_ptr() if scales is not None else None, _code(grad), grad.numel(), act,
-                                                     float(p), call_id, _stream(grad.device)))
-        return dx, None, None, None, None
+            N.check(N.lib.hapx_act_dropout8_backward(dx.data_ptr(), grad.data_ptr(), saved, saved + (n + 127) // 128 * 128 if act == 2 else None,
+                                                     _code(grad), n, act, p, call_id, _stream(grad.device)))
+        return dx, None, None, None
 
 
 def act_dropout8(x: torch.Tensor, act: str, p: float, training: bool = True) -> torch.Tensor:
@@ -219,7 +223,10 @@ def act_dropout8(x: torch.Tensor, act: str, p: float, training: bool = True) -> 
     if act not in _ACTS:
         raise ValueError(f"act_dropout8: the activation is \"relu\" or \"gelu\", got {act!r}")
     p = float(p) if training else 0.0
-    return _ActDropout8.apply(x, _ACTS[act], p, new_call_id() if p > 0.0 else 0, torch.is_grad_enabled())
+    call_id = new_call_id() if p > 0.0 else 0
+    if x.requires_grad and torch.is_grad_enabled():
+        return _ActDropout8.apply(x, _ACTS[act], p, call_id)
+    return _act8(x, _ACTS[act], p, call_id, False)[0]
 
 
 def keep_mask(n: int, p: float, call_id: int, device=None) -> torch.Tensor:

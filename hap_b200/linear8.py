@@ -19,92 +19,122 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import block8
-from .block8 import Block8, _CODES, _empty, _run
-from .comm import _on_device, _stream
+from .block8 import Block8, _CODES, _up
+from .comm import _on_device, _once, _stream
+
+_sizes = {}      # (device, shape, what is asked) -> workspace bytes
 
 
-def _pack(*forms):
-    """Tensors and plain values of some Block8 operands, for ctx."""
-    tensors, meta = [], []
-    for f in forms:
-        if f is None:
-            tensors += [None, None]
-            meta.append(None)
-        else:
-            tensors += [f.values, f.scales]
-            meta.append((f.rows, f.cols))
-    return tensors, meta
+def _forward_workspace(device, m, n, k, prepared, keep_x) -> int:
+    key = (device.index, m, n, k, prepared, keep_x)
+    size = _sizes.get(key)
+    if size is None:
+        size = _sizes[key] = N.lib.hapx_linear8_forward_workspace(m, n, k, prepared, keep_x)
+    return size
 
 
-def _unpack(tensors, meta):
-    return [None if m is None else Block8(tensors[2 * i], tensors[2 * i + 1], *m) for i, m in enumerate(meta)]
+def _backward_workspace(device, m, n, k, dx, dw, db) -> int:
+    key = (device.index, m, n, k, dx, dw, db)
+    size = _sizes.get(key)
+    if size is None:
+        size = _sizes[key] = N.lib.hapx_linear8_backward_workspace(m, n, k, dx, dw, db)
+    return size
 
 
-def _bias_grad(partial: torch.Tensor, rows: int, cols: int, dtype) -> torch.Tensor:
-    db = torch.empty(cols, dtype=dtype, device=partial.device)
-    with _on_device(partial.device):
-        N.check(N.lib.hapx_block8_colsum_join(db.data_ptr(), _CODES[dtype], partial.data_ptr(), rows, cols, _stream(partial.device)))
-    return db
+def _kept_bytes(rows: int, cols: int):
+    """Bytes of an 8-bit matrix and of its scales, rounded up so that pieces laid one after another stay aligned."""
+    return _up(rows * _up(cols, 16), 256), _up(cols, 512) // 512 * _up(rows, 128) * 4
+
+
+def _rows(t: torch.Tensor):
+    """The matrix of a tensor's last dimension (a copy only when its rows do not lie at one pitch) and that pitch."""
+    cols = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(t.numel() // cols, cols)
+    if t.is_contiguous():
+        return t, cols
+    if t.shape[0] > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:
+        return t.contiguous(), cols
+    return t, t.stride(0) if t.shape[0] > 1 else cols
+
+
+def _forward(x, weight, bias, prepared, keep_x, keep_w):
+    """y and the block of kept bytes (x8t, its scales, w8t, its scales; None when neither is asked for)."""
+    device, dtype = x.device, x.dtype
+    k = x.shape[-1]
+    m = x.numel() // k
+    x2, ldx = _rows(x)
+    if prepared is None:
+        n = weight.shape[0]
+        w, ldw = _rows(weight)
+        w_ptr, w8_ptr, w8s_ptr = w.data_ptr(), None, None
+    else:
+        n = prepared.rows
+        ldw, w_ptr, w8_ptr, w8s_ptr = 0, None, prepared.values.data_ptr(), prepared.scales.data_ptr()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    y = torch.empty((*x.shape[:-1], n), dtype=dtype, device=device)
+    if m == 0:
+        keep_x = False
+    kept = xt = xts = wt = wts = None
+    if keep_x or keep_w:
+        (xv, xs), (wv, ws_) = _kept_bytes(k, m) if keep_x else (0, 0), _kept_bytes(k, n) if keep_w else (0, 0)
+        kept = torch.empty(xv + xs + wv + ws_, dtype=torch.uint8, device=device)
+        base = kept.data_ptr()
+        if keep_x:
+            xt, xts = base, base + xv
+        if keep_w:
+            wt, wts = base + xv + xs, base + xv + xs + wv
+    with _on_device(device):
+        need = _forward_workspace(device, max(m, 1), n, k, prepared is not None, keep_x)
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        N.check(N.lib.hapx_linear8_forward(y.data_ptr(), x2.data_ptr(), ldx, w_ptr, ldw, w8_ptr, w8s_ptr,
+                                           bias.data_ptr() if bias is not None else None, _CODES[dtype], m, n, k, xt, xts, wt, wts,
+                                           work.data_ptr() if need else None, need, _stream(device)))
+    return y, kept
 
 
 class _Linear8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, prepared, keep):
-        rows, fin = x.numel() // x.shape[-1], x.shape[-1]
-        x2 = block8._matrix(x.reshape(rows, fin), "linear8")
-        need_x, need_w, need_b = (keep and n for n in ctx.needs_input_grad[:3])
-        need_w = need_w and prepared is None
-        if prepared is None:
-            w8 = block8.quantize_weight(weight, transposed=need_x)
-        else:
-            w8 = prepared
-        x8t = None
-        if rows:
-            x8 = _empty(rows, fin, x.device)
-            x8t = _empty(fin, rows, x.device) if need_w else None
-            _run(x2, False, x8, x8t)
-            y = block8.matmul(x8, w8, bias, x.dtype)
-        else:
-            y = torch.empty((0, w8.rows), dtype=x.dtype, device=x.device)
-        tensors, ctx.forms = _pack(x8t, w8.transposed if need_x else None)
-        ctx.save_for_backward(*tensors)
-        ctx.needs = (need_x, need_w, need_b and bias is not None)
-        ctx.fout, ctx.x_shape, ctx.dtype = w8.rows, x.shape, x.dtype
-        return y.view(*x.shape[:-1], w8.rows)
+    def forward(ctx, x, weight, bias, prepared):
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        y, kept = _forward(x, weight, bias, prepared, need_w, need_x and prepared is None)
+        t = prepared.transposed if prepared is not None and need_x else None
+        ctx.save_for_backward(kept, *((t.values, t.scales) if t is not None else ()))
+        ctx.meta = (x.shape, y.shape[-1], need_x, need_w, need_b)
+        return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
-        need_x, need_w, need_b = ctx.needs
-        x8t, w8t = _unpack(ctx.saved_tensors, ctx.forms)
-        fout, fin = ctx.fout, ctx.x_shape[-1]
-        rows = g.numel() // fout
-        dx = dw = db = None
-        if rows == 0:
-            if need_x:
-                dx = torch.empty(ctx.x_shape, dtype=ctx.dtype, device=g.device)
-            if need_w:
-                dw = torch.zeros((fout, fin), dtype=ctx.dtype, device=g.device)
-            if need_b:
-                db = torch.zeros(fout, dtype=ctx.dtype, device=g.device)
-            return dx, dw, db, None, None
-        g2 = block8._matrix(g.reshape(rows, fout), "linear8 backward")
-        # one read of g: its rows for dx, its columns for dW, partial column sums for db
-        g8 = _empty(rows, fout, g.device) if need_x or not need_w else None
-        g8t = _empty(fout, rows, g.device) if need_w else None
-        partial = torch.empty((block8._blocks(rows), fout), dtype=torch.float32, device=g.device) if need_b else None
-        _run(g2, False, g8, g8t, partial)
-        if need_x:
-            dx = block8.matmul(g8, w8t, None, ctx.dtype).view(ctx.x_shape)
-        if need_w:
-            dw = block8.matmul(g8t, x8t, None, ctx.dtype)
-        if need_b:
-            db = _bias_grad(partial, rows, fout, ctx.dtype)
-        return dx, dw, db, None, None
+        kept, *prepared_t = ctx.saved_tensors
+        x_shape, n, need_x, need_w, need_b = ctx.meta
+        device, dtype = g.device, g.dtype
+        k = x_shape[-1]
+        m = g.numel() // n
+        g2, ldg = _rows(g)
+        dx = torch.empty(x_shape, dtype=dtype, device=device) if need_x else None
+        dw = torch.empty((n, k), dtype=dtype, device=device) if need_w else None
+        db = torch.empty(n, dtype=dtype, device=device) if need_b else None
+        xt = xts = wt = wts = None
+        xv, xs = _kept_bytes(k, m) if need_w and m else (0, 0)
+        if need_w and m:
+            xt, xts = kept.data_ptr(), kept.data_ptr() + xv
+        if prepared_t:
+            wt, wts = prepared_t[0].data_ptr(), prepared_t[1].data_ptr()
+        elif need_x:
+            wt = kept.data_ptr() + xv + xs
+            wts = wt + _kept_bytes(k, n)[0]
+        with _on_device(device):
+            need = _backward_workspace(device, max(m, 1), n, k, need_x, need_w, need_b)
+            work = torch.empty(need, dtype=torch.uint8, device=device)
+            N.check(N.lib.hapx_linear8_backward(dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                                                db.data_ptr() if need_b else None, g2.data_ptr(), ldg, _CODES[dtype], m, n, k, wt, wts, xt, xts,
+                                                work.data_ptr(), need, _stream(device)))
+        return dx, dw, db, None
 
 
 def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -120,7 +150,7 @@ def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Opti
         raise ValueError(f"linear8: at least one input feature is expected, got shape {tuple(input.shape)}")
     prepared = weight if isinstance(weight, Block8) else None
     if prepared is not None:
-        if input.requires_grad and torch.is_grad_enabled() and prepared.transposed is None:
+        if prepared.transposed is None and input.requires_grad and torch.is_grad_enabled():
             raise ValueError("linear8: the input's gradient needs the weight's transposed form: block8.quantize_weight(w, transposed=True)")
         fout, fin, device = prepared.rows, prepared.cols, prepared.device
         weight = None
@@ -139,4 +169,7 @@ def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Opti
             raise TypeError(f"linear8: mixed operand dtypes {input.dtype} and {bias.dtype}")
         if tuple(bias.shape) != (fout,) or bias.device != input.device:
             raise ValueError(f"linear8: the bias must be ({fout},) on {input.device}, got {tuple(bias.shape)} on {bias.device}")
-    return _Linear8.apply(input, weight, bias, prepared, torch.is_grad_enabled())
+    if torch.is_grad_enabled() and (input.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _Linear8.apply(input, weight, bias, prepared)
+    return _forward(input, weight, bias, prepared, False, False)[0]

@@ -10,10 +10,9 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from .comm import _on_device, _stream
+from .comm import _on_device, _once, _stream
 
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16}
 
@@ -118,74 +117,98 @@ def layer_norm_fork(input: torch.Tensor, normalized_shape, weight=None, bias=Non
 
 # ---- the input kept for the backward pass in 8 bits ---------------------------------------------------
 def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+    return None if t is None else t.data_ptr()
 
 
-def _norm8_forward(ctx, x, weight, bias, eps, keep):
-    E = x.shape[-1]
-    xc = x.contiguous()
-    rows = xc.numel() // E
+def _kept8(rows: int, E: int):
+    """Pitch of a row of e4m3 bytes; where the scales and the statistics start behind them; bytes in all."""
     pitch = (E + 15) // 16 * 16
+    scales = rows * pitch
+    stats = scales + 4 * rows * ((E + 127) // 128)
+    return pitch, scales, stats, stats + 8 * rows
+
+
+def _norm8_forward(x, w, b, eps, keep):
+    """y, and - ``keep`` - one block of bytes for the backward pass: the input as e4m3 bytes, its scales, mean and rstd."""
+    E = x.shape[-1]
+    rows = x.numel() // E
+    xc = x.contiguous()
     y = torch.empty_like(xc)
-    saved = scales = stats = mean = rstd = None
-    if keep and any(ctx.needs_input_grad[:3]):
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-        mean, rstd = stats[0], stats[1]
-        saved = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty((rows, (E + 127) // 128), dtype=torch.float32, device=x.device)
-    w = None if weight is None else weight.contiguous()
-    b = None if bias is None else bias.contiguous()
+    pitch, scales_at, stats_at, size = _kept8(rows, E)
+    kept = saved = scales = mean = rstd = None
+    if keep:
+        kept = torch.empty(size, dtype=torch.uint8, device=x.device)
+        saved = kept.data_ptr()
+        scales, mean, rstd = saved + scales_at, saved + stats_at, saved + stats_at + 4 * rows
     with _on_device(x.device):
-        N.check(N.lib.hapx_layer_norm8_forward(xc.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(mean), _ptr(rstd), _ptr(saved), pitch,
-                                               _ptr(scales), _DTYPES[x.dtype], rows, E, float(eps), _stream(x.device)))
-    ctx.save_for_backward(saved, scales, stats, w)
-    ctx.has_bias = bias is not None
+        N.check(N.lib.hapx_layer_norm8_forward(xc.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), mean, rstd, saved, pitch, scales, _DTYPES[x.dtype],
+                                               rows, E, eps, _stream(x.device)))
+    return y, kept
+
+
+def _norm8_save(ctx, x, weight, bias, eps):
+    w = None if weight is None else weight.contiguous()
+    y, kept = _norm8_forward(x, w, None if bias is None else bias.contiguous(), eps, True)
+    ctx.save_for_backward(kept, w)
+    _, ctx.need_w, ctx.need_b, _ = ctx.needs_input_grad
     return y
 
 
 def _norm8_backward(ctx, dy, add):
-    saved, scales, stats, w = ctx.saved_tensors
-    E = dy.shape[-1]
+    kept, w = ctx.saved_tensors
+    E, device, dtype = dy.shape[-1], dy.device, dy.dtype
     rows = dy.numel() // E
-    dyc = dy.contiguous()
+    dy = dy.contiguous()
     add = None if add is None else add.contiguous()
-    dx = torch.empty_like(dyc)
-    dw = torch.empty(E, dtype=dy.dtype, device=dy.device) if w is not None and ctx.needs_input_grad[1] else None
-    db = torch.empty(E, dtype=dy.dtype, device=dy.device) if ctx.has_bias and ctx.needs_input_grad[2] else None
-    work = None
-    if dw is not None or db is not None:
-        work = torch.empty(N.lib.hapx_layer_norm8_backward_workspace(rows, E) // 4, dtype=torch.float32, device=dy.device)
-    with _on_device(dy.device):
-        N.check(N.lib.hapx_layer_norm8_backward(saved.data_ptr(), saved.shape[1], scales.data_ptr(), dyc.data_ptr(), _ptr(w), stats[0].data_ptr(),
-                                                stats[1].data_ptr(), _ptr(add), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work), _DTYPES[dy.dtype], rows, E,
-                                                _stream(dy.device)))
-    return dx, dw, db, None, None
+    dx = torch.empty_like(dy)
+    dw = torch.empty(E, dtype=dtype, device=device) if ctx.need_w else None
+    db = torch.empty(E, dtype=dtype, device=device) if ctx.need_b else None
+    pitch, scales_at, stats_at, _ = _kept8(rows, E)
+    saved = kept.data_ptr()
+    with _on_device(device):
+        work = None
+        if ctx.need_w or ctx.need_b:
+            key = (device.index, rows, E)
+            size = _work8.get(key)
+            if size is None:
+                size = _work8[key] = N.lib.hapx_layer_norm8_backward_workspace(rows, E)
+            work = torch.empty(size, dtype=torch.uint8, device=device)
+        N.check(N.lib.hapx_layer_norm8_backward(saved, pitch, saved + scales_at, dy.data_ptr(), _ptr(w), saved + stats_at,
+                                                saved + stats_at + 4 * rows, _ptr(add), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work),
+                                                _DTYPES[dtype], rows, E, _stream(device)))
+    return dx, dw, db, None
+
+
+_work8 = {}      # (device, rows, E) -> workspace bytes of the backward pass
 
 
 class _LayerNorm8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, keep):
-        return _norm8_forward(ctx, x, weight, bias, eps, keep)
+    def forward(ctx, x, weight, bias, eps):
+        return _norm8_save(ctx, x, weight, bias, eps)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         return _norm8_backward(ctx, dy, None)
 
 
 class _LayerNormFork8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, keep):
+    def forward(ctx, x, weight, bias, eps):
         ctx.set_materialize_grads(False)
-        y = _norm8_forward(ctx, x, weight, bias, eps, keep)
-        return x.view_as(x), y
+        return x.view_as(x), _norm8_save(ctx, x, weight, bias, eps)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, d_residual, dy):
         if dy is None:                       # the normalised branch took no part in the loss
-            return d_residual, None, None, None, None
+            return d_residual, None, None, None
         return _norm8_backward(ctx, dy, d_residual)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _check8(what, input, shape, weight, bias):
@@ -207,7 +230,9 @@ def layer_norm8(input: torch.Tensor, normalized_shape, weight=None, bias=None, e
     statistics of the input itself."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     _check8("layer_norm8", input, shape, weight, bias)
-    return _LayerNorm8.apply(input, weight, bias, eps, torch.is_grad_enabled())
+    if _wants_grad(input, weight, bias):
+        return _LayerNorm8.apply(input, weight, bias, eps)
+    return _norm8_forward(input, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), eps, False)[0]
 
 
 def layer_norm_fork8(input: torch.Tensor, normalized_shape, weight=None, bias=None, eps: float = 1e-5):
@@ -215,4 +240,6 @@ def layer_norm_fork8(input: torch.Tensor, normalized_shape, weight=None, bias=No
     gradient added inside the normalisation's backward kernel."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     _check8("layer_norm_fork8", input, shape, weight, bias)
-    return _LayerNormFork8.apply(input, weight, bias, eps, torch.is_grad_enabled())
+    if _wants_grad(input, weight, bias):
+        return _LayerNormFork8.apply(input, weight, bias, eps)
+    return input, layer_norm8(input, shape, weight, bias, eps)

@@ -451,8 +451,26 @@ int hapx_block8_dequantize(void* out, int dtype, const void* q, int64_t ldq, con
 int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k);
 int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const void* a_scale, const void* b, int64_t ldb, const void* b_scale,
                        const void* bias, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, hapx_stream stream);
+/* F.linear on 8-bit blocks, one call per direction.  x, y, g, dx, dw, db, bias of `dtype` (HAPX_F32 / HAPX_BF16); y, dx,
+ * dw contiguous, ldx / ldw / ldg elements from row to row.
+ *   forward: y[m, n] = x[m, k] w[n, k]^T + bias.  The weight is either w (n x k of `dtype`), quantised inside the call in
+ *     128 x 128 tiles, or - w null - w8 / w8_scale, n x k in 8 bits with rows of k rounded up to 16 bytes.  x8t / x8t_scale
+ *     (may be null): x's columns form, k x m with rows of m rounded up to 16 bytes, kept for dw; w8t / w8t_scale (may be
+ *     null, only with w): the weight's transposed form, k x n with rows of n rounded up to 16 bytes, kept for dx.
+ *   backward: dx[m, k] = g w from w8t, dw[n, k] = g^T x from x8t, db[n] = column sums of g; any of the three may be null.
+ *     m == 0 zeroes dw and db.
+ * `workspace`: as many bytes as the _workspace function says on the current device (`keep_x`: x8t is asked for; dx, dw,
+ * db: which of them are), 16-byte aligned, free to be reused when the call's kernels have run. */
+int64_t hapx_linear8_forward_workspace(int64_t m, int64_t n, int64_t k, int prepared, int keep_x);
+int hapx_linear8_forward(void* y, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* w8, const void* w8_scale, const void* bias,
+                         int dtype, int64_t m, int64_t n, int64_t k, void* x8t, void* x8t_scale, void* w8t, void* w8t_scale, void* workspace,
+                         int64_t workspace_bytes, hapx_stream stream);
+int64_t hapx_linear8_backward_workspace(int64_t m, int64_t n, int64_t k, int dx, int dw, int db);
+int hapx_linear8_backward(void* dx, void* dw, void* db, const void* g, int64_t ldg, int dtype, int64_t m, int64_t n, int64_t k, const void* w8t,
+                          const void* w8t_scale, const void* x8t, const void* x8t_scale, void* workspace, int64_t workspace_bytes,
+                          hapx_stream stream);
 /* hapx_act_dropout and its backward pass with less kept in between.  act 2 (gelu): `saved` holds the input as e4m3
- * bytes (n rounded up to 4, 16-byte aligned), `scales` one float per 128 consecutive elements.  act 1 (relu): `saved`
+ * bytes (n rounded up to 8, 16-byte aligned), `scales` one float per 128 consecutive elements.  act 1 (relu): `saved`
  * holds one bit per element, active and kept (bit i % 8 of byte i / 8), `scales` is not used.  saved null: nothing is
  * kept. */
 int hapx_act_dropout8(void* y, void* saved, float* scales, const void* x, int dtype, int64_t n, int act, double p, uint64_t call_id,
