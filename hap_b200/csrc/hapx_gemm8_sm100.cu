@@ -8,7 +8,7 @@
 // whose structure this kernel has: persistent, warp-specialised, two accumulators used alternately.
 //   warp 0      : TMA producer (128 x 128 byte tiles, 128-byte swizzle; every fourth block also the scales of four blocks)
 //   warp 1      : allocates TMEM; one thread copies scales to tensor memory (tcgen05.cp) and issues tcgen05.mma
-//   warps 2 - 9 : epilogue, two warps per 32 rows: bias, one rounding, bulk stores through a staging tile
+//   the others  : epilogue, a warp per 32 rows x 64 columns: bias, one rounding, bulk stores through a staging tile
 // (An earlier form kept one accumulator per block and the running sums in registers, adding block products with their
 // scales in the epilogue warps; it was bound by the chain commit -> wait -> read -> arrive of its two accumulators.)
 //
@@ -83,7 +83,8 @@ __device__ __forceinline__ void copy_scales(unsigned taddr, unsigned smem) {
 template <bool PAIR>
 struct Cfg {
   static constexpr int BN = PAIR ? 192 : 64;                 // columns of the tile
-  static constexpr int EPI_WARPS = 8;
+  static constexpr int PIECES = BN / 64;                     // 64 columns: 128 bytes of a bfloat16 row
+  static constexpr int EPI_WARPS = 4 * PIECES;               // one piece of 32 rows each
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int STAGES = PAIR ? 6 : 7;
   static constexpr int B_ATOMS = PAIR ? 2 : 1;               // 192 columns from a multiple of 64 on lie in two groups of 128
@@ -123,31 +124,19 @@ __device__ __forceinline__ void stage_row(unsigned char* row, int sw, const floa
   }
 }
 
-// v[j] += bias[n + j] for the columns inside the matrix.
-template <bool OUT_F32, int W>
-__device__ __forceinline__ void add_bias(const Params& p, int n, float (&v)[W]) {
-  if (p.bias_vec && n + W <= p.N) {            // 16-byte loads, the same address in every lane
-    if constexpr (OUT_F32) {
-      const float4* b = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + n);
+// v[j] += bias[n + j] (float32) for the columns inside the matrix; `vec`: all are, and the bias lies on 16 bytes.
+__device__ __forceinline__ void add_bias(const Params& p, int n, bool vec, float (&v)[32]) {
+  const float* bias = static_cast<const float*>(p.bias) + n;
+  if (vec) {
 #pragma unroll
-      for (int j = 0; j < W / 4; ++j) {
-        const float4 x = __ldg(b + j);
-        v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
-      }
-    } else {
-      const uint4* b = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + n);
-#pragma unroll
-      for (int j = 0; j < W / 8; ++j) {
-        const uint4 x = __ldg(b + j);
-        const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { v[8 * j + 2 * e] += __uint_as_float(w[e] << 16); v[8 * j + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u); }
-      }
+    for (int j = 0; j < 8; ++j) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(bias) + j);
+      v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (n + j < p.N) v[j] += OUT_F32 ? static_cast<const float*>(p.bias)[n + j] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n + j]);
+    for (int j = 0; j < 32; ++j)
+      if (n + j < p.N) v[j] += bias[j];
   }
 }
 
@@ -205,14 +194,15 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 
   if (warp == 0) {
     // ---------------- TMA producer (one per CTA) ----------------
-    if (lane == 0) {
-      int stage = 0;
-      unsigned phase = 0;
-      bool ok = true;
-      for (int unit = worker; unit < units && ok; unit += workers) {
-        const Unit u = decode(unit);
-        for (int kb = u.kb0; kb < u.kb1; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u)) { ok = false; break; }
+    int stage = 0;
+    unsigned phase = 0;
+    bool ok = true;
+    for (int unit = worker; unit < units && ok; unit += workers) {
+      const Unit u = decode(unit);
+      for (int kb = u.kb0; kb < u.kb1; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u));
+        if (!ok) break;
+        if (elect_one()) {
           const unsigned sa = base + stage * C::STAGE_BYTES, sb = sa + C::A_BYTES;
           // the scales of four blocks come with the first of them that the unit needs, in the stage's own slot
           const bool scales = kb == u.kb0 || (kb & 3) == 0;
@@ -236,54 +226,62 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
               tma_load_4d(ss + kAtom, &tmSB, 0, u.n0 >> 7, kb >> 2, 0, full_bar(stage));
             }
           }
-          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
+        __syncwarp();
+        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
       }
-      if (!ok) atomicCAS(p.error, 0u, 1u);
     }
+    if (!ok && lane == 0) atomicCAS(p.error, 0u, 1u);
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
-    if (lane == 0 && cta == 0) {
+    if (cta == 0) {
       int stage = 0, acc = 0;
       unsigned phase = 0, acc_phase = 0;
       bool ok = true;
+      // descriptors of the first 32 bytes of a stage; a stage or a step of 32 further on is an addition to the address field
+      const unsigned long long desc_a = make_desc(base, 16u, 1024u), desc_b = make_desc(base + C::A_BYTES, 16u, 1024u);
       for (int unit = worker; unit < units && ok; unit += workers) {
         const Unit u = decode(unit);
         const unsigned d = tmem_base + (unsigned)(acc * C::BN), shift = (unsigned)(u.n0 >> 5) & 3u;   // B's rows start inside a group of 128
-        unsigned sfa = 0, sfb = 0;
-        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u)) { ok = false; break; }
+        unsigned sf = 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), acc_phase ^ 1u));
+        if (!ok) break;
         for (int kb = u.kb0; kb < u.kb1; ++kb) {
-          if (!mbar_wait(full_bar(stage), phase)) { ok = false; break; }
+          ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase));
+          if (!ok) break;
           tc_fence_after();
-          if (kb == u.kb0 || (kb & 3) == 0) {
-            // tcgen05.cp and tcgen05.mma run in the order of their issue, and a set is not written again before the
-            // stages have gone round
-            const unsigned ss = base + kScales + stage * C::SCALE_BYTES;
-            sfa = tmem_base + C::SF_COL + stage * C::SF_SET;
-            sfb = sfa + 4;
-            copy_scales<PAIR>(sfa, ss);
+          const bool scales = kb == u.kb0 || (kb & 3) == 0;
+          if (scales) sf = tmem_base + C::SF_COL + stage * C::SF_SET;
+          if (elect_one()) {
+            if (scales) {
+              // tcgen05.cp and tcgen05.mma run in the order of their issue, and a set is not written again before the
+              // stages have gone round
+              const unsigned ss = base + kScales + stage * C::SCALE_BYTES;
 #pragma unroll
-            for (int i = 0; i < C::B_ATOMS; ++i) copy_scales<PAIR>(sfb + 4 * i, ss + (1 + i) * kAtom);
+              for (int i = 0; i <= C::B_ATOMS; ++i) copy_scales<PAIR>(sf + 4 * i, ss + i * kAtom);
+            }
+            const unsigned long long da = desc_a + (unsigned)(stage * (C::STAGE_BYTES >> 4)), db = desc_b + (unsigned)(stage * (C::STAGE_BYTES >> 4));
+            const unsigned idesc = C::IDESC | ((unsigned)(kb & 3) << 4) | ((unsigned)(kb & 3) << 29);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k) umma8<PAIR>(d, da + 2 * k, db + 2 * k, idesc, sf, sf + 4 + shift, kb != u.kb0 || k != 0);
+            if (PAIR) umma2_commit_both(empty_bar(stage));
+            else umma_commit(empty_bar(stage));
+            if (kb + 1 == u.kb1) {                           // the accumulator is complete
+              if (PAIR) umma2_commit_both(tfull_bar(acc));
+              else umma_commit(tfull_bar(acc));
+            }
           }
-          const unsigned sa = base + stage * C::STAGE_BYTES, sb = sa + C::A_BYTES;
-          const unsigned idesc = C::IDESC | ((unsigned)(kb & 3) << 4) | ((unsigned)(kb & 3) << 29);
-#pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k)
-            umma8<PAIR>(d, make_desc(sa + k * 32u, 16u, 1024u), make_desc(sb + k * 32u, 16u, 1024u), idesc, sfa, sfb + shift, kb != u.kb0 || k != 0);
-          if (PAIR) umma2_commit_both(empty_bar(stage));
-          else umma_commit(empty_bar(stage));
+          __syncwarp();
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        if (PAIR) umma2_commit_both(tfull_bar(acc));
-        else umma_commit(tfull_bar(acc));
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      if (!ok) atomicCAS(p.error, 0u, 2u);
+      if (!ok && lane == 0) atomicCAS(p.error, 0u, 2u);
     }
   } else {
-    // ---------------- epilogue: 32 rows per warp, every other piece of 128 bytes per row ----------------
-    const int q = warp & 3, half = (warp - 2) >> 2;          // q: the TMEM lane quarter this warp may read
+    // ---------------- epilogue: 32 rows x 64 columns of the tile per warp ----------------
+    const int q = warp & 3, part = (warp - 2) >> 2;          // q: the TMEM lane quarter this warp may read
     unsigned char* tile_gen = gen_base + kStore + (warp - 2) * 4096;
     const unsigned tile_u32 = base + kStore + (warp - 2) * 4096;
     int acc = 0;
@@ -291,12 +289,18 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     bool ok = true;
     for (int unit = worker; unit < units; unit += workers) {
       const Unit u = decode(unit);
+      const int n0 = u.n0 + 64 * part, width = min(64, p.N - n0);   // this warp's columns inside the matrix (may be none)
+      const bool bias_vec = p.bias_vec && width == 64;
+      uint4 braw[8];
+      if (!p.out_f32 && bias_vec) {                          // travels during the wait
+#pragma unroll
+        for (int j = 0; j < 8; ++j) braw[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + n0) + j);
+      }
       ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
       if (!ok) break;
       tc_fence_after();
-      const unsigned t = tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(acc * C::BN);
+      const unsigned t = tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(acc * C::BN + 64 * part);
       const long long out_row0 = (long long)u.split * p.m_pad + u.m0 + q * 32;
-      const int width = min(C::BN, p.N - u.n0);              // columns of the tile inside the matrix
       auto drained = [&] {                                   // this warp has read its part of the accumulator
         tc_fence_before();
         __syncwarp();
@@ -305,53 +309,81 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
           else mbar_arrive(tempty_bar(acc));
         }
       };
-      auto drain = [&](auto f32_tag) {
+      // W columns from c on, staged as 128 bytes per row: out in one bulk store, or row by row for any pitch
+      auto send = [&](auto f32_tag, int c) {
         constexpr bool OUT_F32 = decltype(f32_tag)::value;
         constexpr int W = OUT_F32 ? 32 : 64;
-        bool told = false;
-#pragma unroll 1
-        for (int c = half * W; c < width; c += 2 * W) {
-          unsigned r[W];
-          tmem_ld_32x32(t + (unsigned)c, reinterpret_cast<unsigned(&)[32]>(r[0]));
-          if (!OUT_F32) tmem_ld_32x32(t + (unsigned)c + 32, reinterpret_cast<unsigned(&)[32]>(r[W - 32]));
-          tmem_ld_wait();
-          if (c + 2 * W >= width) { drained(); told = true; }
-          float v[W];
-#pragma unroll
-          for (int j = 0; j < W; ++j) v[j] = __uint_as_float(r[j]);
-          if (p.bias) add_bias<OUT_F32, W>(p, u.n0 + c, v);
-          if (lane == 0) bulk_wait_read_0();                 // the previous piece has left the staging tile
+        if (p.tma_store) {
+          fence_proxy_async();
           __syncwarp();
-          stage_row<OUT_F32>(tile_gen + lane * 128, lane & 7, v);
-          if (p.tma_store) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_4d(&tmD, tile_u32, u.n0 + c, (int)out_row0, 0, 0);
-              bulk_commit_group();
-            }
-          } else {                                           // any pitch: rows of the tile one after another, coalesced
-            __syncwarp();
-            const int rows = min(32, p.M - (u.m0 + q * 32));
-            for (int i = 0; i < rows; ++i) {
+          if (lane == 0) {
+            tma_store_4d(&tmD, tile_u32, n0 + c, (int)out_row0, 0, 0);
+            bulk_commit_group();
+          }
+        } else {
+          __syncwarp();
+          const int rows = min(32, p.M - (u.m0 + q * 32));
+          for (int i = 0; i < rows; ++i) {
 #pragma unroll
-              for (int h = 0; h < W / 32; ++h) {
-                const int col = lane + 32 * h, byte = col * (OUT_F32 ? 4 : 2);
-                const unsigned char* src = tile_gen + i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15);
-                if (c + col < width) {
-                  const long long at = (out_row0 + i) * p.ldd + u.n0 + c + col;
-                  if (OUT_F32) static_cast<float*>(p.D)[at] = *reinterpret_cast<const float*>(src);
-                  else static_cast<__nv_bfloat16*>(p.D)[at] = *reinterpret_cast<const __nv_bfloat16*>(src);
-                }
+            for (int h = 0; h < W / 32; ++h) {
+              const int col = lane + 32 * h, byte = col * (OUT_F32 ? 4 : 2);
+              const unsigned char* src = tile_gen + i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15);
+              if (c + col < width) {
+                const long long at = (out_row0 + i) * p.ldd + n0 + c + col;
+                if (OUT_F32) static_cast<float*>(p.D)[at] = *reinterpret_cast<const float*>(src);
+                else static_cast<__nv_bfloat16*>(p.D)[at] = *reinterpret_cast<const __nv_bfloat16*>(src);
               }
             }
-            __syncwarp();
           }
+          __syncwarp();
         }
-        if (!told) drained();                                // no column for this warp in a narrow tile
       };
-      if (p.out_f32) drain(std::true_type{});
-      else drain(std::false_type{});
+      auto staging_free = [&] {                              // the previous store has read the staging tile
+        if (lane == 0) bulk_wait_read_0();
+        __syncwarp();
+      };
+      if (width <= 0) {
+        drained();
+      } else if (p.out_f32) {
+#pragma unroll 1
+        for (int c = 0; c < 64 && c < width; c += 32) {
+          unsigned r[32];
+          tmem_ld_32x32(t + (unsigned)c, r);
+          tmem_ld_wait();
+          if (c + 32 >= width) drained();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          if (p.bias) add_bias(p, n0 + c, bias_vec, v);
+          staging_free();
+          stage_row<true>(tile_gen + lane * 128, lane & 7, v);
+          send(std::true_type{}, c);
+        }
+      } else {
+        unsigned r[64];
+        tmem_ld_32x32(t, reinterpret_cast<unsigned(&)[32]>(r[0]));
+        tmem_ld_32x32(t + 32, reinterpret_cast<unsigned(&)[32]>(r[32]));
+        tmem_ld_wait();
+        drained();
+        float v[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j]);
+        if (bias_vec) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const unsigned w[4] = {braw[j].x, braw[j].y, braw[j].z, braw[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[8 * j + 2 * e] += __uint_as_float(w[e] << 16); v[8 * j + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u); }
+          }
+        } else if (p.bias) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            if (j < width) v[j] += __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n0 + j]);
+        }
+        staging_free();
+        stage_row<false>(tile_gen + lane * 128, lane & 7, v);
+        send(std::false_type{}, 0);
+      }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) bulk_wait_all();
@@ -519,7 +551,7 @@ int run(const Product& pr, int sm_count, cudaStream_t stream) {
   long long out_rows = M;
   if (pl.splits > 1) { p.D = pr.workspace; p.ldd = pl.n_pad; p.out_f32 = 1; p.bias = nullptr; out_rows = pl.splits * pl.m_pad; }
   else { p.D = pr.d; p.ldd = N; p.out_f32 = pr.out_f32; p.bias = pr.bias; }
-  p.bias_vec = (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
+  p.bias_vec = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
   const int es = p.out_f32 ? 4 : 2;
   CUtensorMap tmA, tmB, tmSA, tmSB, tmD;
   std::memset(&tmD, 0, sizeof(tmD));

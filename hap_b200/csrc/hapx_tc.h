@@ -47,6 +47,19 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
   }
   return false;
 }
+// True in one lane of a converged warp.  Roles that issue bulk copies and tensor-core instructions keep the whole warp in
+// their loop and put only the issue under this: addresses and descriptors then stay in uniform registers, where those
+// instructions want them.  Under `lane == 0` every operand is moved there one by one (about 80 cycles for one
+// tcgen05.mma, which made the issuing thread the slowest part of a product of 128-deep steps).
+__device__ __forceinline__ bool elect_one() {
+  unsigned yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
