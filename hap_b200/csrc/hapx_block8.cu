@@ -5,22 +5,37 @@
 // in either direction, so no maximum crosses a tile - and keeps it in registers: warp w holds rows 16w .. 16w + 15,
 // lane l the columns 4l .. 4l + 3.
 #include <algorithm>
+#include <cstring>
+#include <mutex>
 #include <string>
 
 #include "hapx_block8.h"
 #include "hapx_internal.h"
+#include "hapx_tc.h"
 
 namespace hapx {
 namespace block8 {
 
-struct QuantJobs { QuantJob job[2]; long long tiles0, tiles; };     // tiles of the first matrix, of both
+struct QuantJobs {
+  QuantJob job[2];
+  long long tiles0, tiles;       // tiles of the first matrix, of both
+  int bulk[2];                   // the matrix can be fetched by bulk tensor loads (16-byte aligned base and pitch)
+  unsigned* error;               // device word: a wait that ran out
+};
 
-// Four consecutive elements as they are in memory.
+// Four consecutive elements as they are in memory, and what the quantiser asks of them.  A magnitude's pattern is its
+// float32 bits (of a bfloat16 the upper half, with anything below); patterns order like the numbers.  A NaN loses
+// against any number, an infinity wins.
 template <typename T> struct Raw4;
 template <> struct Raw4<__nv_bfloat16> {
   uint2 w;
+  struct Max { __nv_bfloat162 a, b; };                 // of columns 0, 1 and 2, 3
+  static constexpr unsigned kMask = 0xffff0000u;       // a pattern's own bits
+  static __device__ __forceinline__ __nv_bfloat162 two(unsigned v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+  static __device__ __forceinline__ unsigned bits(__nv_bfloat162 v) { return *reinterpret_cast<const unsigned*>(&v); }
   __device__ __forceinline__ void zero() { w = make_uint2(0u, 0u); }
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void load_shared(const unsigned char* tile, int row, int lane) { w = reinterpret_cast<const uint2*>(tile)[row * 32 + lane]; }
   __device__ __forceinline__ void load_some(const __nv_bfloat16* p, int valid) {
     const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
     w.x = (valid > 0 ? h[0] : 0u) | (valid > 1 ? (unsigned)h[1] << 16 : 0u);
@@ -30,15 +45,32 @@ template <> struct Raw4<__nv_bfloat16> {
     f[0] = __uint_as_float(w.x << 16); f[1] = __uint_as_float(w.x & 0xffff0000u);
     f[2] = __uint_as_float(w.y << 16); f[3] = __uint_as_float(w.y & 0xffff0000u);
   }
-  __device__ __forceinline__ float at(int j) const {
-    const unsigned v = j < 2 ? w.x : w.y;
-    return __uint_as_float(j & 1 ? v & 0xffff0000u : v << 16);
+  static __device__ __forceinline__ void clear(Max& m) { m.a = m.b = two(0u); }
+  // joins the column maxima, returns the row's pattern
+  __device__ __forceinline__ unsigned maxima(Max& m) const {
+    const __nv_bfloat162 x = __habs2(two(w.x)), y = __habs2(two(w.y));
+    m.a = __hmax2(m.a, x); m.b = __hmax2(m.b, y);
+    const __nv_bfloat162 r = __hmax2(__hmax2(x, y), two(0u));                       // of two NaN: 0
+    return bits(__hmax2(r, two(__byte_perm(bits(r), 0u, 0x1032))));
+  }
+  static __device__ __forceinline__ void columns(const Max& m, unsigned (&c)[4]) {
+    c[0] = bits(m.a) << 16; c[1] = bits(m.a); c[2] = bits(m.b) << 16; c[3] = bits(m.b);
+  }
+  // infinities become NaN
+  __device__ __forceinline__ void sanitise() {
+    if ((w.x & 0x7f80u) == 0x7f80u) w.x |= 0x7fffu;
+    if ((w.x & 0x7f800000u) == 0x7f800000u) w.x |= 0x7fff0000u;
+    if ((w.y & 0x7f80u) == 0x7f80u) w.y |= 0x7fffu;
+    if ((w.y & 0x7f800000u) == 0x7f800000u) w.y |= 0x7fff0000u;
   }
 };
 template <> struct Raw4<float> {
   float4 v;
+  struct Max { float c[4]; };
+  static constexpr unsigned kMask = 0xffffffffu;
   __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void load_shared(const unsigned char* tile, int row, int lane) { v = reinterpret_cast<const float4*>(tile)[row * 32 + lane]; }
   __device__ __forceinline__ void load_some(const float* p, int valid) {
     zero();
     if (valid > 0) v.x = p[0];
@@ -47,186 +79,187 @@ template <> struct Raw4<float> {
     if (valid > 3) v.w = p[3];
   }
   __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
-  __device__ __forceinline__ float at(int j) const { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
-};
-
-// Running maxima of magnitudes of four columns (two per register for bfloat16); a NaN loses against any number.
-template <typename T> struct Max4;
-template <> struct Max4<__nv_bfloat16> {
-  __nv_bfloat162 a, b;
-  __device__ __forceinline__ void zero() { a = b = __floats2bfloat162_rn(0.f, 0.f); }
-  __device__ __forceinline__ void add(const Raw4<__nv_bfloat16>& r) {
-    const unsigned x = r.w.x & 0x7fff7fffu, y = r.w.y & 0x7fff7fffu;
-    a = __hmax2(a, *reinterpret_cast<const __nv_bfloat162*>(&x));
-    b = __hmax2(b, *reinterpret_cast<const __nv_bfloat162*>(&y));
+  static __device__ __forceinline__ void clear(Max& m) { m.c[0] = m.c[1] = m.c[2] = m.c[3] = 0.f; }
+  __device__ __forceinline__ unsigned maxima(Max& m) const {
+    m.c[0] = fmaxf(m.c[0], fabsf(v.x)); m.c[1] = fmaxf(m.c[1], fabsf(v.y)); m.c[2] = fmaxf(m.c[2], fabsf(v.z)); m.c[3] = fmaxf(m.c[3], fabsf(v.w));
+    return __float_as_uint(fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), 0.f));
   }
-  __device__ __forceinline__ void get(float (&f)[4]) const {
-    f[0] = __low2float(a); f[1] = __high2float(a); f[2] = __low2float(b); f[3] = __high2float(b);
+  static __device__ __forceinline__ void columns(const Max& m, unsigned (&c)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(m.c[j]);
   }
-  static __device__ __forceinline__ float of(const Raw4<__nv_bfloat16>& r) {
-    const unsigned x = r.w.x & 0x7fff7fffu, y = r.w.y & 0x7fff7fffu;
-    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
-    return fmaxf(fmaxf(__low2float(m), __high2float(m)), 0.f);      // of two NaN: 0
-  }
-};
-template <> struct Max4<float> {
-  float m[4];
-  __device__ __forceinline__ void zero() { m[0] = m[1] = m[2] = m[3] = 0.f; }
-  __device__ __forceinline__ void add(const Raw4<float>& r) {
-    m[0] = fmaxf(m[0], fabsf(r.v.x)); m[1] = fmaxf(m[1], fabsf(r.v.y)); m[2] = fmaxf(m[2], fabsf(r.v.z)); m[3] = fmaxf(m[3], fabsf(r.v.w));
-  }
-  __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = m[0]; f[1] = m[1]; f[2] = m[2]; f[3] = m[3]; }
-  static __device__ __forceinline__ float of(const Raw4<float>& r) {
-    return fmaxf(fmaxf(fmaxf(fabsf(r.v.x), fabsf(r.v.y)), fmaxf(fabsf(r.v.z), fabsf(r.v.w))), 0.f);
-  }
+  __device__ __forceinline__ void sanitise() { v = make_float4(finite_or_nan(v.x), finite_or_nan(v.y), finite_or_nan(v.z), finite_or_nan(v.w)); }
 };
 
 // square: one scale per 128 x 128 tile, stored for each of its rows (and columns).
 //
-// The elements stay in their own type in registers (32 of them for bfloat16), so that three blocks fit an SM; the
-// transposed bytes go through shared memory and leave as whole 128-byte rows.
+// Two passes over the tile in registers, where the elements stay in their own type (32 registers for bfloat16, three
+// blocks per SM): the maxima of rows and columns, then - once all scales are known - both forms from one unpacking.  The
+// transposed bytes go through shared memory and leave as whole 128-byte rows.  What bounds it is the bytes in flight: a
+// block fetches its next tile into shared memory by one bulk tensor load while it works on and stores the present one.
 template <typename T>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const __grid_constant__ QuantJobs jobs) {
-  __shared__ float s_col[8][kBlock];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const __grid_constant__ QuantJobs jobs, const __grid_constant__ CUtensorMap map0,
+                                                                               const __grid_constant__ CUtensorMap map1) {
+  extern __shared__ unsigned char s_dynamic[];   // the next tile, 128 x 128 elements
+  unsigned char* s_x = s_dynamic + ((128u - (tc::smem_u32(s_dynamic) & 127u)) & 127u);
+  __shared__ unsigned long long s_bar;
+  __shared__ uint4 s_col[8][32];                 // column maxima of each warp
+  __shared__ float4 s_sum[8][32];                // its column sums
   __shared__ uint4 s_t[kBlock * 8];
   __shared__ int s_odd;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // where this thread's scales lie inside the 512 bytes of a tile (lane i < 16: row 16 warp + i; warp j < 4: column 4 lane + j)
+  const int at_row = ((16 * warp + (lane & 15)) & 31) * 16 + (warp >> 1) * 4, at_col = ((4 * lane + (warp & 3)) & 31) * 16 + (lane >> 3) * 4;
+  const unsigned bar = tc::smem_u32(&s_bar);
+  unsigned phase = 0;
+  if (threadIdx.x == 0) {
+    tc::mbar_init(bar, 1);
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  auto fetch = [&](long long both) {             // by one thread: the tile's load, if it is one
+    const int which = both >= jobs.tiles0;
+    if (both >= jobs.tiles || !jobs.bulk[which]) return;
+    const unsigned tile = (unsigned)(which ? both - jobs.tiles0 : both), col_tiles = (unsigned)jobs.job[which].col_tiles, rt = tile / col_tiles;
+    tc::mbar_expect_tx(bar, kBlock * kBlock * sizeof(T));
+    tc::tma_load_4d(tc::smem_u32(s_x), which ? &map1 : &map0, (int)(tile - rt * col_tiles) * kBlock, (int)rt * kBlock, 0, 0, bar);
+  };
+  if (threadIdx.x == 0) fetch(blockIdx.x);
   for (long long both = blockIdx.x; both < jobs.tiles; both += gridDim.x) {
-    const QuantJob& p = jobs.job[both >= jobs.tiles0];
-    const long long tile = both >= jobs.tiles0 ? both - jobs.tiles0 : both;
-    const T* x = static_cast<const T*>(p.x);
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0 && (p.ldx & 3) == 0;
-    const bool square = p.square != 0;
-    const int rt = (int)(tile / p.col_tiles), ct = (int)(tile % p.col_tiles);
+    const int which = both >= jobs.tiles0;
+    const QuantJob& p = jobs.job[which];
+    const unsigned tile = (unsigned)(which ? both - jobs.tiles0 : both);        // fewer than 2^31
+    const bool square = p.square != 0, want_q = p.q != nullptr, want_qt = p.qt != nullptr, want_sum = p.colsum != nullptr;
+    const int rt = (int)(tile / (unsigned)p.col_tiles), ct = (int)tile - rt * p.col_tiles;
     const long long r0 = (long long)rt * kBlock + 16 * warp, c0 = (long long)ct * kBlock + 4 * lane;
     const int valid = (int)max(0ll, min(4ll, p.cols - c0)), live = (int)max(0ll, min(16ll, p.rows - r0));   // columns, rows of this thread
     Raw4<T> v[16];
-    {
-      const T* src = x + r0 * p.ldx + c0;
-      if (vec && valid == 4) {
+    if (jobs.bulk[which]) {                      // outside the matrix the load has put zeros
+      const bool ok = __syncthreads_and(tc::mbar_wait(bar, phase));
+      phase ^= 1u;
+      if (!ok) {                                 // the same in every thread
+        if (threadIdx.x == 0) atomicCAS(jobs.error, 0u, 4u);
+        return;
+      }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (i < live) v[i].load(src + i * p.ldx);
-          else v[i].zero();
-        }
-      } else {
+      for (int i = 0; i < 16; ++i) v[i].load_shared(s_x, 16 * warp + i, lane);
+      __syncthreads();                           // the tile is in registers: its place is free
+    } else {
+      const T* src = static_cast<const T*>(p.x) + r0 * p.ldx + c0;
+      const bool vec = (reinterpret_cast<uintptr_t>(p.x) & (4 * sizeof(T) - 1)) == 0 && (p.ldx & 3) == 0 && valid == 4;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (i < live) v[i].load_some(src + i * p.ldx, valid);
-          else v[i].zero();
-        }
+      for (int i = 0; i < 16; ++i) {
+        if (i >= live) v[i].zero();
+        else if (vec) v[i].load(src + i * p.ldx);
+        else v[i].load_some(src + i * p.ldx, valid);
       }
     }
-    if (p.colsum) {
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (threadIdx.x == 0) fetch(both + gridDim.x);
+    if (threadIdx.x == 0) s_odd = 0;
+    unsigned rowmax = 0u, col[4];                // lane i < 16: row i's maximum
+    typename Raw4<T>::Max cm;
+    Raw4<T>::clear(cm);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const unsigned r = __reduce_max_sync(0xffffffffu, v[i].maxima(cm));
+      if (lane == i) rowmax = r;
+    }
+    Raw4<T>::columns(cm, col);
+    s_col[warp][lane] = make_uint4(col[0], col[1], col[2], col[3]);
+    __syncthreads();
+    constexpr unsigned kInf = 0x7f800000u;
+    if (max(max(col[0], col[1]), max(col[2], col[3])) >= kInf) s_odd = 1;
+    __syncthreads();
+    const bool odd = s_odd != 0;
+    if (odd) {                                   // an infinity in the tile (rare): NaN in its place, the maxima once more
+      float special[4] = {0.f, 0.f, 0.f, 0.f};   // the sums are those of the original values
+      Raw4<T>::clear(cm);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float f[4];
         v[i].get(f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += f[j];
+        for (int j = 0; j < 4; ++j) special[j] += f[j];
+        v[i].sanitise();
+        const unsigned r = __reduce_max_sync(0xffffffffu, v[i].maxima(cm));
+        if (lane == i) rowmax = r;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s_col[warp][4 * lane + j] = sum[j];
-      __syncthreads();
-      if (threadIdx.x < kBlock && (long long)ct * kBlock + threadIdx.x < p.cols) {
-        float t = 0.f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) t += s_col[w][threadIdx.x];
-        p.colsum[(long long)rt * p.cols + (long long)ct * kBlock + threadIdx.x] = t;
-      }
+      Raw4<T>::columns(cm, col);
+      s_col[warp][lane] = make_uint4(col[0], col[1], col[2], col[3]);
+      s_sum[warp][lane] = make_float4(special[0], special[1], special[2], special[3]);
       __syncthreads();
     }
-    if (threadIdx.x == 0) s_odd = 0;
-    Max4<T> cm;
-    cm.zero();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) cm.add(v[i]);
-    float colbig[4];
-    cm.get(colbig);
-    __syncthreads();
-    // An infinity anywhere in the tile (rare): NaN in its place, and the maxima once more without it.
-    if (fmaxf(fmaxf(colbig[0], colbig[1]), fmaxf(colbig[2], colbig[3])) == __uint_as_float(0x7f800000u)) s_odd = 1;
-    __syncthreads();
-    if (s_odd) {
-      cm.zero();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if constexpr (sizeof(T) == 2) {
-          if ((v[i].w.x & 0x7f80u) == 0x7f80u) v[i].w.x |= 0x7fffu;
-          if ((v[i].w.x & 0x7f800000u) == 0x7f800000u) v[i].w.x |= 0x7fff0000u;
-          if ((v[i].w.y & 0x7f80u) == 0x7f80u) v[i].w.y |= 0x7fffu;
-          if ((v[i].w.y & 0x7f800000u) == 0x7f800000u) v[i].w.y |= 0x7fff0000u;
-        } else {
-          v[i].v = make_float4(finite_or_nan(v[i].v.x), finite_or_nan(v[i].v.y), finite_or_nan(v[i].v.z), finite_or_nan(v[i].v.w));
-        }
-        cm.add(v[i]);
-      }
-      cm.get(colbig);
-    }
-    int ecol[4];
-    if (square) {
-      const float mine = warp_max(fmaxf(fmaxf(colbig[0], colbig[1]), fmaxf(colbig[2], colbig[3])));
-      if (lane == 0) s_col[0][warp] = mine;
-      __syncthreads();
-      float big = s_col[0][0];
-#pragma unroll
-      for (int w = 1; w < 8; ++w) big = fmaxf(big, s_col[0][w]);
-      ecol[0] = ecol[1] = ecol[2] = ecol[3] = scale_exponent(big);
-      const unsigned char byte = (unsigned char)(ecol[0] + 127);
-      if (threadIdx.x < kBlock) {
-        if (p.q) p.s[scale_at((long long)rt * kBlock + threadIdx.x, ct, p.row_tiles)] = byte;
-      } else {
-        if (p.qt) p.st[scale_at((long long)ct * kBlock + threadIdx.x - kBlock, rt, p.col_tiles)] = byte;
-      }
-    } else if (p.qt) {
-      *reinterpret_cast<float4*>(&s_col[warp][4 * lane]) = make_float4(colbig[0], colbig[1], colbig[2], colbig[3]);
-      __syncthreads();
+    if (want_qt || square) {
 #pragma unroll
       for (int w = 0; w < 8; ++w) {
-        const float4 o = *reinterpret_cast<const float4*>(&s_col[w][4 * lane]);
-        colbig[0] = fmaxf(colbig[0], o.x); colbig[1] = fmaxf(colbig[1], o.y); colbig[2] = fmaxf(colbig[2], o.z); colbig[3] = fmaxf(colbig[3], o.w);
+        const uint4 o = s_col[w][lane];
+        col[0] = max(col[0], o.x); col[1] = max(col[1], o.y); col[2] = max(col[2], o.z); col[3] = max(col[3], o.w);
       }
+    }
+    if (square) rowmax = col[0] = col[1] = col[2] = col[3] = __reduce_max_sync(0xffffffffu, max(max(col[0], col[1]), max(col[2], col[3])));
+    const int erow = scale_exponent(__uint_as_float(rowmax & Raw4<T>::kMask));
+    const float inv_row = pow2(-erow);
+    if (want_q && lane < live) p.s[((long long)(ct >> 2) * p.row_tiles + rt) * 512 + (ct & 3) + at_row] = (unsigned char)(erow + 127);
+    float inv_col[4];
+    if (want_qt) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        ecol[j] = scale_exponent(colbig[j]);
-        if (warp == j) p.st[scale_at(c0 + j, rt, p.col_tiles)] = (unsigned char)(ecol[j] + 127);
+        const int e = scale_exponent(__uint_as_float(col[j] & Raw4<T>::kMask));
+        inv_col[j] = pow2(-e);
+        if (warp == j && j < valid) p.st[((long long)(rt >> 2) * p.col_tiles + ct) * 512 + (rt & 3) + at_col] = (unsigned char)(e + 127);
       }
     }
-    if (p.q) {
-      int mine = 0;
-      unsigned char* dst = p.q + r0 * p.ldq + c0;
+    unsigned char* dst = p.q + r0 * p.ldq + c0;
+    const int rows_out = valid > 0 ? live : 0;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    unsigned out_t[4][4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int e = square ? ecol[0] : scale_exponent(warp_max(Max4<T>::of(v[i])));
-        if (!square && lane == i) mine = e;
-        const float inv = pow2(-e);
-        float f[4];
-        v[i].get(f);
-        if (i < live && valid > 0)     // the pitch is a multiple of 16: a partial group of 4 stays inside it
-          *reinterpret_cast<unsigned*>(dst + i * p.ldq) = pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+    for (int g = 0; g < 4; ++g) {                // four rows at a time
+      float f[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * g + i].get(f[i]);
+      if (want_q) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float inv = square ? inv_row : __shfl_sync(0xffffffffu, inv_row, 4 * g + i);
+          if (4 * g + i < rows_out)              // the pitch is a multiple of 16: a partial group of 4 stays inside it
+            *reinterpret_cast<unsigned*>(dst) = pack4(f[i][0] * inv, f[i][1] * inv, f[i][2] * inv, f[i][3] * inv);
+          dst += p.ldq;
+        }
       }
-      if (!square && lane < live) p.s[scale_at(r0 + lane, ct, p.row_tiles)] = (unsigned char)(mine + 127);
-    }
-    if (p.qt) {
+      if (want_qt) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float inv = pow2(-ecol[j]);
-        unsigned w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = pack4(v[4 * k].at(j) * inv, v[4 * k + 1].at(j) * inv, v[4 * k + 2].at(j) * inv, v[4 * k + 3].at(j) * inv);
-        s_t[(4 * lane + j) * 8 + (warp ^ (lane & 7))] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 4; ++j) out_t[j][g] = pack4(f[0][j] * inv_col[j], f[1][j] * inv_col[j], f[2][j] * inv_col[j], f[3][j] * inv_col[j]);
       }
-      __syncthreads();
+      if (want_sum) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {       // a warp writes 4 columns' 128 bytes at a time
-        const int col = k * 32 + warp * 4 + (lane >> 3), chunk = lane & 7;
-        const long long c = (long long)ct * kBlock + col, r = (long long)rt * kBlock + 16 * chunk;
-        if (c < p.cols && r < p.rows) *reinterpret_cast<uint4*>(p.qt + c * p.ldqt + r) = s_t[col * 8 + (chunk ^ ((col >> 2) & 7))];
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[j] += f[i][j];
       }
     }
-    __syncthreads();      // the shared arrays are reused by the next tile
+    if (want_qt) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s_t[(4 * lane + j) * 8 + (warp ^ (lane & 7))] = make_uint4(out_t[j][0], out_t[j][1], out_t[j][2], out_t[j][3]);
+    }
+    if (want_sum && !odd) s_sum[warp][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();                             // the maxima have been read, the transposed bytes and sums written
+    if (want_qt) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {              // a warp writes 4 columns' 128 bytes at a time
+        const int at = k * 32 + warp * 4 + (lane >> 3), chunk = lane & 7;
+        const long long c = (long long)ct * kBlock + at, r = (long long)rt * kBlock + 16 * chunk;
+        if (c < p.cols && r < p.rows) *reinterpret_cast<uint4*>(p.qt + c * p.ldqt + r) = s_t[at * 8 + (chunk ^ ((at >> 2) & 7))];
+      }
+    }
+    if (want_sum && threadIdx.x < kBlock && (long long)ct * kBlock + threadIdx.x < p.cols) {
+      const float* part = reinterpret_cast<const float*>(s_sum);
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t += part[w * kBlock + threadIdx.x];
+      p.colsum[(long long)rt * p.cols + (long long)ct * kBlock + threadIdx.x] = t;
+    }
+    // the next tile writes s_t and s_sum behind two barriers of its own
   }
 }
 
@@ -258,23 +291,65 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned char* __
   }
 }
 
+// The matrix as (column, row) in boxes of 128 x 128.
+static int make_map(CUtensorMap* map, const QuantJob& j, int dtype) {
+  gemm::EncodeTiledFn fn = gemm::encode_fn();
+  if (!fn) return fail(HAPX_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t pitch = (cuuint64_t)j.ldx * (dtype == HAPX_BF16 ? 2 : 4);
+  cuuint64_t dims[4] = {(cuuint64_t)j.cols, (cuuint64_t)j.rows, 1, 1};
+  cuuint64_t strides[3] = {pitch, pitch, pitch};
+  cuuint32_t box[4] = {kBlock, kBlock, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, dtype == HAPX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, const_cast<void*>(j.x), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HAPX_ERR_CUDA, "cuTensorMapEncodeTiled (quantise) failed with code " + std::to_string((int)r));
+  return HAPX_OK;
+}
+
+template <typename T>
+static int launch_quantize(const QuantJobs& jobs, const CUtensorMap* maps, int n_sm, cudaStream_t stream) {
+  constexpr int kShared = kBlock * kBlock * sizeof(T) + 128;
+  {  // function attributes are per device
+    static bool set[64] = {};
+    static std::mutex mutex;
+    int device = 0;
+    HAPX_CUDA(cudaGetDevice(&device));
+    if (device < 0 || device >= 64) return fail(HAPX_ERR_ARGUMENT, "block8_quantize: device index out of range");
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!set[device]) {
+      HAPX_CUDA(cudaFuncSetAttribute(quantize_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+      set[device] = true;
+    }
+  }
+  const int grid = (int)std::min<long long>(jobs.tiles, (long long)n_sm * (sizeof(T) == 2 ? 3 : 2));     // one resident wave
+  quantize_kernel<T><<<grid, 256, kShared, stream>>>(jobs, maps[0], maps[1]);
+  HAPX_CUDA(cudaGetLastError());
+  count_launch();
+  return HAPX_OK;
+}
+
 int quantize(QuantJob* job, int n_jobs, int dtype, cudaStream_t stream) {
-  int n_sm = 0;
-  if (int e = sm_count(&n_sm)) return e;
   QuantJobs jobs;
+  CUtensorMap maps[2];
+  std::memset(maps, 0, sizeof(maps));
+  int n_sm = 0;
+  if (int e = gemm::error_word(&jobs.error, &n_sm)) return e;
+  const long long es = dtype == HAPX_BF16 ? 2 : 4;
   for (int i = 0; i < n_jobs; ++i) {
     job[i].row_tiles = (int)((job[i].rows + kBlock - 1) / kBlock);
     job[i].col_tiles = (int)((job[i].cols + kBlock - 1) / kBlock);
     jobs.job[i] = job[i];
     jobs.tiles = (i ? jobs.tiles0 : 0) + (long long)job[i].row_tiles * job[i].col_tiles;
     if (i == 0) jobs.tiles0 = jobs.tiles;
+    // the map's extents and its coordinates are 32 bits wide
+    jobs.bulk[i] = (reinterpret_cast<uintptr_t>(job[i].x) & 15u) == 0 && job[i].ldx * es % 16 == 0 && job[i].ldx * es < (1ll << 40) &&
+                   job[i].rows < 0x7fffff00 && job[i].cols < 0x7fffff00;
+    if (jobs.bulk[i])
+      if (int e = make_map(&maps[i], job[i], dtype)) return e;
   }
-  const int grid = (int)std::min<long long>(jobs.tiles, (long long)n_sm * 16);
-  if (dtype == HAPX_BF16) quantize_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(jobs);
-  else quantize_kernel<float><<<grid, 256, 0, stream>>>(jobs);
-  HAPX_CUDA(cudaGetLastError());
-  count_launch();
-  return HAPX_OK;
+  if (n_jobs == 1) jobs.bulk[1] = 0;
+  return dtype == HAPX_BF16 ? launch_quantize<__nv_bfloat16>(jobs, maps, n_sm, stream) : launch_quantize<float>(jobs, maps, n_sm, stream);
 }
 
 }  // namespace block8

@@ -41,11 +41,17 @@ __device__ __forceinline__ float finite_or_nan(float v) {
   return (__float_as_uint(v) & 0x7fffffffu) >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : v;
 }
 
-// Two values, already scaled, as two e4m3 bytes (the first in the low byte); NaN stays NaN.
-__device__ __forceinline__ unsigned pack2(float lo, float hi) {
-  return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+// Four values, already scaled, as four e4m3 bytes (the first in the low byte); NaN stays NaN.
+__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
+  unsigned r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
 }
-__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) { return pack2(a, b) | (pack2(c, d) << 16); }
 __device__ __forceinline__ float2 unpack2(unsigned two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
