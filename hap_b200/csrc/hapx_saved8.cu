@@ -26,42 +26,76 @@ using namespace block8;
 
 enum Act { ACT_RELU = 1, ACT_GELU = 2 };
 
-// Phi(v) = erfc(-v / sqrt 2) / 2 and e = exp(-v^2 / 2).  erfc(z) = e^{-z^2} t P(t) for z >= 0 with t = 1 / (1 + 0.33 z): P is a
-// least-maximum fit of degree 7 to erfcx(z) / t over 0 <= z <= 9.3, relative error 8.2e-8, so the tail keeps its relative
-// accuracy (which y = v Phi(v) needs for negative v) and shares its exponential with the density.
+// Phi(v) = erfc(-v / sqrt 2) / 2 and e = exp(-v^2 / 2) = 2^(-u^2), u = |v| sqrt(log2(e) / 2).  For v < 0 it is the tail
+// e t P(t) with t = 1 / (1 + 0.36 u): P is a least-maximum fit to erfcx(|v| / sqrt 2) / (2 t) over |v| <= 13, so the tail
+// keeps its relative accuracy, which y = v Phi(v) needs, and shares its exponential with the density.  Degree 7 for
+// float32 tensors (relative error 1.0e-7), degree 5 for bfloat16 ones (4.1e-6, a 950th of their rounding).
+template <bool WIDE>
 __device__ __forceinline__ float normal_cdf(float v, float& e) {
-  const float z = fabsf(v) * 0.70710678118654752f;
-  const float t = __fdividef(1.f, fmaf(0.33f, z, 1.f));
-  e = exp2f(v * v * -0.72134752044448170f);               // log2(e) / 2
-  float q = fmaf(-0.1359295927870348f, t, 0.4626916833556958f);
-  q = fmaf(q, t, -0.3554451549092876f);
-  q = fmaf(q, t, 0.41254758607072767f);
-  q = fmaf(q, t, 0.04500733930570897f);
-  q = fmaf(q, t, 0.20192486623134484f);
-  q = fmaf(q, t, 0.18283706989561532f);
-  q = fmaf(q, t, 0.1863661211613116f);
-  const float tail = 0.5f * q * t * e;
+  const float u = fabsf(v) * 0.84932180028801907f;
+  float t;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.36f, u, 1.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-u * u));
+  float q;
+  if (WIDE) {
+    q = fmaf(0.03657762301083756f, t, -0.15125760273443148f);
+    q = fmaf(q, t, 0.18092026515553128f);
+    q = fmaf(q, t, -0.0342253215659978f);
+    q = fmaf(q, t, 0.11920223581958944f);
+    q = fmaf(q, t, 0.10414048504390966f);
+    q = fmaf(q, t, 0.12269694252912236f);
+    q = fmaf(q, t, 0.12194542414330234f);
+  } else {
+    q = fmaf(-0.07647082273966256f, t, 0.19837717655503154f);
+    q = fmaf(q, t, -0.0008176733719744526f);
+    q = fmaf(q, t, 0.1393556059441193f);
+    q = fmaf(q, t, 0.11727338761580286f);
+    q = fmaf(q, t, 0.1222832162766118f);
+  }
+  const float tail = q * t * e;
   return v >= 0.f ? 1.f - tail : tail;
 }
 
-// Eight consecutive elements; `vec`: p is aligned to 16 bytes.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int valid, float (&f)[8]) {
-  if (vec && valid >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
-      const unsigned u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+// Eight consecutive elements as they are in memory (`vec`: p is aligned to 16 bytes), so that those of the next round can
+// wait in registers.
+template <typename T> struct Raw8;
+template <> struct Raw8<__nv_bfloat16> {
+  uint4 w;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, bool vec, int valid) {
+    if (vec && valid >= 8) {
+      w = *reinterpret_cast<const uint4*>(p);
     } else {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    }
-  } else {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+      unsigned u[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = j < valid ? to_f(p[j]) : 0.f;
+      for (int i = 0; i < 4; ++i) u[i] = (2 * i < valid ? h[2 * i] : 0u) | (2 * i + 1 < valid ? (unsigned)h[2 * i + 1] << 16 : 0u);
+      w = make_uint4(u[0], u[1], u[2], u[3]);
+    }
   }
-}
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+  }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p, bool vec, int valid) {
+    if (vec && valid >= 8) {
+      a = *reinterpret_cast<const float4*>(p);
+      b = *reinterpret_cast<const float4*>(p + 4);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = j < valid ? p[j] : 0.f;
+      a = make_float4(f[0], f[1], f[2], f[3]);
+      b = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool vec, int valid, const float (&f)[8]) {
   if (vec && valid >= 8) {
@@ -85,42 +119,51 @@ __device__ __forceinline__ void store8(T* p, bool vec, int valid, const float (&
 }
 
 // A thread holds eight consecutive elements (one evaluation of the generator), sixteen lanes a block of 128; a warp takes
-// kActUnroll pieces of 256 elements at a time, their loads in flight together.
+// kActUnroll pieces of 256 elements at a time, and fetches those of its next round before it works on the present ones
+// (without that, waiting for loads was the largest share: 42 M bfloat16 elements of gelu in 52 us).
 constexpr int kActUnroll = 2;
-template <typename T, int ACT>
+template <typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ x, T* __restrict__ y, unsigned char* __restrict__ saved,
                                                           float* __restrict__ scales, long long n, unsigned threshold, float keep_scale,
                                                           const rng::State* st, unsigned long long call_id) {
   const int lane = threadIdx.x & 31;
   const bool vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0;
   rng::Key key = {0u, 0u, 0u, 0u};
-  if (threshold) key = rng::make_key(st, call_id);
+  if (DROP) key = rng::make_key(st, call_id);
   constexpr int kPiece = 256 * kActUnroll;
-  const long long pieces = (n + kPiece - 1) / kPiece;
-  for (long long piece = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); piece < pieces; piece += (long long)gridDim.x * 8) {
-    float v[kActUnroll][8];
+  const long long pieces = (n + kPiece - 1) / kPiece, stride = (long long)gridDim.x * 8, first = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  Raw8<T> next[kActUnroll];
+  auto fetch = [&](long long piece) {
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
       const long long e0 = piece * kPiece + 256 * u + 8 * lane;
-      load8(x + e0, vec, (int)max(0ll, min(8ll, n - e0)), v[u]);
+      next[u].load(x + e0, vec, (int)max(0ll, min(8ll, n - e0)));
     }
+  };
+  if (first < pieces) fetch(first);
+  for (long long piece = first; piece < pieces; piece += stride) {
+    float v[kActUnroll][8];
+#pragma unroll
+    for (int u = 0; u < kActUnroll; ++u) next[u].get(v[u]);
+    if (piece + stride < pieces) fetch(piece + stride);
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
       const long long e0 = piece * kPiece + 256 * u + 8 * lane;
       const int valid = (int)max(0ll, min(8ll, n - e0));
       unsigned keep = 0xffu, bits = 0u;
-      if (threshold) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
+      if (DROP) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
       float o[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float k = (keep >> j) & 1u ? keep_scale : 0.f, w = v[u][j];
+        const float w = v[u][j];
         if (ACT == ACT_RELU) {
-          o[j] = (w <= 0.f ? 0.f : w) * k;          // NaN passes
-          bits |= (w > 0.f && j < valid ? 1u : 0u) << j;
+          o[j] = w <= 0.f ? 0.f : w;                // NaN passes
+          bits |= (w > 0.f ? 1u : 0u) << j;
         } else {
           float e;
-          o[j] = w * normal_cdf(w, e) * k;
+          o[j] = w * normal_cdf<sizeof(T) == 4>(w, e);
         }
+        if (DROP) o[j] *= (keep >> j) & 1u ? keep_scale : 0.f;
       }
       store8(y + e0, vec, valid, o);
       if (!saved) continue;                         // nothing asks for a gradient
@@ -129,7 +172,12 @@ __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ 
       } else {
         float big = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { v[u][j] = finite_or_nan(v[u][j]); big = fmaxf(big, fabsf(v[u][j])); }
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(v[u][j]));          // a NaN loses
+        if (__any_sync(0xffffffffu, big == __uint_as_float(0x7f800000u))) {    // rare: infinities become NaN
+          big = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { v[u][j] = finite_or_nan(v[u][j]); big = fmaxf(big, fabsf(v[u][j])); }
+        }
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
         const int e = scale_exponent(big);
@@ -143,7 +191,7 @@ __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ 
   }
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__ dy, const unsigned char* __restrict__ saved,
                                                            const float* __restrict__ scales, T* __restrict__ dx, long long n,
                                                            unsigned threshold, float keep_scale, const rng::State* st,
@@ -151,24 +199,33 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
   const int lane = threadIdx.x & 31;
   const bool vec = ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx)) & 15u) == 0;
   rng::Key key = {0u, 0u, 0u, 0u};
-  if (ACT == ACT_GELU && threshold) key = rng::make_key(st, call_id);
+  if (ACT == ACT_GELU && DROP) key = rng::make_key(st, call_id);
   constexpr int kPiece = 256 * kActUnroll;
-  const long long pieces = (n + kPiece - 1) / kPiece;
-  for (long long piece = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); piece < pieces; piece += (long long)gridDim.x * 8) {
-    float d[kActUnroll][8], s[kActUnroll];
-    uint2 w[kActUnroll];
+  const long long pieces = (n + kPiece - 1) / kPiece, stride = (long long)gridDim.x * 8, first = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  Raw8<T> next[kActUnroll];
+  uint2 next_w[kActUnroll];
+  float next_s[kActUnroll];
+  auto fetch = [&](long long piece) {
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
       const long long e0 = piece * kPiece + 256 * u + 8 * lane;
       const int valid = (int)max(0ll, min(8ll, n - e0));
-      load8(dy + e0, vec, valid, d[u]);
-      w[u] = make_uint2(0u, 0u);
-      s[u] = 0.f;
+      next[u].load(dy + e0, vec, valid);
+      next_w[u] = make_uint2(0u, 0u);
+      next_s[u] = 0.f;
       if (valid > 0) {
-        if (ACT == ACT_RELU) w[u].x = saved[e0 >> 3];
-        else { w[u] = *reinterpret_cast<const uint2*>(saved + e0); s[u] = scales[e0 / kBlock]; }
+        if (ACT == ACT_RELU) next_w[u].x = saved[e0 >> 3];
+        else { next_w[u] = *reinterpret_cast<const uint2*>(saved + e0); next_s[u] = scales[e0 / kBlock]; }
       }
     }
+  };
+  if (first < pieces) fetch(first);
+  for (long long piece = first; piece < pieces; piece += stride) {
+    float d[kActUnroll][8], s[kActUnroll];
+    uint2 w[kActUnroll];
+#pragma unroll
+    for (int u = 0; u < kActUnroll; ++u) { next[u].get(d[u]); w[u] = next_w[u]; s[u] = next_s[u]; }
+    if (piece + stride < pieces) fetch(piece + stride);
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
       const long long e0 = piece * kPiece + 256 * u + 8 * lane;
@@ -179,15 +236,16 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
         for (int j = 0; j < 8; ++j) o[j] = (w[u].x >> j) & 1u ? d[u][j] * keep_scale : 0.f;
       } else {
         unsigned keep = 0xffu;
-        if (threshold) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
+        if (DROP) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
         const unsigned half[4] = {w[u].x & 0xffffu, w[u].x >> 16, w[u].y & 0xffffu, w[u].y >> 16};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float2 two = unpack2(half[j >> 1]);
           const float h = (j & 1 ? two.y : two.x) * s[u];
           float e;
-          const float cdf = normal_cdf(h, e);
-          o[j] = d[u][j] * ((keep >> j) & 1u ? keep_scale : 0.f) * fmaf(h * 0.3989422804014327f, e, cdf);
+          const float cdf = normal_cdf<sizeof(T) == 4>(h, e);
+          o[j] = d[u][j] * fmaf(h * 0.3989422804014327f, e, cdf);
+          if (DROP) o[j] *= (keep >> j) & 1u ? keep_scale : 0.f;
         }
       }
       store8(dx + e0, vec, valid, o);
@@ -560,11 +618,14 @@ int hapx_act_dropout8(void* y, void* saved, float* scales, const void* x, int dt
     if (int e = rng_state(&st)) return e;
   int grid = 1;
   if (int e = grid_for((n + 2048 * kActUnroll - 1) / (2048 * kActUnroll), 8, &grid)) return e;
-  const float ks = (float)(1.0 / (1.0 - p));
+  const float ks = thr ? (float)(1.0 / (1.0 - p)) : 1.f;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   unsigned char* sv = static_cast<unsigned char*>(saved);
-#define HAPX_ACT8(T, A) \
-  act_forward_kernel<T, A><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), static_cast<T*>(y), sv, scales, n, thr, ks, st, call_id)
+#define HAPX_ACT8(T, A)                                                                                                                     \
+  do {                                                                                                                                      \
+    if (thr) act_forward_kernel<T, A, true><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), static_cast<T*>(y), sv, scales, n, thr, ks, st, call_id); \
+    else act_forward_kernel<T, A, false><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), static_cast<T*>(y), sv, scales, n, thr, ks, st, call_id);    \
+  } while (0)
   if (dtype == HAPX_BF16) { if (act == ACT_RELU) HAPX_ACT8(__nv_bfloat16, ACT_RELU); else HAPX_ACT8(__nv_bfloat16, ACT_GELU); }
   else { if (act == ACT_RELU) HAPX_ACT8(float, ACT_RELU); else HAPX_ACT8(float, ACT_GELU); }
 #undef HAPX_ACT8
@@ -586,11 +647,14 @@ int hapx_act_dropout8_backward(void* dx, const void* dy, const void* saved, cons
     if (int e = rng_state(&st)) return e;
   int grid = 1;
   if (int e = grid_for((n + 2048 * kActUnroll - 1) / (2048 * kActUnroll), 8, &grid)) return e;
-  const float ks = (float)(1.0 / (1.0 - p));
+  const float ks = thr ? (float)(1.0 / (1.0 - p)) : 1.f;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const unsigned char* sv = static_cast<const unsigned char*>(saved);
-#define HAPX_ACT8(T, A) \
-  act_backward_kernel<T, A><<<grid, 256, 0, stream>>>(static_cast<const T*>(dy), sv, scales, static_cast<T*>(dx), n, thr, ks, st, call_id)
+#define HAPX_ACT8(T, A)                                                                                                                      \
+  do {                                                                                                                                       \
+    if (thr) act_backward_kernel<T, A, true><<<grid, 256, 0, stream>>>(static_cast<const T*>(dy), sv, scales, static_cast<T*>(dx), n, thr, ks, st, call_id); \
+    else act_backward_kernel<T, A, false><<<grid, 256, 0, stream>>>(static_cast<const T*>(dy), sv, scales, static_cast<T*>(dx), n, thr, ks, st, call_id);    \
+  } while (0)
   if (dtype == HAPX_BF16) { if (act == ACT_RELU) HAPX_ACT8(__nv_bfloat16, ACT_RELU); else HAPX_ACT8(__nv_bfloat16, ACT_GELU); }
   else { if (act == ACT_RELU) HAPX_ACT8(float, ACT_RELU); else HAPX_ACT8(float, ACT_GELU); }
 #undef HAPX_ACT8
