@@ -13,6 +13,7 @@
 #include <mutex>
 #include <set>
 #include <string>
+#include <type_traits>
 #include <utility>
 
 #include "hapx_block8.h"
@@ -134,24 +135,29 @@ __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ 
   const long long pieces = (n + kPiece - 1) / kPiece, stride = (long long)gridDim.x * 8, first = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   Raw8<T> next[kActUnroll];
   auto fetch = [&](long long piece) {
+    const long long at = piece * kPiece + 8 * lane;
+    const bool inside = vec && (piece + 1) * kPiece <= n;
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
-      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
-      next[u].load(x + e0, vec, (int)max(0ll, min(8ll, n - e0)));
+      if (inside) next[u].load(x + at + 256 * u, true, 8);
+      else next[u].load(x + at + 256 * u, vec, (int)max(0ll, min(8ll, n - (at + 256 * u))));
     }
   };
-  if (first < pieces) fetch(first);
-  for (long long piece = first; piece < pieces; piece += stride) {
+  auto work = [&](long long piece, auto full_tag) {
+    constexpr bool FULL = decltype(full_tag)::value;
+    const long long at = piece * kPiece + 8 * lane;
+    T* yp = y + at;
+    unsigned char* sp = saved + (ACT == ACT_RELU ? at >> 3 : at);
+    float* cp = scales + at / kBlock;
     float v[kActUnroll][8];
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) next[u].get(v[u]);
     if (piece + stride < pieces) fetch(piece + stride);
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
-      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
-      const int valid = (int)max(0ll, min(8ll, n - e0));
+      const int valid = FULL ? 8 : (int)max(0ll, min(8ll, n - (at + 256 * u)));
       unsigned keep = 0xffu, bits = 0u;
-      if (DROP) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
+      if (DROP) keep = rng::keep_bits(rng::philox(key, (unsigned long long)((at + 256 * u) >> 3)), threshold);
       float o[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -165,10 +171,10 @@ __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ 
         }
         if (DROP) o[j] *= (keep >> j) & 1u ? keep_scale : 0.f;
       }
-      store8(y + e0, vec, valid, o);
+      store8(yp + 256 * u, FULL || vec, valid, o);
       if (!saved) continue;                         // nothing asks for a gradient
       if (ACT == ACT_RELU) {
-        if (valid > 0) saved[e0 >> 3] = (unsigned char)(bits & keep);
+        if (FULL || valid > 0) sp[32 * u] = (unsigned char)(bits & keep);
       } else {
         float big = 0.f;
 #pragma unroll
@@ -182,13 +188,18 @@ __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ 
         for (int d = 8; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
         const int e = scale_exponent(big);
         const float inv = pow2(-e);
-        if ((lane & 15) == 0 && valid > 0) scales[e0 / kBlock] = pow2(e);
-        if (valid > 0)        // n rounded up to 8 bytes
-          *reinterpret_cast<uint2*>(saved + e0) = make_uint2(pack4(v[u][0] * inv, v[u][1] * inv, v[u][2] * inv, v[u][3] * inv),
-                                                             pack4(v[u][4] * inv, v[u][5] * inv, v[u][6] * inv, v[u][7] * inv));
+        if ((lane & 15) == 0 && (FULL || valid > 0)) cp[2 * u] = pow2(e);
+        if (FULL || valid > 0)        // n rounded up to 8 bytes
+          *reinterpret_cast<uint2*>(sp + 256 * u) = make_uint2(pack4(v[u][0] * inv, v[u][1] * inv, v[u][2] * inv, v[u][3] * inv),
+                                                               pack4(v[u][4] * inv, v[u][5] * inv, v[u][6] * inv, v[u][7] * inv));
       }
     }
-  }
+  };
+  if (first < pieces) fetch(first);
+  const long long whole = vec ? n / kPiece : 0;     // pieces that lie inside the tensor, aligned
+  long long piece = first;
+  for (; piece < whole; piece += stride) work(piece, std::true_type{});
+  for (; piece < pieces; piece += stride) work(piece, std::false_type{});
 }
 
 template <typename T, int ACT, bool DROP>
@@ -206,21 +217,26 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
   uint2 next_w[kActUnroll];
   float next_s[kActUnroll];
   auto fetch = [&](long long piece) {
+    const long long at = piece * kPiece + 8 * lane;
+    const unsigned char* sp = saved + (ACT == ACT_RELU ? at >> 3 : at);
+    const float* cp = scales + at / kBlock;
+    const bool inside = vec && (piece + 1) * kPiece <= n;
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
-      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
-      const int valid = (int)max(0ll, min(8ll, n - e0));
-      next[u].load(dy + e0, vec, valid);
+      const int valid = inside ? 8 : (int)max(0ll, min(8ll, n - (at + 256 * u)));
+      if (inside) next[u].load(dy + at + 256 * u, true, 8);
+      else next[u].load(dy + at + 256 * u, vec, valid);
       next_w[u] = make_uint2(0u, 0u);
       next_s[u] = 0.f;
       if (valid > 0) {
-        if (ACT == ACT_RELU) next_w[u].x = saved[e0 >> 3];
-        else { next_w[u] = *reinterpret_cast<const uint2*>(saved + e0); next_s[u] = scales[e0 / kBlock]; }
+        if (ACT == ACT_RELU) next_w[u].x = sp[32 * u];
+        else { next_w[u] = *reinterpret_cast<const uint2*>(sp + 256 * u); next_s[u] = cp[2 * u]; }
       }
     }
   };
-  if (first < pieces) fetch(first);
-  for (long long piece = first; piece < pieces; piece += stride) {
+  auto work = [&](long long piece, auto full_tag) {
+    constexpr bool FULL = decltype(full_tag)::value;
+    const long long at = piece * kPiece + 8 * lane;
     float d[kActUnroll][8], s[kActUnroll];
     uint2 w[kActUnroll];
 #pragma unroll
@@ -228,15 +244,14 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
     if (piece + stride < pieces) fetch(piece + stride);
 #pragma unroll
     for (int u = 0; u < kActUnroll; ++u) {
-      const long long e0 = piece * kPiece + 256 * u + 8 * lane;
-      const int valid = (int)max(0ll, min(8ll, n - e0));
+      const int valid = FULL ? 8 : (int)max(0ll, min(8ll, n - (at + 256 * u)));
       float o[8];
       if (ACT == ACT_RELU) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = (w[u].x >> j) & 1u ? d[u][j] * keep_scale : 0.f;
       } else {
         unsigned keep = 0xffu;
-        if (DROP) keep = rng::keep_bits(rng::philox(key, (unsigned long long)(e0 >> 3)), threshold);
+        if (DROP) keep = rng::keep_bits(rng::philox(key, (unsigned long long)((at + 256 * u) >> 3)), threshold);
         const unsigned half[4] = {w[u].x & 0xffffu, w[u].x >> 16, w[u].y & 0xffffu, w[u].y >> 16};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -248,9 +263,14 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
           if (DROP) o[j] *= (keep >> j) & 1u ? keep_scale : 0.f;
         }
       }
-      store8(dx + e0, vec, valid, o);
+      store8(dx + at + 256 * u, FULL || vec, valid, o);
     }
-  }
+  };
+  if (first < pieces) fetch(first);
+  const long long whole = vec ? n / kPiece : 0;     // pieces that lie inside the tensor, aligned
+  long long piece = first;
+  for (; piece < whole; piece += stride) work(piece, std::true_type{});
+  for (; piece < pieces; piece += stride) work(piece, std::false_type{});
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
