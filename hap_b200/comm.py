@@ -54,6 +54,18 @@ def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
+def _launch(device, entry, *args) -> None:
+    """Call a C entry point whose last argument is the stream, on the tensors' device and its current stream."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        N.check(code)
+
+
 def _once(backward):
     """A backward pass made of kernels has no derivative of its own: ``once_differentiable``, which says so when a second
     derivative is asked for, without its cost in the ordinary case (a backward pass runs with gradients disabled)."""

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .comm import _on_device, _once, _stream
+from .comm import _launch, _on_device, _once, _stream
 
 _next_call_id = 0
 
@@ -178,17 +178,17 @@ def act_dropout(x: torch.Tensor, act: str, p: float, training: bool = True) -> t
 def _act8(x, act, p, call_id, keep):
     """The activation, and - ``keep`` - what its backward pass needs: gelu its input as e4m3 bytes followed by one float32
     scale per 128 consecutive elements, relu one bit per element (active and kept)."""
-    (x,) = _dense(x)
+    if not x.is_contiguous():
+        (x,) = _dense(x)
     n = x.numel()
     y = torch.empty_like(x)
     kept = saved = scales = None
     if keep:
         values = (n + 127) // 128 * 128 if act == 2 else (n + 7) // 8
-        kept = torch.empty(values + (values // 32 if act == 2 else 0), dtype=torch.uint8, device=x.device)
+        kept = x.new_empty(values + (values // 32 if act == 2 else 0), dtype=torch.uint8)
         saved = kept.data_ptr()
         scales = saved + values if act == 2 else None
-    with _on_device(x.device):
-        N.check(N.lib.hapx_act_dropout8(y.data_ptr(), saved, scales, x.data_ptr(), _code(x), n, act, p, call_id, _stream(x.device)))
+    _launch(x.device, N.lib.hapx_act_dropout8, y.data_ptr(), saved, scales, x.data_ptr(), _code(x), n, act, p, call_id)
     return y, kept
 
 
@@ -209,9 +209,8 @@ class _ActDropout8(torch.autograd.Function):
         dx = torch.empty_like(grad) if grad.is_contiguous() else torch.empty_strided(grad.shape, strides, dtype=grad.dtype, device=grad.device)
         n = grad.numel()
         saved = kept.data_ptr()
-        with _on_device(grad.device):
-            N.check(N.lib.hapx_act_dropout8_backward(dx.data_ptr(), grad.data_ptr(), saved, saved + (n + 127) // 128 * 128 if act == 2 else None,
-                                                     _code(grad), n, act, p, call_id, _stream(grad.device)))
+        _launch(grad.device, N.lib.hapx_act_dropout8_backward, dx.data_ptr(), grad.data_ptr(), saved,
+                saved + (n + 127) // 128 * 128 if act == 2 else None, _code(grad), n, act, p, call_id)
         return dx, None, None, None
 
 

@@ -23,7 +23,7 @@ import torch
 from . import _native as N
 from . import block8
 from .block8 import Block8, _CODES, _up
-from .comm import _on_device, _once, _stream
+from .comm import _launch, _on_device, _once
 
 _sizes = {}      # (device, shape, what is asked) -> workspace bytes
 
@@ -32,7 +32,8 @@ def _forward_workspace(device, m, n, k, prepared, keep_x) -> int:
     key = (device.index, m, n, k, prepared, keep_x)
     size = _sizes.get(key)
     if size is None:
-        size = _sizes[key] = N.lib.hapx_linear8_forward_workspace(m, n, k, prepared, keep_x)
+        with _on_device(device):
+            size = _sizes[key] = N.lib.hapx_linear8_forward_workspace(m, n, k, prepared, keep_x)
     return size
 
 
@@ -40,7 +41,8 @@ def _backward_workspace(device, m, n, k, dx, dw, db) -> int:
     key = (device.index, m, n, k, dx, dw, db)
     size = _sizes.get(key)
     if size is None:
-        size = _sizes[key] = N.lib.hapx_linear8_backward_workspace(m, n, k, dx, dw, db)
+        with _on_device(device):
+            size = _sizes[key] = N.lib.hapx_linear8_backward_workspace(m, n, k, dx, dw, db)
     return size
 
 
@@ -76,24 +78,22 @@ def _forward(x, weight, bias, prepared, keep_x, keep_w):
         ldw, w_ptr, w8_ptr, w8s_ptr = 0, None, prepared.values.data_ptr(), prepared.scales.data_ptr()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    y = torch.empty((*x.shape[:-1], n), dtype=dtype, device=device)
+    y = x.new_empty((*x.shape[:-1], n))
     if m == 0:
         keep_x = False
     kept = xt = xts = wt = wts = None
     if keep_x or keep_w:
         (xv, xs), (wv, ws_) = _kept_bytes(k, m) if keep_x else (0, 0), _kept_bytes(k, n) if keep_w else (0, 0)
-        kept = torch.empty(xv + xs + wv + ws_, dtype=torch.uint8, device=device)
+        kept = x.new_empty(xv + xs + wv + ws_, dtype=torch.uint8)
         base = kept.data_ptr()
         if keep_x:
             xt, xts = base, base + xv
         if keep_w:
             wt, wts = base + xv + xs, base + xv + xs + wv
-    with _on_device(device):
-        need = _forward_workspace(device, max(m, 1), n, k, prepared is not None, keep_x)
-        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        N.check(N.lib.hapx_linear8_forward(y.data_ptr(), x2.data_ptr(), ldx, w_ptr, ldw, w8_ptr, w8s_ptr,
-                                           bias.data_ptr() if bias is not None else None, _CODES[dtype], m, n, k, xt, xts, wt, wts,
-                                           work.data_ptr() if need else None, need, _stream(device)))
+    need = _forward_workspace(device, m or 1, n, k, prepared is not None, keep_x)
+    work = x.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(device, N.lib.hapx_linear8_forward, y.data_ptr(), x2.data_ptr(), ldx, w_ptr, ldw, w8_ptr, w8s_ptr,
+            bias.data_ptr() if bias is not None else None, _CODES[dtype], m, n, k, xt, xts, wt, wts, work.data_ptr() if need else None, need)
     return y, kept
 
 
@@ -116,9 +116,9 @@ class _Linear8(torch.autograd.Function):
         k = x_shape[-1]
         m = g.numel() // n
         g2, ldg = _rows(g)
-        dx = torch.empty(x_shape, dtype=dtype, device=device) if need_x else None
-        dw = torch.empty((n, k), dtype=dtype, device=device) if need_w else None
-        db = torch.empty(n, dtype=dtype, device=device) if need_b else None
+        dx = g.new_empty(x_shape) if need_x else None
+        dw = g.new_empty((n, k)) if need_w else None
+        db = g.new_empty(n) if need_b else None
         xt = xts = wt = wts = None
         xv, xs = _kept_bytes(k, m) if need_w and m else (0, 0)
         if need_w and m:
@@ -128,12 +128,10 @@ class _Linear8(torch.autograd.Function):
         elif need_x:
             wt = kept.data_ptr() + xv + xs
             wts = wt + _kept_bytes(k, n)[0]
-        with _on_device(device):
-            need = _backward_workspace(device, max(m, 1), n, k, need_x, need_w, need_b)
-            work = torch.empty(need, dtype=torch.uint8, device=device)
-            N.check(N.lib.hapx_linear8_backward(dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
-                                                db.data_ptr() if need_b else None, g2.data_ptr(), ldg, _CODES[dtype], m, n, k, wt, wts, xt, xts,
-                                                work.data_ptr(), need, _stream(device)))
+        need = _backward_workspace(device, m or 1, n, k, need_x, need_w, need_b)
+        work = g.new_empty(need, dtype=torch.uint8)
+        _launch(device, N.lib.hapx_linear8_backward, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                db.data_ptr() if need_b else None, g2.data_ptr(), ldg, _CODES[dtype], m, n, k, wt, wts, xt, xts, work.data_ptr(), need)
         return dx, dw, db, None
 
 
@@ -144,31 +142,32 @@ def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Opti
     the input needs the weight's transposed form (``quantize_weight(w, transposed=True)``)."""
     if not input.is_cuda:
         raise RuntimeError(f"linear8: hap_b200 has no CPU path; tensor is on {input.device}")
-    if input.dtype not in _CODES:
-        raise TypeError(f"linear8: operands must be bfloat16 or float32, got {input.dtype}")
-    if input.dim() < 1 or input.shape[-1] < 1:
-        raise ValueError(f"linear8: at least one input feature is expected, got shape {tuple(input.shape)}")
-    prepared = weight if isinstance(weight, Block8) else None
-    if prepared is not None:
+    dtype, shape = input.dtype, input.shape
+    if dtype not in _CODES:
+        raise TypeError(f"linear8: operands must be bfloat16 or float32, got {dtype}")
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"linear8: at least one input feature is expected, got shape {tuple(shape)}")
+    prepared = None
+    if isinstance(weight, Block8):
+        prepared, weight = weight, None
         if prepared.transposed is None and input.requires_grad and torch.is_grad_enabled():
             raise ValueError("linear8: the input's gradient needs the weight's transposed form: block8.quantize_weight(w, transposed=True)")
         fout, fin, device = prepared.rows, prepared.cols, prepared.device
-        weight = None
     else:
         if weight.dim() != 2 or weight.shape[0] < 1:
             raise ValueError(f"linear8: the weight must be (out_features, in_features), got shape {tuple(weight.shape)}")
-        if weight.dtype != input.dtype:
-            raise TypeError(f"linear8: mixed operand dtypes {input.dtype} and {weight.dtype}")
+        if weight.dtype != dtype:
+            raise TypeError(f"linear8: mixed operand dtypes {dtype} and {weight.dtype}")
         (fout, fin), device = weight.shape, weight.device
-    if fin != input.shape[-1]:
-        raise ValueError(f"linear8: input features {input.shape[-1]} != weight in_features {fin}")
+    if fin != shape[-1]:
+        raise ValueError(f"linear8: input features {shape[-1]} != weight in_features {fin}")
     if device != input.device:
         raise ValueError(f"linear8: input is on {input.device}, weight on {device}")
     if bias is not None:
-        if bias.dtype != input.dtype:
-            raise TypeError(f"linear8: mixed operand dtypes {input.dtype} and {bias.dtype}")
-        if tuple(bias.shape) != (fout,) or bias.device != input.device:
-            raise ValueError(f"linear8: the bias must be ({fout},) on {input.device}, got {tuple(bias.shape)} on {bias.device}")
+        if bias.dtype != dtype:
+            raise TypeError(f"linear8: mixed operand dtypes {dtype} and {bias.dtype}")
+        if bias.shape != (fout,) or bias.device != device:
+            raise ValueError(f"linear8: the bias must be ({fout},) on {device}, got {tuple(bias.shape)} on {bias.device}")
     if torch.is_grad_enabled() and (input.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _Linear8.apply(input, weight, bias, prepared)

@@ -12,7 +12,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native as N
-from .comm import _on_device, _once, _stream
+from .comm import _launch, _on_device, _once
 
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16}
 
@@ -137,12 +137,11 @@ def _norm8_forward(x, w, b, eps, keep):
     pitch, scales_at, stats_at, size = _kept8(rows, E)
     kept = saved = scales = mean = rstd = None
     if keep:
-        kept = torch.empty(size, dtype=torch.uint8, device=x.device)
+        kept = x.new_empty(size, dtype=torch.uint8)
         saved = kept.data_ptr()
         scales, mean, rstd = saved + scales_at, saved + stats_at, saved + stats_at + 4 * rows
-    with _on_device(x.device):
-        N.check(N.lib.hapx_layer_norm8_forward(xc.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), mean, rstd, saved, pitch, scales, _DTYPES[x.dtype],
-                                               rows, E, eps, _stream(x.device)))
+    _launch(x.device, N.lib.hapx_layer_norm8_forward, xc.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), mean, rstd, saved, pitch, scales,
+            _DTYPES[x.dtype], rows, E, eps)
     return y, kept
 
 
@@ -161,21 +160,20 @@ def _norm8_backward(ctx, dy, add):
     dy = dy.contiguous()
     add = None if add is None else add.contiguous()
     dx = torch.empty_like(dy)
-    dw = torch.empty(E, dtype=dtype, device=device) if ctx.need_w else None
-    db = torch.empty(E, dtype=dtype, device=device) if ctx.need_b else None
+    dw = dy.new_empty(E) if ctx.need_w else None
+    db = dy.new_empty(E) if ctx.need_b else None
     pitch, scales_at, stats_at, _ = _kept8(rows, E)
     saved = kept.data_ptr()
-    with _on_device(device):
-        work = None
-        if ctx.need_w or ctx.need_b:
-            key = (device.index, rows, E)
-            size = _work8.get(key)
-            if size is None:
+    work = None
+    if ctx.need_w or ctx.need_b:
+        key = (device.index, rows, E)
+        size = _work8.get(key)
+        if size is None:
+            with _on_device(device):
                 size = _work8[key] = N.lib.hapx_layer_norm8_backward_workspace(rows, E)
-            work = torch.empty(size, dtype=torch.uint8, device=device)
-        N.check(N.lib.hapx_layer_norm8_backward(saved, pitch, saved + scales_at, dy.data_ptr(), _ptr(w), saved + stats_at,
-                                                saved + stats_at + 4 * rows, _ptr(add), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work),
-                                                _DTYPES[dtype], rows, E, _stream(device)))
+        work = dy.new_empty(size, dtype=torch.uint8)
+    _launch(device, N.lib.hapx_layer_norm8_backward, saved, pitch, saved + scales_at, dy.data_ptr(), _ptr(w), saved + stats_at,
+            saved + stats_at + 4 * rows, _ptr(add), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work), _DTYPES[dtype], rows, E)
     return dx, dw, db, None
 
 
@@ -207,8 +205,8 @@ class _LayerNormFork8(torch.autograd.Function):
         return _norm8_backward(ctx, dy, d_residual)
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _wants_grad(x, w, b) -> bool:
+    return torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad) or (b is not None and b.requires_grad))
 
 
 def _check8(what, input, shape, weight, bias):
@@ -219,7 +217,7 @@ def _check8(what, input, shape, weight, bias):
     if len(shape) != 1 or input.dim() < 1 or input.shape[-1] != shape[0] or shape[0] < 1:
         raise ValueError(f"{what}: normalises the last dimension only, got normalized_shape {shape} for an input of shape {tuple(input.shape)}")
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.dtype != input.dtype or tuple(t.shape) != shape or t.device != input.device):
+        if t is not None and (t.dtype != input.dtype or t.shape != shape or t.device != input.device):
             raise ValueError(f"{what}: the {name} must be {shape}, {input.dtype}, on {input.device}; got {tuple(t.shape)}, {t.dtype}, on {t.device}")
 
 
