@@ -27,6 +27,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "hapx_internal.h"
 #include "hapx_tc.h"
@@ -41,7 +42,8 @@ constexpr int BK = 128;      // one block of the contraction: one 128-byte swizz
 constexpr int UMMA_K = 32;
 constexpr unsigned kAtom = 512;      // scales of 128 rows x 4 blocks
 
-struct Params {
+// One product of a launch.
+struct Problem {
   int M, N, k_blocks;
   void* D; long long ldd;
   const void* bias;          // N values of D's type, or null
@@ -49,8 +51,19 @@ struct Params {
   int m_tiles, n_tiles;
   int splits, kb_per_split;  // > 1: the blocks are cut into ranges; each writes a float32 partial tile to rows [split * m_pad, ...)
   long long m_pad;
+  const float* colsum;       // null, or colsum_tiles x M floats whose column sums go to colsum_out (the bias gradient that
+  int colsum_tiles;          // belongs to a weight gradient: see the epilogue)
+  int colsum_f32;
+  void* colsum_out;
+};
+// One or two products; units (tile, range of blocks) of the first, which has the longer ones, are dealt out first.
+struct Params {
+  Problem pr[2];
+  int units[2];
+  int rounds;                // of the second product's units that every worker takes part in: see the kernel
   unsigned* error;
 };
+struct Maps { CUtensorMap a[2], b[2], sa[2], sb[2], d[2]; };
 
 template <bool PAIR>
 __device__ __forceinline__ void umma8(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned sfa, unsigned sfb,
@@ -125,7 +138,7 @@ __device__ __forceinline__ void stage_row(unsigned char* row, int sw, const floa
 }
 
 // v[j] += bias[n + j] (float32) for the columns inside the matrix; `vec`: all are, and the bias lies on 16 bytes.
-__device__ __forceinline__ void add_bias(const Params& p, int n, bool vec, float (&v)[32]) {
+__device__ __forceinline__ void add_bias(const Problem& p, int n, bool vec, float (&v)[32]) {
   const float* bias = static_cast<const float*>(p.bias) + n;
   if (vec) {
 #pragma unroll
@@ -142,8 +155,7 @@ __device__ __forceinline__ void add_bias(const Params& p, int n, bool vec, float
 
 template <bool PAIR>
 __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
-gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
-             const __grid_constant__ CUtensorMap tmSB, const __grid_constant__ CUtensorMap tmD, const Params p) {
+gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params params) {
   using C = Cfg<PAIR>;
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -160,27 +172,41 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = PAIR ? (int)cluster_ctarank() : 0;       // 0 leads the pair
   const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
-  const int units = p.m_tiles * p.n_tiles * p.splits;
-  struct Unit { int m0, n0, split, kb0, kb1; };
-  auto decode = [&](int unit) {
-    Unit u;
+  // A worker's units in order: its share of the first product's, dealt round by round; then of the second's - `rounds`
+  // rounds over all workers, and what is left over the workers that had no unit in the first product's last, partly
+  // filled round.  So the longer units of one product and the shorter ones of the other even out without a counter in
+  // memory.
+  const int left = params.units[0] % workers, own0 = params.units[0] / workers + (worker < left ? 1 : 0);
+  struct Unit { int which, m0, n0, split, kb0, kb1; };
+  auto next_unit = [&](int step, Unit& u) {
+    int unit = step * workers + worker;
+    u.which = step >= own0;
+    if (u.which) {
+      const int t = step - own0;
+      if (t < params.rounds) unit = t * workers + worker;
+      else if (worker >= left) unit = params.rounds * workers + (t - params.rounds) * (workers - left) + worker - left;
+      else return false;
+      if (unit >= params.units[1]) return false;
+    }
+    const Problem& p = params.pr[u.which];
     const int tile = unit / p.splits;
     u.split = unit - tile * p.splits;
     u.m0 = (tile % p.m_tiles) * (PAIR ? 2 * BM : BM) + cta * BM;
     u.n0 = (tile / p.m_tiles) * C::BN;
     u.kb0 = u.split * p.kb_per_split;
     u.kb1 = min(u.kb0 + p.kb_per_split, p.k_blocks);
-    return u;
+    return true;
   };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), (PAIR ? 2 : 1) * C::EPI_WARPS); }
     fence_barrier_init();
-    prefetch_tensormap(&tmA);
-    prefetch_tensormap(&tmB);
-    prefetch_tensormap(&tmSA);
-    prefetch_tensormap(&tmSB);
+    const int which = own0 == 0;
+    prefetch_tensormap(&maps.a[which]);
+    prefetch_tensormap(&maps.b[which]);
+    prefetch_tensormap(&maps.sa[which]);
+    prefetch_tensormap(&maps.sb[which]);
   }
   if (warp == 1) {
     if (PAIR) { tmem_alloc2(tmem_slot, C::TMEM_COLS); tmem_relinquish2(); }
@@ -197,8 +223,8 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     int stage = 0;
     unsigned phase = 0;
     bool ok = true;
-    for (int unit = worker; unit < units && ok; unit += workers) {
-      const Unit u = decode(unit);
+    Unit u;
+    for (int step = 0; ok && next_unit(step, u); ++step) {
       for (int kb = u.kb0; kb < u.kb1; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u));
         if (!ok) break;
@@ -211,19 +237,19 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
           if (PAIR) {
             const unsigned bar = map_to_cta(full_bar(stage), 0);
             if (cta == 0) mbar_expect_tx(full_bar(stage), 2 * bytes);     // the bytes of both CTAs
-            tma_load_4d_pair(sa, &tmA, kb * BK, u.m0, 0, 0, bar);
-            tma_load_4d_pair(sb, &tmB, kb * BK, u.n0 + cta * (C::BN / 2), 0, 0, bar);
+            tma_load_4d_pair(sa, &maps.a[u.which], kb * BK, u.m0, 0, 0, bar);
+            tma_load_4d_pair(sb, &maps.b[u.which], kb * BK, u.n0 + cta * (C::BN / 2), 0, 0, bar);
             if (scales) {
-              tma_load_4d_pair(ss, &tmSA, 0, u.m0 >> 7, kb >> 2, 0, bar);
-              tma_load_4d_pair(ss + kAtom, &tmSB, 0, u.n0 >> 7, kb >> 2, 0, bar);
+              tma_load_4d_pair(ss, &maps.sa[u.which], 0, u.m0 >> 7, kb >> 2, 0, bar);
+              tma_load_4d_pair(ss + kAtom, &maps.sb[u.which], 0, u.n0 >> 7, kb >> 2, 0, bar);
             }
           } else {
             mbar_expect_tx(full_bar(stage), bytes);
-            tma_load_4d(sa, &tmA, kb * BK, u.m0, 0, 0, full_bar(stage));
-            tma_load_4d(sb, &tmB, kb * BK, u.n0, 0, 0, full_bar(stage));
+            tma_load_4d(sa, &maps.a[u.which], kb * BK, u.m0, 0, 0, full_bar(stage));
+            tma_load_4d(sb, &maps.b[u.which], kb * BK, u.n0, 0, 0, full_bar(stage));
             if (scales) {
-              tma_load_4d(ss, &tmSA, 0, u.m0 >> 7, kb >> 2, 0, full_bar(stage));
-              tma_load_4d(ss + kAtom, &tmSB, 0, u.n0 >> 7, kb >> 2, 0, full_bar(stage));
+              tma_load_4d(ss, &maps.sa[u.which], 0, u.m0 >> 7, kb >> 2, 0, full_bar(stage));
+              tma_load_4d(ss + kAtom, &maps.sb[u.which], 0, u.n0 >> 7, kb >> 2, 0, full_bar(stage));
             }
           }
         }
@@ -231,7 +257,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok && lane == 0) atomicCAS(p.error, 0u, 1u);
+    if (!ok && lane == 0) atomicCAS(params.error, 0u, 1u);
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
     if (cta == 0) {
@@ -240,8 +266,8 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
       bool ok = true;
       // descriptors of the first 32 bytes of a stage; a stage or a step of 32 further on is an addition to the address field
       const unsigned long long desc_a = make_desc(base, 16u, 1024u), desc_b = make_desc(base + C::A_BYTES, 16u, 1024u);
-      for (int unit = worker; unit < units && ok; unit += workers) {
-        const Unit u = decode(unit);
+      Unit u;
+      for (int step = 0; ok && next_unit(step, u); ++step) {
         const unsigned d = tmem_base + (unsigned)(acc * C::BN), shift = (unsigned)(u.n0 >> 5) & 3u;   // B's rows start inside a group of 128
         unsigned sf = 0;
         ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), acc_phase ^ 1u));
@@ -277,7 +303,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         if (!ok) break;
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      if (!ok && lane == 0) atomicCAS(p.error, 0u, 2u);
+      if (!ok && lane == 0) atomicCAS(params.error, 0u, 2u);
     }
   } else {
     // ---------------- epilogue: 32 rows x 64 columns of the tile per warp ----------------
@@ -287,14 +313,26 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     int acc = 0;
     unsigned acc_phase = 0;
     bool ok = true;
-    for (int unit = worker; unit < units; unit += workers) {
-      const Unit u = decode(unit);
+    Unit u;
+    for (int step = 0; next_unit(step, u); ++step) {
+      const Problem& p = params.pr[u.which];
+      if (p.colsum && u.n0 == 0 && part == 0 && u.split == 0) {
+        // the bias gradient of a weight gradient's rows: the partial column sums of the quantiser, added in their order
+        // by the warps that have to wait for this tile anyway
+        const int row = u.m0 + q * 32 + lane;
+        if (row < p.M) {
+          float sum = 0.f;
+#pragma unroll 8
+          for (int i = 0; i < p.colsum_tiles; ++i) sum += __ldg(p.colsum + (long long)i * p.M + row);
+          if (p.colsum_f32) static_cast<float*>(p.colsum_out)[row] = sum;
+          else static_cast<__nv_bfloat16*>(p.colsum_out)[row] = __float2bfloat16_rn(sum);
+        }
+      }
       const int n0 = u.n0 + 64 * part, width = min(64, p.N - n0);   // this warp's columns inside the matrix (may be none)
       const bool bias_vec = p.bias_vec && width == 64;
-      uint4 braw[8];
-      if (!p.out_f32 && bias_vec) {                          // travels during the wait
-#pragma unroll
-        for (int j = 0; j < 8; ++j) braw[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + n0) + j);
+      if (bias_vec && lane == 0) {                           // comes closer during the wait
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + (long long)n0 * (p.out_f32 ? 4 : 2)));
+        if (p.out_f32) asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + (long long)n0 * 4 + 128));
       }
       ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
       if (!ok) break;
@@ -317,22 +355,29 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            tma_store_4d(&tmD, tile_u32, n0 + c, (int)out_row0, 0, 0);
+            tma_store_4d(&maps.d[u.which], tile_u32, n0 + c, (int)out_row0, 0, 0);
             bulk_commit_group();
           }
         } else {
           __syncwarp();
           const int rows = min(32, p.M - (u.m0 + q * 32));
-          for (int i = 0; i < rows; ++i) {
+          constexpr int ES = OUT_F32 ? 4 : 2;
+          using Bits = typename std::conditional<OUT_F32, unsigned, unsigned short>::type;
 #pragma unroll
-            for (int h = 0; h < W / 32; ++h) {
-              const int col = lane + 32 * h, byte = col * (OUT_F32 ? 4 : 2);
-              const unsigned char* src = tile_gen + i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15);
-              if (c + col < width) {
-                const long long at = (out_row0 + i) * p.ldd + n0 + c + col;
-                if (OUT_F32) static_cast<float*>(p.D)[at] = *reinterpret_cast<const float*>(src);
-                else static_cast<__nv_bfloat16*>(p.D)[at] = *reinterpret_cast<const __nv_bfloat16*>(src);
-              }
+          for (int h = 0; h < W / 32; ++h) {
+            const int col = lane + 32 * h, byte = col * ES;
+            if (c + col >= width) continue;
+            const unsigned char* src = tile_gen + (byte & 15);
+            Bits* dst = static_cast<Bits*>(p.D) + out_row0 * p.ldd + n0 + c + col;
+#pragma unroll 1
+            for (int i0 = 0; i0 < rows; i0 += 8) {           // eight rows in flight
+              Bits v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const Bits*>(src + (i0 + i) * 128 + (((byte >> 4) ^ i) << 4));
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i0 + i < rows) dst[i * p.ldd] = v[i];
+              dst += 8 * p.ldd;
             }
           }
           __syncwarp();
@@ -371,7 +416,8 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         if (bias_vec) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const unsigned w[4] = {braw[j].x, braw[j].y, braw[j].z, braw[j].w};
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + n0) + j);
+            const unsigned w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) { v[8 * j + 2 * e] += __uint_as_float(w[e] << 16); v[8 * j + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u); }
           }
@@ -387,7 +433,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) bulk_wait_all();
-    if (!ok) atomicCAS(p.error, 0u, 3u);
+    if (!ok) atomicCAS(params.error, 0u, 3u);
   }
 
   tc_fence_before();
@@ -449,35 +495,85 @@ static int make_map(CUtensorMap* map, const void* ptr, CUtensorMapDataType type,
   return HAPX_OK;
 }
 
-// How a product is cut: the pair kernel or the single one, and into how many ranges of blocks.
-struct Plan { bool pair; int splits, kb_per_split; long long m_pad; int n_pad; };
+// How a product is cut: by the pair kernel or the single one, and into how many ranges of blocks.
+struct Plan { bool pair; int splits, kb_per_split; long long m_pad, tiles; int n_pad, blocks; };
 
-static Plan plan_of(long long M, long long N, long long K, int sm_count) {
+static Plan plan_whole(long long M, long long N, long long K, bool pair) {
   Plan pl;
-  pl.pair = M > BM;
-  const long long bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true>::BN : Cfg<false>::BN;
-  const long long m_tiles = (M + bm - 1) / bm, tiles = m_tiles * ((N + bn - 1) / bn);
-  const int blocks = (int)((K + BK - 1) / BK), workers = pl.pair ? sm_count / 2 : sm_count;
-  pl.splits = 1; pl.kb_per_split = blocks; pl.m_pad = m_tiles * bm; pl.n_pad = (int)((N + 3) / 4 * 4);
-  // A long contraction over few tiles leaves SMs idle, or the last round of tiles nearly empty: cut the blocks into
-  // ranges whose float32 partial tiles a second kernel adds in a fixed order.  In microseconds: rounds x blocks x the
-  // time of one block, and for a split the partial tiles written and read back at about 4 TB/s plus a launch.
-  const double block_us = pl.pair ? 0.25 : 0.15, partial = 8.0 * (double)pl.m_pad * pl.n_pad / 4e6;
-  auto rounds = [&](long long units) { return (double)((units + workers - 1) / workers); };
-  double best = rounds(tiles) * blocks * block_us;
-  for (int sp = 2; sp <= 16 && sp * 4 <= blocks; ++sp) {
-    const int per = (blocks + sp - 1) / sp;
-    if ((sp - 1) * per >= blocks) continue;                 // an empty last range
-    if (4.0 * sp * (double)pl.m_pad * pl.n_pad > 512e6) break;
-    const double cost = rounds(tiles * sp) * per * block_us + 3.0 + sp * partial;
-    if (cost < 0.9 * best) { pl.splits = sp; pl.kb_per_split = per; best = cost; }
-  }
+  pl.pair = pair;
+  const long long bm = pair ? 2 * BM : BM, bn = pair ? Cfg<true>::BN : Cfg<false>::BN, m_tiles = (M + bm - 1) / bm;
+  pl.tiles = m_tiles * ((N + bn - 1) / bn);
+  pl.blocks = (int)((K + BK - 1) / BK);
+  pl.splits = 1; pl.kb_per_split = pl.blocks; pl.m_pad = m_tiles * bm; pl.n_pad = (int)((N + 3) / 4 * 4);
   return pl;
 }
+static bool cut(Plan& pl, int splits) {        // false where a range would be empty or the partial tiles too large
+  const int per = (pl.blocks + splits - 1) / splits;
+  if (splits > 1 && (splits * 4 > pl.blocks || (splits - 1) * per >= pl.blocks || 4.0 * splits * (double)pl.m_pad * pl.n_pad > 512e6)) return false;
+  pl.splits = splits; pl.kb_per_split = per;
+  return true;
+}
+// Microseconds of one block of a tile (measured: 0.30 to 0.33 of a pair's 256 x 192, long contractions), and of a split:
+// its partial tiles written and read back at about 4 TB/s plus a launch.
+static double block_us(bool pair) { return pair ? 0.30 : 0.15; }
+static double split_us(const Plan& pl) { return pl.splits > 1 ? 3.0 + pl.splits * 8.0 * (double)pl.m_pad * pl.n_pad / 4e6 : 0.0; }
+
+// A long contraction over few tiles leaves SMs idle, or the last round of tiles nearly empty: cut the blocks into ranges
+// whose float32 partial tiles a second kernel adds in a fixed order, where that costs less by a clear margin.
+static Plan plan_of(long long M, long long N, long long K, int sm_count) {
+  Plan best = plan_whole(M, N, K, M > BM), pl = best;
+  const int workers = pl.pair ? sm_count / 2 : sm_count;
+  auto cost = [&](const Plan& q) { return (double)((q.tiles * q.splits + workers - 1) / workers) * q.kb_per_split * block_us(q.pair) + split_us(q); };
+  for (int sp = 2; sp <= 16; ++sp)
+    if (cut(pl, sp) && cost(pl) < 0.9 * cost(best)) best = pl;
+  return best;
+}
+
+// Blocks until the last worker is done with two products dealt out as the kernel does it, the longer units first; and
+// the number of rounds of the second product's units for all workers.
+static long long makespan(const Plan& a, const Plan& b, int workers, int* rounds) {
+  const long long ua = a.tiles * a.splits, ub = b.tiles * b.splits, la = a.kb_per_split, lb = b.kb_per_split;
+  const long long full = ua / workers, left = ua % workers;
+  if (left == 0) {
+    *rounds = (int)((ub + workers - 1) / workers);
+    return full * la + *rounds * lb;
+  }
+  const long long ideal = (ua * la + ub * lb + workers - 1) / workers, guess = std::max(0ll, (ideal - (full + 1) * la) / lb);
+  long long best = -1;
+  for (long long r = guess; r <= guess + 1; ++r) {
+    const long long all = std::min(r, (ub + workers - 1) / workers), rest = std::max(0ll, ub - all * workers);
+    const long long more = (rest + workers - left - 1) / (workers - left);
+    const long long t = std::max((full + 1) * la + (ub > 0 ? all : 0) * lb, full * la + (all + more) * lb);
+    if (best < 0 || t < best) { best = t; *rounds = (int)all; }
+  }
+  return best;
+}
+
+// Two products in one launch of the pair kernel: which goes first, its cut, the other's.
+struct PairPlan { Plan pl[2]; int first, rounds; };
+static PairPlan plan_two(const Product& x, const Product& y, int sm_count) {
+  const Plan whole[2] = {plan_whole(x.m, x.n, x.k, true), plan_whole(y.m, y.n, y.k, true)};
+  const int workers = sm_count / 2;
+  PairPlan best;
+  double best_us = -1.0;
+  for (int cx = 1; cx <= 16; cx = cx < 4 ? cx + 1 : cx * 2) {
+    for (int cy = 1; cy <= 16; cy = cy < 4 ? cy + 1 : cy * 2) {
+      if (cx > 1 && cy > 1) continue;                       // one of the two at most
+      PairPlan t;
+      t.pl[0] = whole[0]; t.pl[1] = whole[1];
+      if (!cut(t.pl[0], cx) || !cut(t.pl[1], cy)) continue;
+      t.first = t.pl[1].kb_per_split > t.pl[0].kb_per_split;
+      const double us = makespan(t.pl[t.first], t.pl[!t.first], workers, &t.rounds) * block_us(true) + split_us(t.pl[0]) + split_us(t.pl[1]);
+      if (best_us < 0.0 || us < 0.9 * best_us) { best = t; best_us = us; }
+    }
+  }
+  return best;
+}
+
+static long long partial_bytes(const Plan& pl) { return pl.splits > 1 ? pl.splits * pl.m_pad * pl.n_pad * 4 : 0; }
 
 template <bool PAIR>
-static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmSA, const CUtensorMap& tmSB, const CUtensorMap& tmD,
-                  const Params& p, int sm_count, cudaStream_t stream) {
+static int launch(const Maps& maps, const Params& p, int sm_count, cudaStream_t stream) {
   using C = Cfg<PAIR>;
   auto kernel = gemm8_kernel<PAIR>;
   static int limit_of[64] = {};             // per device: function attributes and occupancy belong to one
@@ -509,10 +605,10 @@ static int launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensor
       limit_of[device] = limit;
     }
   }
-  const long long units = (long long)p.m_tiles * p.n_tiles * p.splits;
-  if (units > 0x7fffffff) return fail(HAPX_ERR_EXTENT, "block8_matmul: too many tiles");
-  cfg.gridDim = dim3((unsigned)std::min<long long>(units, limit) * (PAIR ? 2 : 1));
-  HAPX_CUDA(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmSA, tmSB, tmD, p));
+  // one product: no more workers than units; two: as many as the plan dealt them out to
+  const int workers = PAIR && p.units[1] > 0 ? std::min(limit, sm_count / 2) : std::min(p.units[0], limit);
+  cfg.gridDim = dim3((unsigned)(workers * (PAIR ? 2 : 1)));
+  HAPX_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, p));
   count_launch();
   return HAPX_OK;
 }
@@ -532,48 +628,81 @@ static int make_scale_map(CUtensorMap* map, const void* ptr, long long rows, int
   return HAPX_OK;
 }
 
-long long workspace_bytes(long long m, long long n, long long k, int sm_count) {
-  const Plan pl = plan_of(m, n, k, sm_count);
-  return pl.splits > 1 ? pl.splits * pl.m_pad * pl.n_pad * 4 : 0;
+long long workspace_bytes(long long m, long long n, long long k, int sm_count) { return partial_bytes(plan_of(m, n, k, sm_count)); }
+
+// One product as entry i of a launch; `partial`: where its partial tiles go.
+static int describe(const Product& pr, const Plan& pl, void* partial, int i, Maps* maps, Params* params) {
+  const long long M = pr.m, N = pr.n, K = pr.k;
+  const int bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true>::BN : Cfg<false>::BN;
+  Problem& p = params->pr[i];
+  p = Problem();
+  p.M = (int)M; p.N = (int)N; p.k_blocks = pl.blocks;
+  p.splits = pl.splits; p.kb_per_split = pl.kb_per_split; p.m_pad = pl.m_pad;
+  p.m_tiles = (p.M + bm - 1) / bm; p.n_tiles = (p.N + bn - 1) / bn;
+  if (pl.tiles * pl.splits > 0x3fffffff) return fail(HAPX_ERR_EXTENT, "block8_matmul: too many tiles");
+  params->units[i] = (int)(pl.tiles * pl.splits);
+  long long out_rows = M;
+  if (pl.splits > 1) { p.D = partial; p.ldd = pl.n_pad; p.out_f32 = 1; p.bias = nullptr; out_rows = pl.splits * pl.m_pad; }
+  else { p.D = pr.d; p.ldd = N; p.out_f32 = pr.out_f32; p.bias = pr.bias; }
+  p.bias_vec = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
+  p.colsum = pr.colsum; p.colsum_tiles = pr.colsum_tiles; p.colsum_f32 = pr.out_f32; p.colsum_out = pr.colsum_out;
+  const int es = p.out_f32 ? 4 : 2;
+  if (int e = make_map(&maps->a[i], pr.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, pr.lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
+  if (int e = make_map(&maps->b[i], pr.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, pr.ldb, BK, pl.pair ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
+  if (int e = make_scale_map(&maps->sa[i], pr.a_scale, M, p.k_blocks, 1)) return e;
+  if (int e = make_scale_map(&maps->sb[i], pr.b_scale, N, p.k_blocks, pl.pair ? Cfg<true>::B_ATOMS : Cfg<false>::B_ATOMS)) return e;
+  p.tma_store = (reinterpret_cast<uintptr_t>(p.D) & 15u) == 0 && (p.ldd * es) % 16 == 0;
+  if (p.tma_store)
+    return make_map(&maps->d[i], p.D, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, pl.splits > 1 ? pl.n_pad : N,
+                    out_rows, p.ldd, 128 / es, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+  return HAPX_OK;
+}
+
+static int join(const Product& pr, const Plan& pl, const void* partial, int sm_count, cudaStream_t stream) {
+  if (pl.splits == 1) return HAPX_OK;
+  const int grid = (int)std::min<long long>((pr.m * (pl.n_pad / 4) + 255) / 256, (long long)sm_count * 8);
+  const float* ws = static_cast<const float*>(partial);
+  if (pr.out_f32) gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, pr.m, (int)pr.n, pl.m_pad, pl.n_pad, static_cast<const float*>(pr.bias),
+                                                              static_cast<float*>(pr.d));
+  else gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, pr.m, (int)pr.n, pl.m_pad, pl.n_pad, static_cast<const __nv_bfloat16*>(pr.bias),
+                                                   static_cast<__nv_bfloat16*>(pr.d));
+  HAPX_CUDA(cudaGetLastError());
+  count_launch();
+  return HAPX_OK;
 }
 
 int run(const Product& pr, int sm_count, cudaStream_t stream) {
-  unsigned* error = nullptr;
-  if (int e = gemm::error_word(&error, nullptr)) return e;
-  const long long M = pr.m, N = pr.n, K = pr.k;
-  const Plan pl = plan_of(M, N, K, sm_count);
-  Params p = Params();
-  p.M = (int)M; p.N = (int)N; p.k_blocks = (int)((K + BK - 1) / BK);
-  p.splits = pl.splits; p.kb_per_split = pl.kb_per_split; p.m_pad = pl.m_pad;
-  p.error = error;
-  const int bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true>::BN : Cfg<false>::BN;
-  p.m_tiles = (p.M + bm - 1) / bm; p.n_tiles = (p.N + bn - 1) / bn;
-  long long out_rows = M;
-  if (pl.splits > 1) { p.D = pr.workspace; p.ldd = pl.n_pad; p.out_f32 = 1; p.bias = nullptr; out_rows = pl.splits * pl.m_pad; }
-  else { p.D = pr.d; p.ldd = N; p.out_f32 = pr.out_f32; p.bias = pr.bias; }
-  p.bias_vec = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
-  const int es = p.out_f32 ? 4 : 2;
-  CUtensorMap tmA, tmB, tmSA, tmSB, tmD;
-  std::memset(&tmD, 0, sizeof(tmD));
-  if (int e = make_map(&tmA, pr.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, pr.lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
-  if (int e = make_map(&tmB, pr.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, pr.ldb, BK, pl.pair ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
-                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
-  if (int e = make_scale_map(&tmSA, pr.a_scale, M, p.k_blocks, 1)) return e;
-  if (int e = make_scale_map(&tmSB, pr.b_scale, N, p.k_blocks, pl.pair ? Cfg<true>::B_ATOMS : Cfg<false>::B_ATOMS)) return e;
-  p.tma_store = (reinterpret_cast<uintptr_t>(p.D) & 15u) == 0 && (p.ldd * es) % 16 == 0;
-  if (p.tma_store)
-    if (int e = make_map(&tmD, p.D, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, pl.splits > 1 ? pl.n_pad : N,
-                         out_rows, p.ldd, 128 / es, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE)) return e;
-  if (int e = pl.pair ? launch<true>(tmA, tmB, tmSA, tmSB, tmD, p, sm_count, stream) : launch<false>(tmA, tmB, tmSA, tmSB, tmD, p, sm_count, stream)) return e;
-  if (pl.splits > 1) {
-    const int grid = (int)std::min<long long>((M * (pl.n_pad / 4) + 255) / 256, (long long)sm_count * 8);
-    const float* ws = static_cast<const float*>(pr.workspace);
-    if (pr.out_f32) gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, M, p.N, pl.m_pad, pl.n_pad, static_cast<const float*>(pr.bias), static_cast<float*>(pr.d));
-    else gemm8_join_kernel<<<grid, 256, 0, stream>>>(ws, pl.splits, M, p.N, pl.m_pad, pl.n_pad, static_cast<const __nv_bfloat16*>(pr.bias),
-                                                     static_cast<__nv_bfloat16*>(pr.d));
-    HAPX_CUDA(cudaGetLastError());
-    count_launch();
-  }
+  Params params = Params();
+  Maps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  if (int e = gemm::error_word(&params.error, nullptr)) return e;
+  const Plan pl = plan_of(pr.m, pr.n, pr.k, sm_count);
+  if (int e = describe(pr, pl, pr.workspace, 0, &maps, &params)) return e;
+  if (int e = pl.pair ? launch<true>(maps, params, sm_count, stream) : launch<false>(maps, params, sm_count, stream)) return e;
+  return join(pr, pl, pr.workspace, sm_count, stream);
+}
+
+long long workspace_bytes_two(const Product& x, const Product& y, int sm_count) {
+  const PairPlan t = plan_two(x, y, sm_count);
+  return partial_bytes(t.pl[0]) + partial_bytes(t.pl[1]);
+}
+
+int run_two(const Product& x, const Product& y, int sm_count, cudaStream_t stream) {
+  Params params = Params();
+  Maps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  if (int e = gemm::error_word(&params.error, nullptr)) return e;
+  const PairPlan t = plan_two(x, y, sm_count);
+  const Product* pr[2] = {&x, &y};
+  void* partial[2] = {x.workspace, static_cast<char*>(x.workspace) + partial_bytes(t.pl[0])};
+  for (int i = 0; i < 2; ++i)
+    if (int e = describe(*pr[i], t.pl[i], partial[i], i == t.first ? 0 : 1, &maps, &params)) return e;
+  params.rounds = t.rounds;
+  if (int e = launch<true>(maps, params, sm_count, stream)) return e;
+  for (int i = 0; i < 2; ++i)
+    if (int e = join(*pr[i], t.pl[i], partial[i], sm_count, stream)) return e;
   return HAPX_OK;
 }
 

@@ -87,9 +87,15 @@ struct Product {
   const void* bias = nullptr;
   long long m = 0, n = 0, k = 0;
   void* workspace = nullptr;
+  // null, or colsum_tiles x m floats: the launch also writes their column sums, added in order, to colsum_out (m values
+  // of d's type)
+  const float* colsum = nullptr; int colsum_tiles = 0; void* colsum_out = nullptr;
 };
 long long workspace_bytes(long long m, long long n, long long k, int sm_count);
 int run(const Product& p, int sm_count, cudaStream_t stream);
+// Two independent products in one launch (x.workspace serves both).
+long long workspace_bytes_two(const Product& x, const Product& y, int sm_count);
+int run_two(const Product& x, const Product& y, int sm_count, cudaStream_t stream);
 }  // namespace gemm8
 
 // Multiprocessors of the current device (asked for once per device).

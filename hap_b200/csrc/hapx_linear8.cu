@@ -2,7 +2,7 @@
 //
 // Forward: x in 1 x 128 blocks (and, for the weight gradient, in 128 x 1 blocks, transposed), w in 128 x 128 tiles (and
 // transposed, for the input gradient), both in one launch, then the product.  Backward: g likewise in both forms from one
-// read, with the partial sums of the bias gradient, then the two products.
+// read, with the partial sums of the bias gradient, then the two products in one launch, which joins those sums.
 //
 // A few tokens through a weight that is already in 8 bits (thin_kernel) need no tensor cores: the time is that of one
 // launch and of reading the weight.  Every thread block makes the 8-bit form of x for itself in shared memory, a warp
@@ -152,9 +152,17 @@ static Backward layout_backward(void* base, long long m, long long n, long long 
   if (dx || !dw) { b.g8 = c.take(m * up(n, 16)); b.g8s = c.take(scale_bytes(m, n)); }      // the quantiser writes one form at least
   if (dw) { b.g8t = c.take(n * up(m, 16)); b.g8ts = c.take(scale_bytes(n, m)); }
   if (db) b.colsum = c.take((m + kBlock - 1) / kBlock * n * 4);
-  long long split = 0;                                                                        // one after the other on the stream
-  if (dx) split = gemm8::workspace_bytes(m, k, n, n_sm);
-  if (dw) split = std::max(split, gemm8::workspace_bytes(n, k, m, n_sm));
+  long long split = 0;
+  if (dx && dw) {
+    gemm8::Product x, w;
+    x.m = m; x.n = k; x.k = n;
+    w.m = n; w.n = k; w.k = m;
+    split = gemm8::workspace_bytes_two(x, w, n_sm);
+  } else if (dx) {
+    split = gemm8::workspace_bytes(m, k, n, n_sm);
+  } else if (dw) {
+    split = gemm8::workspace_bytes(n, k, m, n_sm);
+  }
   b.split = c.take(split);
   b.bytes = c.used;
   return b;
@@ -267,18 +275,21 @@ int hapx_linear8_backward(void* dx, void* dw, void* db, const void* g, int64_t l
   j.x = g; j.rows = m; j.cols = n; j.ldx = ldg; j.q = b.g8; j.ldq = up(n, 16); j.s = b.g8s; j.qt = b.g8t; j.ldqt = up(m, 16); j.st = b.g8ts;
   j.colsum = reinterpret_cast<float*>(b.colsum);
   if (int e = quantize(&j, 1, dtype, stream)) return e;
-  gemm8::Product p;
-  p.out_f32 = dtype == HAPX_F32; p.workspace = b.split;
+  gemm8::Product px, pw;
   if (dx) {
-    p.d = dx; p.a = b.g8; p.lda = up(n, 16); p.a_scale = b.g8s; p.b = w8t; p.ldb = up(n, 16); p.b_scale = w8t_scale; p.m = m; p.n = k; p.k = n;
-    if (int e = gemm8::run(p, n_sm, stream)) return e;
+    px.d = dx; px.out_f32 = dtype == HAPX_F32; px.a = b.g8; px.lda = up(n, 16); px.a_scale = b.g8s; px.b = w8t; px.ldb = up(n, 16);
+    px.b_scale = w8t_scale; px.m = m; px.n = k; px.k = n; px.workspace = b.split;
   }
   if (dw) {
-    p.d = dw; p.a = b.g8t; p.lda = up(m, 16); p.a_scale = b.g8ts; p.b = x8t; p.ldb = up(m, 16); p.b_scale = x8t_scale; p.m = n; p.n = k; p.k = m;
-    if (int e = gemm8::run(p, n_sm, stream)) return e;
+    pw.d = dw; pw.out_f32 = dtype == HAPX_F32; pw.a = b.g8t; pw.lda = up(m, 16); pw.a_scale = b.g8ts; pw.b = x8t; pw.ldb = up(m, 16);
+    pw.b_scale = x8t_scale; pw.m = n; pw.n = k; pw.k = m; pw.workspace = b.split;
+    if (db) { pw.colsum = reinterpret_cast<const float*>(b.colsum); pw.colsum_tiles = (int)((m + kBlock - 1) / kBlock); pw.colsum_out = db; }
   }
-  if (db) return hapx_block8_colsum_join(db, dtype, reinterpret_cast<const float*>(b.colsum), m, n, stream_);
-  return HAPX_OK;
+  if (dx && dw) return gemm8::run_two(px, pw, n_sm, stream);
+  if (dw) return gemm8::run(pw, n_sm, stream);
+  if (dx)
+    if (int e = gemm8::run(px, n_sm, stream)) return e;
+  return db ? hapx_block8_colsum_join(db, dtype, reinterpret_cast<const float*>(b.colsum), m, n, stream_) : HAPX_OK;
 }
 
 }  // extern "C"
