@@ -100,5 +100,73 @@ __device__ __forceinline__ void store4(T* p, bool vec, int valid, const float (&
   }
 }
 
+// Four consecutive elements as they are in memory, and what the quantiser asks of them.  A magnitude's pattern is its
+// float32 bits (of a bfloat16 the upper half, with anything below); patterns order like the numbers.  A NaN loses
+// against any number, an infinity wins.
+template <typename T> struct Raw4;
+template <> struct Raw4<__nv_bfloat16> {
+  uint2 w;
+  struct Max { __nv_bfloat162 a, b; };                 // of columns 0, 1 and 2, 3
+  static constexpr unsigned kMask = 0xffff0000u;       // a pattern's own bits
+  static __device__ __forceinline__ __nv_bfloat162 two(unsigned v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+  static __device__ __forceinline__ unsigned bits(__nv_bfloat162 v) { return *reinterpret_cast<const unsigned*>(&v); }
+  __device__ __forceinline__ void zero() { w = make_uint2(0u, 0u); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void load_shared(const unsigned char* tile, int row, int lane) { w = reinterpret_cast<const uint2*>(tile)[row * 32 + lane]; }
+  __device__ __forceinline__ void load_some(const __nv_bfloat16* p, int valid) {
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    w.x = (valid > 0 ? h[0] : 0u) | (valid > 1 ? (unsigned)h[1] << 16 : 0u);
+    w.y = (valid > 2 ? h[2] : 0u) | (valid > 3 ? (unsigned)h[3] << 16 : 0u);
+  }
+  __device__ __forceinline__ void get(float (&f)[4]) const {
+    f[0] = __uint_as_float(w.x << 16); f[1] = __uint_as_float(w.x & 0xffff0000u);
+    f[2] = __uint_as_float(w.y << 16); f[3] = __uint_as_float(w.y & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void clear(Max& m) { m.a = m.b = two(0u); }
+  // joins the column maxima, returns the row's pattern
+  __device__ __forceinline__ unsigned maxima(Max& m) const {
+    const __nv_bfloat162 x = __habs2(two(w.x)), y = __habs2(two(w.y));
+    m.a = __hmax2(m.a, x); m.b = __hmax2(m.b, y);
+    const __nv_bfloat162 r = __hmax2(__hmax2(x, y), two(0u));                       // of two NaN: 0
+    return bits(__hmax2(r, two(__byte_perm(bits(r), 0u, 0x1032))));
+  }
+  static __device__ __forceinline__ void columns(const Max& m, unsigned (&c)[4]) {
+    c[0] = bits(m.a) << 16; c[1] = bits(m.a); c[2] = bits(m.b) << 16; c[3] = bits(m.b);
+  }
+  // infinities become NaN
+  __device__ __forceinline__ void sanitise() {
+    if ((w.x & 0x7f80u) == 0x7f80u) w.x |= 0x7fffu;
+    if ((w.x & 0x7f800000u) == 0x7f800000u) w.x |= 0x7fff0000u;
+    if ((w.y & 0x7f80u) == 0x7f80u) w.y |= 0x7fffu;
+    if ((w.y & 0x7f800000u) == 0x7f800000u) w.y |= 0x7fff0000u;
+  }
+};
+template <> struct Raw4<float> {
+  float4 v;
+  struct Max { float c[4]; };
+  static constexpr unsigned kMask = 0xffffffffu;
+  __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void load_shared(const unsigned char* tile, int row, int lane) { v = reinterpret_cast<const float4*>(tile)[row * 32 + lane]; }
+  __device__ __forceinline__ void load_some(const float* p, int valid) {
+    zero();
+    if (valid > 0) v.x = p[0];
+    if (valid > 1) v.y = p[1];
+    if (valid > 2) v.z = p[2];
+    if (valid > 3) v.w = p[3];
+  }
+  __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+  static __device__ __forceinline__ void clear(Max& m) { m.c[0] = m.c[1] = m.c[2] = m.c[3] = 0.f; }
+  __device__ __forceinline__ unsigned maxima(Max& m) const {
+    m.c[0] = fmaxf(m.c[0], fabsf(v.x)); m.c[1] = fmaxf(m.c[1], fabsf(v.y)); m.c[2] = fmaxf(m.c[2], fabsf(v.z)); m.c[3] = fmaxf(m.c[3], fabsf(v.w));
+    return __float_as_uint(fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), 0.f));
+  }
+  static __device__ __forceinline__ void columns(const Max& m, unsigned (&c)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(m.c[j]);
+  }
+  __device__ __forceinline__ void sanitise() { v = make_float4(finite_or_nan(v.x), finite_or_nan(v.y), finite_or_nan(v.z), finite_or_nan(v.w)); }
+};
+
 }  // namespace block8
 }  // namespace hapx

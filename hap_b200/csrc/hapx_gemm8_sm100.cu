@@ -17,6 +17,10 @@
 // (768, 2304) are whole numbers of such tiles.  Single kernel (M <= 128): 128 x 64 tiles, so that a narrow product still
 // spreads over the SMs.
 //
+// Single kernel with X (a float type): the first operand comes as it is, bfloat16 or float32, and eight more warps make its
+// 8-bit tiles and scales in shared memory as the blocks go by, for themselves in every thread block: one launch for a few
+// rows (16 x 768 -> 2304: 7.2 us).
+//
 // Every mbarrier wait is bounded; on expiry a role raises the error word and leaves, the others follow as their own
 // waits run out, TMEM is freed and the kernel returns.
 #include <cuda.h>
@@ -29,6 +33,7 @@
 #include <string>
 #include <type_traits>
 
+#include "hapx_block8.h"
 #include "hapx_internal.h"
 #include "hapx_tc.h"
 
@@ -62,6 +67,8 @@ struct Params {
   int units[2];
   int rounds;                // of the second product's units that every worker takes part in: see the kernel
   unsigned* error;
+  const void* x; long long ldx;   // the first operand as it is, M x K, for the kernel that converts it
+  int K;
 };
 struct Maps { CUtensorMap a[2], b[2], sa[2], sb[2], d[2]; };
 
@@ -93,12 +100,13 @@ __device__ __forceinline__ void copy_scales(unsigned taddr, unsigned smem) {
   else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-template <bool PAIR>
+template <bool PAIR, bool CONVERT = false>
 struct Cfg {
   static constexpr int BN = PAIR ? 192 : 64;                 // columns of the tile
   static constexpr int PIECES = BN / 64;                     // 64 columns: 128 bytes of a bfloat16 row
   static constexpr int EPI_WARPS = 4 * PIECES;               // one piece of 32 rows each
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int CONVERT_WARPS = CONVERT ? 8 : 0;      // every eighth block each
+  static constexpr int THREADS = 64 + 32 * (EPI_WARPS + CONVERT_WARPS);
   static constexpr int STAGES = PAIR ? 6 : 7;
   static constexpr int B_ATOMS = PAIR ? 2 : 1;               // 192 columns from a multiple of 64 on lie in two groups of 128
   static constexpr unsigned A_BYTES = BM * BK;
@@ -153,10 +161,11 @@ __device__ __forceinline__ void add_bias(const Problem& p, int n, bool vec, floa
   }
 }
 
-template <bool PAIR>
-__global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
+template <bool PAIR, typename X>
+__global__ void __launch_bounds__(Cfg<PAIR, !std::is_void<X>::value>::THREADS, 1)
 gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params params) {
-  using C = Cfg<PAIR>;
+  constexpr bool CONVERT = !std::is_void<X>::value;
+  using C = Cfg<PAIR, CONVERT>;
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -199,7 +208,7 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
   };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), CONVERT ? 2 : 1); mbar_init(empty_bar(s), 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), (PAIR ? 2 : 1) * C::EPI_WARPS); }
     fence_barrier_init();
     const int which = own0 == 0;
@@ -231,9 +240,9 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
         if (elect_one()) {
           const unsigned sa = base + stage * C::STAGE_BYTES, sb = sa + C::A_BYTES;
           // the scales of four blocks come with the first of them that the unit needs, in the stage's own slot
-          const bool scales = kb == u.kb0 || (kb & 3) == 0;
+          const bool scales = CONVERT || kb == u.kb0 || (kb & 3) == 0;
           const unsigned ss = base + kScales + stage * C::SCALE_BYTES;
-          const unsigned bytes = C::STAGE_BYTES + (scales ? C::SCALE_BYTES : 0u);
+          const unsigned bytes = CONVERT ? C::B_BYTES + C::SCALE_BYTES - kAtom : C::STAGE_BYTES + (scales ? C::SCALE_BYTES : 0u);
           if (PAIR) {
             const unsigned bar = map_to_cta(full_bar(stage), 0);
             if (cta == 0) mbar_expect_tx(full_bar(stage), 2 * bytes);     // the bytes of both CTAs
@@ -245,10 +254,10 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
             }
           } else {
             mbar_expect_tx(full_bar(stage), bytes);
-            tma_load_4d(sa, &maps.a[u.which], kb * BK, u.m0, 0, 0, full_bar(stage));
+            if (!CONVERT) tma_load_4d(sa, &maps.a[u.which], kb * BK, u.m0, 0, 0, full_bar(stage));
             tma_load_4d(sb, &maps.b[u.which], kb * BK, u.n0, 0, 0, full_bar(stage));
             if (scales) {
-              tma_load_4d(ss, &maps.sa[u.which], 0, u.m0 >> 7, kb >> 2, 0, full_bar(stage));
+              if (!CONVERT) tma_load_4d(ss, &maps.sa[u.which], 0, u.m0 >> 7, kb >> 2, 0, full_bar(stage));
               tma_load_4d(ss + kAtom, &maps.sb[u.which], 0, u.n0 >> 7, kb >> 2, 0, full_bar(stage));
             }
           }
@@ -276,7 +285,7 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
           ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase));
           if (!ok) break;
           tc_fence_after();
-          const bool scales = kb == u.kb0 || (kb & 3) == 0;
+          const bool scales = CONVERT || kb == u.kb0 || (kb & 3) == 0;
           if (scales) sf = tmem_base + C::SF_COL + stage * C::SF_SET;
           if (elect_one()) {
             if (scales) {
@@ -304,6 +313,83 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
       if (!ok && lane == 0) atomicCAS(params.error, 0u, 2u);
+    }
+  } else if (CONVERT && warp >= 2 + C::EPI_WARPS) {
+    // ---------------- 8-bit tiles of the first operand: a warp per block, R rows at a time ----------------
+    // (A block's rows over all warps would put the loads' latency and the fence into every block: 2 us each.)
+    if constexpr (CONVERT) {
+      const int mine = warp - 2 - C::EPI_WARPS, M = params.pr[0].M, K = params.K;     // the rows are those of one tile: M <= 128
+      const X* x = static_cast<const X*>(params.x) + 4 * lane;
+      const bool vec = (params.ldx & 3) == 0 && (reinterpret_cast<uintptr_t>(params.x) & (4 * sizeof(X) - 1)) == 0;
+      constexpr int R = 8;                                   // 16 for bfloat16 was no faster
+      block8::Raw4<X> next[R];
+      auto fetch = [&](int kb, int r0) {
+        const int valid = max(0, min(4, K - kb * BK - 4 * lane));
+        const X* src = x + (long long)kb * BK + r0 * params.ldx;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (r0 + i >= M || valid == 0) next[i].zero();
+          else if (vec && valid == 4) next[i].load(src + i * params.ldx);
+          else next[i].load_some(src + i * params.ldx, valid);
+        }
+      };
+      int stage = 0, turn = 0;
+      unsigned phase = 0;
+      bool ok = true;
+      Unit u;
+      for (int step = 0; ok && next_unit(step, u); ++step) {
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
+          if (turn == mine) {
+            fetch(kb, 0);
+            ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u));
+            if (!ok) break;
+            unsigned char* tile = gen_base + stage * C::STAGE_BYTES;
+            unsigned char* scales = gen_base + kScales + stage * C::SCALE_BYTES + (kb & 3);
+            for (int r0 = 0; r0 < M; r0 += R) {
+              block8::Raw4<X> v[R];
+#pragma unroll
+              for (int i = 0; i < R; ++i) v[i] = next[i];
+              if (r0 + R < M) fetch(kb, r0 + R);
+              unsigned big = 0u;                               // lane i < R: the pattern of row i's maximum
+              auto maxima = [&] {
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                  typename block8::Raw4<X>::Max unused;
+                  block8::Raw4<X>::clear(unused);
+                  const unsigned r = __reduce_max_sync(0xffffffffu, v[i].maxima(unused));
+                  if (lane == i) big = r;
+                }
+              };
+              maxima();
+              if (__any_sync(0xffffffffu, big >= 0x7f800000u)) {   // an infinity (rare): NaN in its place
+#pragma unroll
+                for (int i = 0; i < R; ++i) v[i].sanitise();
+                maxima();
+              }
+              const int e = block8::scale_exponent(__uint_as_float(big & block8::Raw4<X>::kMask));
+              const float inv_mine = block8::pow2(-e);
+#pragma unroll
+              for (int i = 0; i < R; ++i) {                    // a row's 16-byte chunks are swizzled by its number mod 8
+                const float inv = __shfl_sync(0xffffffffu, inv_mine, i);
+                float f[4];
+                v[i].get(f);
+                *reinterpret_cast<unsigned*>(tile + (r0 + i) * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4) =
+                    block8::pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+              }
+              if (lane < R) {
+                const int r = r0 + lane;
+                scales[(r & 31) * 16 + (r >> 5) * 4] = (unsigned char)(e + 127);
+              }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full_bar(stage));
+          }
+          if (++turn == C::CONVERT_WARPS) turn = 0;
+          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok && lane == 0) atomicCAS(params.error, 0u, 4u);
     }
   } else {
     // ---------------- epilogue: 32 rows x 64 columns of the tile per warp ----------------
@@ -572,10 +658,10 @@ static PairPlan plan_two(const Product& x, const Product& y, int sm_count) {
 
 static long long partial_bytes(const Plan& pl) { return pl.splits > 1 ? pl.splits * pl.m_pad * pl.n_pad * 4 : 0; }
 
-template <bool PAIR>
+template <bool PAIR, typename X>
 static int launch(const Maps& maps, const Params& p, int sm_count, cudaStream_t stream) {
-  using C = Cfg<PAIR>;
-  auto kernel = gemm8_kernel<PAIR>;
+  using C = Cfg<PAIR, !std::is_void<X>::value>;
+  auto kernel = gemm8_kernel<PAIR, X>;
   static int limit_of[64] = {};             // per device: function attributes and occupancy belong to one
   static std::mutex mutex;
   int device = 0;
@@ -647,11 +733,13 @@ static int describe(const Product& pr, const Plan& pl, void* partial, int i, Map
   p.bias_vec = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
   p.colsum = pr.colsum; p.colsum_tiles = pr.colsum_tiles; p.colsum_f32 = pr.out_f32; p.colsum_out = pr.colsum_out;
   const int es = p.out_f32 ? 4 : 2;
-  if (int e = make_map(&maps->a[i], pr.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, pr.lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B,
+  if (pr.a)
+    if (int e = make_map(&maps->a[i], pr.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, pr.lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
   if (int e = make_map(&maps->b[i], pr.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, pr.ldb, BK, pl.pair ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
-  if (int e = make_scale_map(&maps->sa[i], pr.a_scale, M, p.k_blocks, 1)) return e;
+  if (pr.a)
+    if (int e = make_scale_map(&maps->sa[i], pr.a_scale, M, p.k_blocks, 1)) return e;
   if (int e = make_scale_map(&maps->sb[i], pr.b_scale, N, p.k_blocks, pl.pair ? Cfg<true>::B_ATOMS : Cfg<false>::B_ATOMS)) return e;
   p.tma_store = (reinterpret_cast<uintptr_t>(p.D) & 15u) == 0 && (p.ldd * es) % 16 == 0;
   if (p.tma_store)
@@ -680,7 +768,24 @@ int run(const Product& pr, int sm_count, cudaStream_t stream) {
   if (int e = gemm::error_word(&params.error, nullptr)) return e;
   const Plan pl = plan_of(pr.m, pr.n, pr.k, sm_count);
   if (int e = describe(pr, pl, pr.workspace, 0, &maps, &params)) return e;
-  if (int e = pl.pair ? launch<true>(maps, params, sm_count, stream) : launch<false>(maps, params, sm_count, stream)) return e;
+  if (int e = pl.pair ? launch<true, void>(maps, params, sm_count, stream) : launch<false, void>(maps, params, sm_count, stream)) return e;
+  return join(pr, pl, pr.workspace, sm_count, stream);
+}
+
+// 64 x 1024 -> 4096 takes 16.4 us this way and 9.0 with the quantiser in front, 16 tokens 8.0 and about 9: the limit lies
+// where the launch that is saved (5 us of host time) no longer pays.
+bool converts(long long m) { return m <= 32; }
+
+int run_converting(const Product& pr, const void* x, int dtype, long long ldx, int sm_count, cudaStream_t stream) {
+  Params params = Params();
+  Maps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  if (int e = gemm::error_word(&params.error, nullptr)) return e;
+  const Plan pl = plan_of(pr.m, pr.n, pr.k, sm_count);
+  if (int e = describe(pr, pl, pr.workspace, 0, &maps, &params)) return e;
+  params.x = x; params.ldx = ldx; params.K = (int)pr.k;
+  if (int e = dtype == HAPX_BF16 ? launch<false, __nv_bfloat16>(maps, params, sm_count, stream) : launch<false, float>(maps, params, sm_count, stream))
+    return e;
   return join(pr, pl, pr.workspace, sm_count, stream);
 }
 
@@ -700,7 +805,7 @@ int run_two(const Product& x, const Product& y, int sm_count, cudaStream_t strea
   for (int i = 0; i < 2; ++i)
     if (int e = describe(*pr[i], t.pl[i], partial[i], i == t.first ? 0 : 1, &maps, &params)) return e;
   params.rounds = t.rounds;
-  if (int e = launch<true>(maps, params, sm_count, stream)) return e;
+  if (int e = launch<true, void>(maps, params, sm_count, stream)) return e;
   for (int i = 0; i < 2; ++i)
     if (int e = join(*pr[i], t.pl[i], partial[i], sm_count, stream)) return e;
   return HAPX_OK;

@@ -93,6 +93,10 @@ struct Product {
 };
 long long workspace_bytes(long long m, long long n, long long k, int sm_count);
 int run(const Product& p, int sm_count, cudaStream_t stream);
+// The same with the first operand as it is: x (m x k of `dtype`, ldx elements from row to row) instead of p.a, for as many
+// rows as `converts` allows; the launch makes its 8-bit form.
+bool converts(long long m);
+int run_converting(const Product& p, const void* x, int dtype, long long ldx, int sm_count, cudaStream_t stream);
 // Two independent products in one launch (x.workspace serves both).
 long long workspace_bytes_two(const Product& x, const Product& y, int sm_count);
 int run_two(const Product& x, const Product& y, int sm_count, cudaStream_t stream);

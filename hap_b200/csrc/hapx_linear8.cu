@@ -4,8 +4,8 @@
 // transposed, for the input gradient), both in one launch, then the product.  Backward: g likewise in both forms from one
 // read, with the partial sums of the bias gradient, then the two products in one launch, which joins those sums.
 //
-// A few tokens through a weight that is already in 8 bits (thin_kernel) need no tensor cores: the time is that of one
-// launch and of reading the weight.  Every thread block makes the 8-bit form of x for itself in shared memory, a warp
+// Up to 32 tokens through a weight that is already in 8 bits take one launch: the product's, which converts x by itself.
+// A few tokens (thin_kernel) need no tensor cores: the time is that of the launch and of reading the weight.  Every thread block makes the 8-bit form of x for itself in shared memory, a warp
 // multiplies a row of w with all tokens from registers; the values multiplied are those of the other path.
 #include <algorithm>
 #include <mutex>
@@ -19,11 +19,11 @@ namespace linear8 {
 
 using namespace block8;
 
-constexpr int kThinTokens = 8;              // above, the tensor-core path is no slower (measured: see launch_thin)
+constexpr int kThinTokens = 2;              // 4 x 768 -> 33280 takes 24 us here and 13 on the tensor cores, 1 x 768 -> 2304 3.5 and 6.4
 constexpr int kThinElements = 24 * 1024;    // tokens x in_features that fit shared memory as float32 (96 KiB)
 
 // MT: tokens, rounded up to a power of two.
-template <typename T, int MT>
+template <typename T, int MT, int ROWS>
 __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long long ldx, const unsigned char* __restrict__ w, long long ldw,
                                                    const unsigned char* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y, int M,
                                                    int N, int K) {
@@ -48,43 +48,60 @@ __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long
     if (lane == 0) s_s[m * blocks + kb] = pow2(e);
   }
   __syncthreads();
+  // ROWS rows of w at a time: their loads in flight together, x read from shared memory once for all of them
   const long long groups = ((long long)N + kBlock - 1) / kBlock;
-  for (int n = blockIdx.x * 8 + warp; n < N; n += gridDim.x * 8) {
-    float acc[MT];
+  for (int n0 = (blockIdx.x * 8 + warp) * ROWS; n0 < N; n0 += gridDim.x * 8 * ROWS) {
+    float acc[ROWS][MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = 0.f;
-    for (int k = 16 * lane; k < K; k += 512) {           // 16 values of one block of 128; what lies behind K is zero in s_x
-      const uint4 raw = *reinterpret_cast<const uint4*>(w + (long long)n * ldw + k);
-      const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[r][m] = 0.f;
+    for (int k = 16 * lane; k < K; k += 512) {           // 16 values of one block of 128
+      uint4 raw[ROWS];
+      int e[ROWS];
       const int kb = k / kBlock;
-      const float sw = pow2((int)ws[scale_at(n, kb, groups)] - 127);
-      float part[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) part[m] = 0.f;
+      for (int r = 0; r < ROWS; ++r) {
+        const int n = min(n0 + r, N - 1);
+        raw[r] = __ldg(reinterpret_cast<const uint4*>(w + (long long)n * ldw + k));
+        e[r] = ws[scale_at(n, kb, groups)];
+      }
+      float part[ROWS][MT];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) part[r][m] = 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float2 a = unpack2(words[c] & 0xffffu), b = unpack2(words[c] >> 16);
         const int left = K - (k + 4 * c);                // bytes behind the row's end are padding
-        const float v[4] = {left > 0 ? a.x : 0.f, left > 1 ? a.y : 0.f, left > 2 ? b.x : 0.f, left > 3 ? b.y : 0.f};
+        float4 xv[MT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if (m < M) {
-            const float4 xv = *reinterpret_cast<const float4*>(s_x + (long long)m * kpad + k + 4 * c);
-            part[m] = fmaf(v[0], xv.x, fmaf(v[1], xv.y, fmaf(v[2], xv.z, fmaf(v[3], xv.w, part[m]))));
-          }
+        for (int m = 0; m < MT; ++m) xv[m] = *reinterpret_cast<const float4*>(s_x + (long long)min(m, M - 1) * kpad + k + 4 * c);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const unsigned word = c == 0 ? raw[r].x : c == 1 ? raw[r].y : c == 2 ? raw[r].z : raw[r].w;
+          const float2 a = unpack2(word & 0xffffu), b = unpack2(word >> 16);
+          const float v[4] = {left > 0 ? a.x : 0.f, left > 1 ? a.y : 0.f, left > 2 ? b.x : 0.f, left > 3 ? b.y : 0.f};
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            part[r][m] = fmaf(v[0], xv[m].x, fmaf(v[1], xv[m].y, fmaf(v[2], xv[m].z, fmaf(v[3], xv[m].w, part[r][m]))));
         }
       }
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        if (m < M) acc[m] = fmaf(part[m] * sw, s_s[m * blocks + kb], acc[m]);
+      for (int m = 0; m < MT; ++m) {
+        const float sx = s_s[min(m, M - 1) * blocks + kb];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) acc[r][m] = fmaf(part[r][m] * pow2(e[r] - 127), sx, acc[r][m]);
+      }
     }
-    const float bn = bias ? to_f(bias[n]) : 0.f;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m < M) {
+    for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
-        if (lane == m) y[(long long)m * N + n] = from_f<T>(bias ? acc[m] + bn : acc[m]);
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[r][m] += __shfl_xor_sync(0xffffffffu, acc[r][m], o);
+        if (lane == r * MT + m && m < M && n0 + r < N)
+          y[(long long)m * N + n0 + r] = from_f<T>(bias ? acc[r][m] + to_f(bias[n0 + r]) : acc[r][m]);
       }
     }
   }
@@ -94,7 +111,8 @@ template <typename T, int MT>
 static int launch_thin(const void* x, long long ldx, const void* w, long long ldw, const void* ws, const void* bias, void* y, int M, int N, int K,
                        int n_sm, cudaStream_t stream) {
   const int kpad = (K + kBlock - 1) / kBlock * kBlock, smem = M * kpad * 4 + M * (kpad / kBlock) * 4;
-  auto kernel = thin_kernel<T, MT>;
+  constexpr int ROWS = 4;
+  auto kernel = thin_kernel<T, MT, ROWS>;
   {  // function attributes are per device
     static bool set[64] = {};
     static std::mutex mutex;
@@ -107,7 +125,7 @@ static int launch_thin(const void* x, long long ldx, const void* w, long long ld
       set[device] = true;
     }
   }
-  const int grid = std::min((N + 7) / 8, n_sm * 2);
+  const int grid = std::min((N + 8 * ROWS - 1) / (8 * ROWS), n_sm * (smem <= 48 * 1024 ? 4 : 2));
   kernel<<<grid, 256, smem, stream>>>(static_cast<const T*>(x), ldx, static_cast<const unsigned char*>(w), ldw, static_cast<const unsigned char*>(ws),
                                       static_cast<const T*>(bias), static_cast<T*>(y), M, N, K);
   HAPX_CUDA(cudaGetLastError());
@@ -132,12 +150,20 @@ struct Carve {
 };
 
 struct Forward { unsigned char *x8, *x8s, *w8, *w8s, *split; long long bytes; };
-static Forward layout_forward(void* base, long long m, long long n, long long k, bool prepared, bool thin_path, int n_sm) {
+// How x reaches the product: kThin, kConvert (both for a weight in 8 bits, when x's form is not kept), kQuantise.
+enum Path { kThin, kConvert, kQuantise };
+static Path path_of(long long m, long long k, bool prepared, bool keep_x) {
+  if (!prepared || keep_x) return kQuantise;
+  return thin(m, k) ? kThin : gemm8::converts(m) ? kConvert : kQuantise;
+}
+static Forward layout_forward(void* base, long long m, long long n, long long k, bool prepared, Path path, int n_sm) {
   Carve c(base);
   Forward f = {};
-  if (!thin_path) {
-    f.x8 = c.take(m * up(k, 16));
-    f.x8s = c.take(scale_bytes(m, k));
+  if (path != kThin) {
+    if (path == kQuantise) {
+      f.x8 = c.take(m * up(k, 16));
+      f.x8s = c.take(scale_bytes(m, k));
+    }
     if (!prepared) { f.w8 = c.take(n * up(k, 16)); f.w8s = c.take(scale_bytes(n, k)); }
     f.split = c.take(gemm8::workspace_bytes(m, n, k, n_sm));
   }
@@ -187,7 +213,7 @@ extern "C" {
 int64_t hapx_linear8_forward_workspace(int64_t m, int64_t n, int64_t k, int prepared, int keep_x) {
   int n_sm = 0;
   if (m < 1 || n < 1 || k < 1 || sm_count(&n_sm)) return 0;
-  return layout_forward(nullptr, m, n, k, prepared != 0, prepared && !keep_x && thin(m, k), n_sm).bytes;
+  return layout_forward(nullptr, m, n, k, prepared != 0, path_of(m, k, prepared != 0, keep_x != 0), n_sm).bytes;
 }
 
 int hapx_linear8_forward(void* y, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* w8, const void* w8_scale, const void* bias,
@@ -204,25 +230,26 @@ int hapx_linear8_forward(void* y, const void* x, int64_t ldx, const void* w, int
   int n_sm = 0;
   if (int e = sm_count(&n_sm)) return e;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const bool thin_path = prepared && !x8t && thin(m, k);
-  const Forward f = layout_forward(workspace, m, n, k, prepared, thin_path, n_sm);
+  const Path path = path_of(m, k, prepared, x8t != nullptr);
+  const Forward f = layout_forward(workspace, m, n, k, prepared, path, n_sm);
   if (workspace_bytes < f.bytes || (f.bytes > 0 && (!workspace || !aligned(workspace))))
     return fail(HAPX_ERR_ARGUMENT, "linear8_forward: the workspace must be 16-byte aligned and as large as hapx_linear8_forward_workspace says");
-  if (thin_path) {
+  if (path == kThin) {
     const int M = (int)m, N = (int)n, K = (int)k;
 #define HAPX_THIN(T, MT) return launch_thin<T, MT>(x, ldx, w8, up(k, 16), w8_scale, bias, y, M, N, K, n_sm, stream)
     if (dtype == HAPX_BF16) {
       if (m == 1) HAPX_THIN(__nv_bfloat16, 1);
-      if (m == 2) HAPX_THIN(__nv_bfloat16, 2);
-      if (m <= 4) HAPX_THIN(__nv_bfloat16, 4);
-      HAPX_THIN(__nv_bfloat16, 8);
+      HAPX_THIN(__nv_bfloat16, 2);
     }
     if (m == 1) HAPX_THIN(float, 1);
-    if (m == 2) HAPX_THIN(float, 2);
-    if (m <= 4) HAPX_THIN(float, 4);
-    HAPX_THIN(float, 8);
+    HAPX_THIN(float, 2);
 #undef HAPX_THIN
   }
+  gemm8::Product p;
+  p.d = y; p.out_f32 = dtype == HAPX_F32; p.lda = up(k, 16);
+  p.b = prepared ? w8 : f.w8; p.ldb = up(k, 16); p.b_scale = prepared ? w8_scale : f.w8s;
+  p.bias = bias; p.m = m; p.n = n; p.k = k; p.workspace = f.split;
+  if (path == kConvert) return gemm8::run_converting(p, x, dtype, ldx, n_sm, stream);
   QuantJob jobs[2];
   int n_jobs = 0;
   if (m > 0) {
@@ -237,10 +264,7 @@ int hapx_linear8_forward(void* y, const void* x, int64_t ldx, const void* w, int
   }
   if (int e = quantize(jobs, n_jobs, dtype, stream)) return e;
   if (m == 0) return HAPX_OK;
-  gemm8::Product p;
-  p.d = y; p.out_f32 = dtype == HAPX_F32; p.a = f.x8; p.lda = up(k, 16); p.a_scale = f.x8s;
-  p.b = prepared ? w8 : f.w8; p.ldb = up(k, 16); p.b_scale = prepared ? w8_scale : f.w8s;
-  p.bias = bias; p.m = m; p.n = n; p.k = k; p.workspace = f.split;
+  p.a = f.x8; p.a_scale = f.x8s;
   return gemm8::run(p, n_sm, stream);
 }
 

@@ -233,6 +233,29 @@ def test_linear8_prepared_weight():
     check_linear((y, xg.grad, None, bg.grad), want, 77, 300, 130)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,fin,fout", [(1, 768, 2304), (1, 1, 1), (2, 130, 77), (3, 5000, 64), (8, 1000, 129), (8, 4096, 40), (9, 768, 768), (33, 129, 300),
+                                           (64, 1024, 512), (65, 100, 200), (100, 640, 33), (128, 513, 264), (129, 256, 192), (40, 8192, 64)])
+def test_linear8_few_tokens_prepared_weight(dtype, rows, fin, fout):
+    """Every way the tokens reach the product (a warp per output, converted inside the product, quantised before it) gives
+    the result of the plain call; rows with infinities and NaN, strided rows."""
+    import hap_b200
+    from hap_b200 import block8
+    x, w, b, g = linear_inputs(rows, fin, fout, dtype)
+    want = B.linear8(x, w, b, g)[:1]
+    w8 = block8.quantize_weight(w.to(DEV))
+    y = hap_b200.linear8(x.to(DEV), w8, b.to(DEV))
+    check_linear((y,), want, rows, fin, fout)
+    wide = torch.zeros(rows, 2 * fin + 3, dtype=dtype, device=DEV)
+    wide[:, 1:1 + fin] = x.to(DEV)
+    assert torch.equal(hap_b200.linear8(wide[:, 1:1 + fin], w8, b.to(DEV)), y)
+    x[rows // 2, fin // 2] = float("inf")
+    x[0, 0] = float("nan")
+    y = hap_b200.linear8(x.to(DEV), w8).cpu()
+    bad = torch.isnan(x).any(1) | torch.isinf(x).any(1)
+    assert bool(torch.isnan(y[bad]).all()) and bool(torch.isfinite(y[~bad]).all())
+
+
 def test_linear8_refusals():
     import hap_b200
     from hap_b200 import block8
