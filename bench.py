@@ -946,7 +946,7 @@ def run_lm_cpu(world, batch_per_rank, layers):
             "step_s": r["s"]}
 
 
-def lm_step(args, job, kind, plan, use_graph, dropout_p):
+def lm_step(args, job, kind, plan, use_graph, dropout_p, block8=False):
     """Time the training step of one program (``kind``: lm / vit / moe) at job.n_gpus GPUs: device time per
     step (CUDA events, max over ranks) and the end-to-end time with the inputs coming from pinned host memory
     every step and the loss read back on the host."""
@@ -1004,6 +1004,8 @@ def lm_step(args, job, kind, plan, use_graph, dropout_p):
             hap_b200.fxpass.sparsify_moe(graph)         # dispatch / combine as row gathers instead of dense one-hot contractions
         if W > 1 and not args.lm_no_prefetch:
             hap_b200.fxpass.prefetch_parameter_gathers(graph)   # parameter gathers early, on the side stream
+        if block8:
+            hap_b200.fxpass.use_block8(graph)           # products in 8-bit blocks, inputs kept for the backward pass in 8 bits
         return torch.fx.GraphModule(model, graph)
 
     if W == 1:
@@ -1104,8 +1106,8 @@ def lm_step(args, job, kind, plan, use_graph, dropout_p):
     result = {
         "metric": "spmd_step_samples_per_s", "value": B / (ms * 1e-3), "unit": "samples/s", "n_gpus": n_gpus, "steps": args.steps,
         "warmup": max(args.warmup, 3), "ms_per_step": ms, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-        "dtype": "bf16", "data": "synthetic",
-        "config": {"workload": f"{desc}, global batch {B} split {lb}", "parameters": n_params, "plan": plan, "batch_split": lb,
+        "dtype": "e4m3 blocks (linear products), bf16" if block8 else "bf16", "data": "synthetic",
+        "config": {"workload": f"{desc}{', 8-bit blocks' if block8 else ''}, global batch {B} split {lb}", "parameters": n_params, "plan": plan, "batch_split": lb,
                    "executor": "CUDA graph of the whole iteration" if use_graph else "eager fx GraphModule",
                    "l2": "activations and weights of a step exceed L2 by far", "loss": losses[-1]},
         "roofline": {"bound": "tensor", "kernel": "gemm2_bf16_kernel (all linear / attention contractions of the busiest rank)",
@@ -1137,7 +1139,7 @@ def run_lm_step(args, job):
 
 def run_lm(args):
     job = Job(args.gpus)
-    result = lm_step(args, job, args.lm_model, args.lm_plan, args.lm_graph, args.lm_dropout)
+    result = lm_step(args, job, args.lm_model, args.lm_plan, args.lm_graph, args.lm_dropout, args.lm_block8)
     if job.rank == 0 and job.n_gpus == 1 and not args.no_cpu_baseline and args.lm_model == "lm":
         result["cpu_baseline"] = run_lm_cpu(2, 2, 2)
     job.finish()
@@ -1413,6 +1415,7 @@ def main():
     ap.add_argument("--lm-plan", default="dp_zero", choices=["dp", "dp_zero", "tp"])
     ap.add_argument("--lm-no-prefetch", action="store_true", help="gather sharded parameters where they are used, on the main stream")
     ap.add_argument("--lm-no-fuse", action="store_true", help="run the program as emitted, without the elementwise fusion pass")
+    ap.add_argument("--lm-block8", action="store_true", help="lm workload: the program on the 8-bit operators (fxpass.use_block8)")
     ap.add_argument("--lm-graph", action="store_true", help="capture the training step into a CUDA graph")
     ap.add_argument("--gemm-tokens", type=int, default=8192)
     ap.add_argument("--gemm-layers", default="", help="comma-separated layer names to restrict the gemm workload to")
