@@ -280,9 +280,10 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // ---- layer_norm ---------------------------------------------------------------------------------------
-// A row belongs to a team of W warps; warp w of it holds the blocks of 128 columns w, w + W, ... (NB of them at most) in
-// registers, lane l the columns 4l .. 4l + 3 of each.  A thread block has 8 / W teams.  Rows of up to 8192 columns are read
-// once; longer ones take the kernels below these.
+// A row belongs to a team of W warps; warp w of it holds the groups of 256 columns w, w + W, ... (NG of them at most) in
+// registers, lane l the columns 8l .. 8l + 7 of each, so that sixteen lanes hold a block of 128.  A thread block has 8 / W
+// teams, and a team fetches its next row before it works on the present one.  Rows of up to 8192 columns are read once;
+// longer ones take the kernels below these.  VEC: rows and parameters lie on 16 bytes and E is a multiple of 8.
 constexpr int kTeamColumns = 8192;
 
 // Sum over a team (`s`: one float per warp of the block, reused after the next call's other buffer).
@@ -300,130 +301,191 @@ __device__ __forceinline__ float team_sum(float v, float* s, int warp) {
   return v;
 }
 
-template <typename T, int W, int NB>
-__global__ void __launch_bounds__(256, NB <= 4 ? 4 : NB <= 6 ? 3 : 2) norm_forward_team_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b,
-                                                                                 T* __restrict__ y, float* __restrict__ mean_out,
-                                                                                 float* __restrict__ rstd_out, unsigned char* __restrict__ q,
-                                                                                 long long ldq, float* __restrict__ s, long long rows, int E, float eps) {
+// Columns of a thread's eight that lie inside the row.
+template <bool VEC>
+__device__ __forceinline__ int valid_of(int E, int c) { return VEC ? (c < E ? 8 : 0) : max(0, min(8, E - c)); }
+
+template <typename T, int W, int NG, bool VEC>
+__global__ void __launch_bounds__(256, 2) norm_forward_team_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b,
+                                                                   T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                                   unsigned char* __restrict__ q, long long ldq, float* __restrict__ s, long long rows,
+                                                                   int E, float eps) {
   __shared__ float s_sum[2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W, blocks = (E + kBlock - 1) / kBlock;
-  const bool vec = (E & 3) == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(w) |
-                                     reinterpret_cast<uintptr_t>(b)) & (4 * sizeof(T) - 1)) == 0;
+  Raw8<T> next[NG];
   const float inv_e = 1.f / (float)E;
-  for (long long row = (long long)blockIdx.x * (8 / W) + warp / W; row < rows; row += (long long)gridDim.x * (8 / W)) {
-    const T* xr = x + row * E;
-    float v[NB][4], sum = 0.f;
+  const long long stride = (long long)gridDim.x * (8 / W);
+  auto fetch = [&](long long row) {
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int c = (part + k * W) * kBlock + 4 * lane;
-      load4(xr + c, vec, max(0, min(4, E - c)), v[k]);
+    for (int k = 0; k < NG; ++k) {
+      const int c = (part + k * W) * 256 + 8 * lane;
+      next[k].load(x + row * E + c, VEC, valid_of<VEC>(E, c));
     }
+  };
+  long long row = (long long)blockIdx.x * (8 / W) + warp / W;
+  if (row < rows) fetch(row);
+  for (; row < rows; row += stride) {
+    float v[NG][8], sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) sum += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
+    for (int k = 0; k < NG; ++k) {
+      next[k].get(v[k]);
+      sum += ((v[k][0] + v[k][1]) + (v[k][2] + v[k][3])) + ((v[k][4] + v[k][5]) + (v[k][6] + v[k][7]));
+    }
+    if (row + stride < rows) fetch(row + stride);
     const float mean = team_sum<W>(sum, s_sum[0], warp) * inv_e;
     float sq = 0.f;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int valid = E - ((part + k * W) * kBlock + 4 * lane);
+    for (int k = 0; k < NG; ++k) {
+      const int valid = valid_of<VEC>(E, (part + k * W) * 256 + 8 * lane);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const float d = j < valid ? v[k][j] - mean : 0.f;
         sq = fmaf(d, d, sq);
       }
     }
     const float rstd = rsqrtf(team_sum<W>(sq, s_sum[1], warp) * inv_e + eps);
-    float my_scale = 0.f;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
-      float g[4] = {1.f, 1.f, 1.f, 1.f}, h[4] = {0.f, 0.f, 0.f, 0.f}, o[4], big = 0.f;
-      if (w) load4(w + c, vec, valid, g);
-      if (b) load4(b + c, vec, valid, h);
+    for (int k = 0; k < NG; ++k) {
+      const int c = (part + k * W) * 256 + 8 * lane, valid = valid_of<VEC>(E, c);
+      float o[8], f[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o[j] = fmaf((v[k][j] - mean) * rstd, g[j], h[j]);
-        v[k][j] = finite_or_nan(v[k][j]);
-        big = fmaxf(big, fabsf(v[k][j]));
+      for (int j = 0; j < 8; ++j) o[j] = (v[k][j] - mean) * rstd;
+      if (w) {
+        Raw8<T> p;
+        p.load(w + c, VEC, valid);                 // from the first-level cache, row after row
+        p.get(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] *= f[j];
       }
-      store4(y + row * E + c, vec, valid, o);
-      if (q) {                                    // a gradient is asked for
-        const int e = scale_exponent(warp_max(big));
+      if (b) {
+        Raw8<T> p;
+        p.load(b + c, VEC, valid);
+        p.get(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] += f[j];
+      }
+      store8(y + row * E + c, VEC, valid, o);
+      if (q) {                                     // a gradient is asked for
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(v[k][j]));            // a NaN loses
+        if (__any_sync(0xffffffffu, big == __uint_as_float(0x7f800000u))) {      // rare: infinities become NaN
+          big = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { v[k][j] = finite_or_nan(v[k][j]); big = fmaxf(big, fabsf(v[k][j])); }
+        }
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+        const int e = scale_exponent(big);
         const float inv = pow2(-e);
-        if (lane == k) my_scale = pow2(e);
-        if (valid > 0) *reinterpret_cast<unsigned*>(q + row * ldq + c) = pack4(v[k][0] * inv, v[k][1] * inv, v[k][2] * inv, v[k][3] * inv);
+        if (valid > 0) {
+          if ((lane & 15) == 0) s[row * blocks + c / kBlock] = pow2(e);
+          *reinterpret_cast<uint2*>(q + row * ldq + c) = make_uint2(pack4(v[k][0] * inv, v[k][1] * inv, v[k][2] * inv, v[k][3] * inv),
+                                                                    pack4(v[k][4] * inv, v[k][5] * inv, v[k][6] * inv, v[k][7] * inv));
+        }
       }
     }
-    if (q) {
-      if (lane < NB && part + lane * W < blocks) s[row * blocks + part + lane * W] = my_scale;
-      if (part == 0 && lane == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
-    }
+    if (q && part == 0 && lane == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
   }
 }
 
 // dx of the rows, and partial[block][0][c] = sum dy z, partial[block][1][c] = sum dy over the rows the thread block took.  The
-// running sums of a warp's columns lie in shared memory, owned by the warp (registers would leave a third of the warps).
-template <typename T, int W, int NB>
+// running sums of a warp's columns lie in shared memory, owned by the warp: in registers, next to the prefetched row, they
+// would leave half of the warps.
+template <typename T, int W, int NG, bool VEC>
 __global__ void __launch_bounds__(256, 2) norm_backward_team_kernel(const unsigned char* __restrict__ q, long long ldq, const float* __restrict__ s,
                                                                     const T* __restrict__ dy, const T* __restrict__ w,
                                                                     const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                                                                     const T* __restrict__ add, T* __restrict__ dx, float* __restrict__ partial,
                                                                     long long rows, int E) {
-  extern __shared__ float4 s_acc[];               // [warp][NB][2][32 lanes]
+  extern __shared__ float4 s_acc[];               // [warp][NG][dw: first and second four columns, db: the same][32 lanes]
   __shared__ float s_sum[2][2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W, blocks = (E + kBlock - 1) / kBlock;
-  const bool vec = (E & 3) == 0 && ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(w) |
-                                     reinterpret_cast<uintptr_t>(add)) & (4 * sizeof(T) - 1)) == 0;
-  float4* acc = s_acc + (long long)warp * NB * 64 + lane;
+  constexpr bool KEEP = sizeof(T) == 2;            // the residual gradient of the next row is fetched ahead too
+  float4* acc = s_acc + (long long)warp * NG * 128 + lane;
   if (partial) {
 #pragma unroll
-    for (int k = 0; k < 2 * NB; ++k) acc[32 * k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < 4 * NG; ++k) acc[32 * k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const float inv_e = 1.f / (float)E;
-  int flip = 0;
-  for (long long row = (long long)blockIdx.x * (8 / W) + warp / W; row < rows; row += (long long)gridDim.x * (8 / W), flip ^= 1) {
-    const float mean = mean_in[row], rstd = rstd_in[row];
-    const float my_scale = lane < NB && part + lane * W < blocks ? s[row * blocks + part + lane * W] : 0.f;
-    float g[NB][4], z[NB][4], s1 = 0.f, s2 = 0.f;
-    unsigned raw[NB];
+  Raw8<T> next_g[NG], next_r[KEEP ? NG : 1];
+  uint2 next_q[NG];
+  float next_s[NG], next_mean = 0.f, next_rstd = 0.f;
+  auto fetch = [&](long long row) {
+    next_mean = mean_in[row];
+    next_rstd = rstd_in[row];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
-      load4(dy + row * E + c, vec, valid, g[k]);
-      raw[k] = valid > 0 ? *reinterpret_cast<const unsigned*>(q + row * ldq + c) : 0u;
+    for (int k = 0; k < NG; ++k) {
+      const int c = (part + k * W) * 256 + 8 * lane, valid = valid_of<VEC>(E, c);
+      next_g[k].load(dy + row * E + c, VEC, valid);
+      if (KEEP && add) next_r[k].load(add + row * E + c, VEC, valid);
+      next_q[k] = valid > 0 ? *reinterpret_cast<const uint2*>(q + row * ldq + c) : make_uint2(0u, 0u);
+      next_s[k] = valid > 0 ? s[row * blocks + c / kBlock] : 0.f;
     }
+  };
+  const float inv_e = 1.f / (float)E;
+  const long long stride = (long long)gridDim.x * (8 / W);
+  int flip = 0;
+  long long row = (long long)blockIdx.x * (8 / W) + warp / W;
+  if (row < rows) fetch(row);
+  for (; row < rows; row += stride, flip ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
+    Raw8<T> res[KEEP ? NG : 1];
+    float g[NG][8], z[NG][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
-      const float sc = __shfl_sync(0xffffffffu, my_scale, k);
-      const float2 lo = unpack2(raw[k] & 0xffffu), hi = unpack2(raw[k] >> 16);
-      const float h[4] = {lo.x, lo.y, hi.x, hi.y};
+    for (int k = 0; k < NG; ++k) {
+      const int valid = valid_of<VEC>(E, (part + k * W) * 256 + 8 * lane);
+      next_g[k].get(g[k]);
+      const unsigned half[4] = {next_q[k].x & 0xffffu, next_q[k].x >> 16, next_q[k].y & 0xffffu, next_q[k].y >> 16};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z[k][j] = j < valid ? (h[j] * sc - mean) * rstd : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const float2 two = unpack2(half[i]);
+        z[k][2 * i] = 2 * i < valid ? fmaf(two.x, next_s[k], -mean) * rstd : 0.f;       // two.x times its scale is exact
+        z[k][2 * i + 1] = 2 * i + 1 < valid ? fmaf(two.y, next_s[k], -mean) * rstd : 0.f;
+      }
+      if (KEEP && add) res[k] = next_r[k];
+    }
+    if (row + stride < rows) fetch(row + stride);
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      const int c = (part + k * W) * 256 + 8 * lane, valid = valid_of<VEC>(E, c);
       if (partial) {
-        float4 a = acc[64 * k], d = acc[64 * k + 32];
-        a.x = fmaf(g[k][0], z[k][0], a.x); a.y = fmaf(g[k][1], z[k][1], a.y); a.z = fmaf(g[k][2], z[k][2], a.z); a.w = fmaf(g[k][3], z[k][3], a.w);
-        d.x += g[k][0]; d.y += g[k][1]; d.z += g[k][2]; d.w += g[k][3];
-        acc[64 * k] = a;
-        acc[64 * k + 32] = d;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float4 a = acc[128 * k + 32 * h], d = acc[128 * k + 64 + 32 * h];
+          a.x = fmaf(g[k][4 * h], z[k][4 * h], a.x); a.y = fmaf(g[k][4 * h + 1], z[k][4 * h + 1], a.y);
+          a.z = fmaf(g[k][4 * h + 2], z[k][4 * h + 2], a.z); a.w = fmaf(g[k][4 * h + 3], z[k][4 * h + 3], a.w);
+          d.x += g[k][4 * h]; d.y += g[k][4 * h + 1]; d.z += g[k][4 * h + 2]; d.w += g[k][4 * h + 3];
+          acc[128 * k + 32 * h] = a;
+          acc[128 * k + 64 + 32 * h] = d;
+        }
       }
       if (w) {
-        float ww[4];
-        load4(w + c, vec, valid, ww);
+        Raw8<T> p;
+        float f[8];
+        p.load(w + c, VEC, valid);
+        p.get(f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) g[k][j] *= ww[j];
+        for (int j = 0; j < 8; ++j) g[k][j] *= f[j];
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { s1 += g[k][j]; s2 = fmaf(g[k][j], z[k][j], s2); }
+      for (int j = 0; j < 8; ++j) { s1 += g[k][j]; s2 = fmaf(g[k][j], z[k][j], s2); }
     }
     const float m1 = team_sum<W>(s1, s_sum[flip][0], warp) * inv_e, m2 = team_sum<W>(s2, s_sum[flip][1], warp) * inv_e;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int c = (part + k * W) * kBlock + 4 * lane, valid = max(0, min(4, E - c));
-      float o[4], r[4] = {0.f, 0.f, 0.f, 0.f};
-      if (add) load4(add + row * E + c, vec, valid, r);
+    for (int k = 0; k < NG; ++k) {
+      const int c = (part + k * W) * 256 + 8 * lane, valid = valid_of<VEC>(E, c);
+      float o[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = fmaf(rstd, g[k][j] - m1 - z[k][j] * m2, r[j]);
-      store4(dx + row * E + c, vec, valid, o);
+      for (int j = 0; j < 8; ++j) o[j] = rstd * (g[k][j] - m1 - z[k][j] * m2);
+      if (add) {
+        Raw8<T> p;
+        float f[8];
+        if (KEEP) p = res[k]; else p.load(add + row * E + c, VEC, valid);
+        p.get(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] += f[j];
+      }
+      store8(dx + row * E + c, VEC, valid, o);
     }
   }
   if (!partial) return;
@@ -432,10 +494,11 @@ __global__ void __launch_bounds__(256, 2) norm_backward_team_kernel(const unsign
   float* out = partial + (long long)blockIdx.x * 2 * E;
   const float* flat = reinterpret_cast<const float*>(s_acc);
   for (int i = threadIdx.x; i < 2 * E; i += 256) {
-    const int which = i >= E, c = which ? i - E : i, block = c / kBlock, at = c % kBlock;
+    const int which = i >= E, c = which ? i - E : i, group = c >> 8, in_lane = c & 7, at = (c >> 3) & 31;
+    const int offset = (2 * which + (in_lane >> 2)) * 128 + at * 4 + (in_lane & 3);
     float sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < 8 / W; ++t) sum += flat[(((long long)(t * W + block % W) * NB + block / W) * 2 + which) * kBlock + at];
+    for (int t = 0; t < 8 / W; ++t) sum += flat[((t * W + group % W) * NG + group / W) * 512 + offset];
     out[i] = sum;
   }
 }
@@ -594,16 +657,20 @@ static int check_norm(const char* who, int dtype, int64_t rows, int64_t E) {
   return HAPX_OK;
 }
 
-// Warps per row and blocks of 128 columns per warp (at most) for a row of E <= kTeamColumns.
-static int team_warps(long long E) { return E <= 1024 ? 1 : E <= 2048 ? 2 : E <= 4096 ? 4 : 8; }
+// Warps per row, and groups of 256 columns per warp at most, for a row of E <= kTeamColumns.
+static int team_warps(long long E) { return E <= 768 ? 1 : E <= 1024 ? 2 : E <= 2048 ? 4 : 8; }
 #define HAPX_LN8_SWITCH(E)                  \
-  if ((E) <= 256) HAPX_LN8_TEAM(1, 2);      \
-  else if ((E) <= 512) HAPX_LN8_TEAM(1, 4); \
-  else if ((E) <= 768) HAPX_LN8_TEAM(1, 6); \
-  else if ((E) <= 1024) HAPX_LN8_TEAM(1, 8); \
-  else if ((E) <= 2048) HAPX_LN8_TEAM(2, 8); \
-  else if ((E) <= 4096) HAPX_LN8_TEAM(4, 8); \
-  else if ((E) <= kTeamColumns) HAPX_LN8_TEAM(8, 8);
+  if ((E) <= 256) HAPX_LN8_TEAM(1, 1);      \
+  else if ((E) <= 512) HAPX_LN8_TEAM(1, 2); \
+  else if ((E) <= 768) HAPX_LN8_TEAM(1, 3); \
+  else if ((E) <= 1024) HAPX_LN8_TEAM(2, 2); \
+  else if ((E) <= 2048) HAPX_LN8_TEAM(4, 2); \
+  else if ((E) <= 4096) HAPX_LN8_TEAM(8, 2); \
+  else if ((E) <= kTeamColumns) HAPX_LN8_TEAM(8, 4);
+
+static bool on_16_bytes(const void* a, const void* b, const void* c, const void* d) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
+}
 
 // 64 KiB of dynamic shared memory for a kernel on the current device (asked for once).
 static int allow_shared(const void* kernel) {
@@ -696,11 +763,14 @@ int hapx_layer_norm8_forward(const void* x, const void* gamma, const void* beta,
 #define HAPX_LN8(T, KERNEL, THREADS) \
   KERNEL<<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(gamma), static_cast<const T*>(beta), static_cast<T*>(y), mean, \
                                        rstd, q, ld_saved, scales, rows, (int)E, (float)eps)
-#define HAPX_LN8_TEAM(W, NB)                                                                    \
-  do {                                                                                          \
-    if (int e = grid_for((rows + 8 / W - 1) / (8 / W), NB <= 4 ? 4 : NB <= 6 ? 3 : 2, &grid)) return e; \
-    if (dtype == HAPX_BF16) HAPX_LN8(__nv_bfloat16, (norm_forward_team_kernel<__nv_bfloat16, W, NB>), 256); \
-    else HAPX_LN8(float, (norm_forward_team_kernel<float, W, NB>), 256);                        \
+  const bool vec = E % 8 == 0 && on_16_bytes(x, y, gamma, beta);
+#define HAPX_LN8_TEAM(W, NG)                                                                                                     \
+  do {                                                                                                                           \
+    if (int e = grid_for((rows + 8 / W - 1) / (8 / W), 2, &grid)) return e;                                                      \
+    if (dtype == HAPX_BF16) { if (vec) HAPX_LN8(__nv_bfloat16, (norm_forward_team_kernel<__nv_bfloat16, W, NG, true>), 256);     \
+                              else HAPX_LN8(__nv_bfloat16, (norm_forward_team_kernel<__nv_bfloat16, W, NG, false>), 256); }      \
+    else { if (vec) HAPX_LN8(float, (norm_forward_team_kernel<float, W, NG, true>), 256);                                        \
+           else HAPX_LN8(float, (norm_forward_team_kernel<float, W, NG, false>), 256); }                                         \
   } while (0)
   HAPX_LN8_SWITCH(E)
   else {
@@ -741,19 +811,20 @@ int hapx_layer_norm8_backward(const void* saved, int64_t ld_saved, const float* 
   long long slices = 0;
   int grid = 1;
   if (rows > 0) {
-#define HAPX_LN8_RUN(T, W, NB)                                                                                                              \
+    const bool vec = E % 8 == 0 && on_16_bytes(dy, dx, gamma, add);
+#define HAPX_LN8_RUN(T, W, NG, VEC)                                                                                                         \
   do {                                                                                                                                      \
-    auto kernel = norm_backward_team_kernel<T, W, NB>;                                                                                      \
+    auto kernel = norm_backward_team_kernel<T, W, NG, VEC>;                                                                                 \
     if (int e = allow_shared(reinterpret_cast<const void*>(kernel))) return e;                                                              \
-    kernel<<<grid, 256, params ? 8 * NB * 1024 : 0, stream>>>(q, ld_saved, scales, static_cast<const T*>(dy), static_cast<const T*>(gamma), mean, \
+    kernel<<<grid, 256, params ? 8 * NG * 2048 : 0, stream>>>(q, ld_saved, scales, static_cast<const T*>(dy), static_cast<const T*>(gamma), mean, \
                                                               rstd, static_cast<const T*>(add), static_cast<T*>(dx), partial, rows, (int)E); \
   } while (0)
-#define HAPX_LN8_TEAM(W, NB)                                                             \
+#define HAPX_LN8_TEAM(W, NG)                                                             \
   do {                                                                                   \
     if (int e = grid_for((rows + 8 / W - 1) / (8 / W), 2, &grid)) return e;              \
     slices = grid;                                                                       \
-    if (dtype == HAPX_BF16) HAPX_LN8_RUN(__nv_bfloat16, W, NB);                          \
-    else HAPX_LN8_RUN(float, W, NB);                                                     \
+    if (dtype == HAPX_BF16) { if (vec) HAPX_LN8_RUN(__nv_bfloat16, W, NG, true); else HAPX_LN8_RUN(__nv_bfloat16, W, NG, false); } \
+    else { if (vec) HAPX_LN8_RUN(float, W, NG, true); else HAPX_LN8_RUN(float, W, NG, false); }                                    \
   } while (0)
     HAPX_LN8_SWITCH(E)
     else {
