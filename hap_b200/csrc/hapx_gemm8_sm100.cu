@@ -266,7 +266,10 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
         if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok && lane == 0) atomicCAS(params.error, 0u, 1u);
+    if (!ok) {
+      if (lane == 0) atomicCAS(params.error, 0u, 1u);
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);      // a millisecond for the copies in flight to land
+    }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
     if (cta == 0) {
@@ -691,8 +694,7 @@ static int launch(const Maps& maps, const Params& p, int sm_count, cudaStream_t 
       limit_of[device] = limit;
     }
   }
-  // one product: no more workers than units; two: as many as the plan dealt them out to
-  const int workers = PAIR && p.units[1] > 0 ? std::min(limit, sm_count / 2) : std::min(p.units[0], limit);
+  const int workers = std::min(p.units[0] + p.units[1], limit);
   cfg.gridDim = dim3((unsigned)(workers * (PAIR ? 2 : 1)));
   HAPX_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, p));
   count_launch();

@@ -231,11 +231,19 @@ def test_linear8_prepared_weight():
     xg, bg = leaf(x), leaf(b)
     hap_b200.linear8(xg, block8.quantize_weight(w.to(DEV), transposed=True), bg).backward(g.to(DEV))
     check_linear((y, xg.grad, None, bg.grad), want, 77, 300, 130)
+    bg = leaf(b)
+    hap_b200.linear8(x.to(DEV), w8, bg).backward(g.to(DEV))                  # only the bias learns
+    check_linear((None, None, None, bg.grad), want, 77, 300, 130)
+    # a weight in 1 x 128 blocks serves too
+    w1 = block8.quantize(w.to(DEV))
+    y1 = hap_b200.linear8(x.to(DEV), w1)
+    xv, wv = B.fast_rows(x), B.fast_rows(w)
+    close(y1, xv @ wv.t(), sum_slack(xv.abs() @ wv.abs().t(), 300))
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("rows,fin,fout", [(1, 768, 2304), (1, 1, 1), (2, 130, 77), (3, 5000, 64), (8, 1000, 129), (8, 4096, 40), (9, 768, 768), (33, 129, 300),
-                                           (64, 1024, 512), (65, 100, 200), (100, 640, 33), (128, 513, 264), (129, 256, 192), (40, 8192, 64)])
+                                           (64, 1024, 512), (65, 100, 200), (100, 640, 33), (128, 513, 264), (129, 256, 192), (40, 8192, 64), (20, 8192, 64), (1, 25000, 40)])
 def test_linear8_few_tokens_prepared_weight(dtype, rows, fin, fout):
     """Every way the tokens reach the product (a warp per output, converted inside the product, quantised before it) gives
     the result of the plain call; rows with infinities and NaN, strided rows."""
@@ -254,6 +262,38 @@ def test_linear8_few_tokens_prepared_weight(dtype, rows, fin, fout):
     y = hap_b200.linear8(x.to(DEV), w8).cpu()
     bad = torch.isnan(x).any(1) | torch.isinf(x).any(1)
     assert bool(torch.isnan(y[bad]).all()) and bool(torch.isfinite(y[~bad]).all())
+
+
+def test_linear8_uses_the_same_leaf_twice_and_keeps_its_graph():
+    import hap_b200
+    x, w, b, g = linear_inputs(60, 96, 96, F32)
+    xg, wg = leaf(x), leaf(w)
+    y = hap_b200.linear8(hap_b200.linear8(xg, wg), wg)
+    first = torch.autograd.grad(y, [xg, wg], g.to(DEV), retain_graph=True)
+    again = torch.autograd.grad(y, [xg, wg], g.to(DEV))
+    for a, c in zip(first, again):
+        assert torch.equal(a, c) and float(a.abs().max()) > 0
+    mid = hap_b200.linear8(xg.detach(), wg.detach()).requires_grad_(True)
+    w1, w2 = leaf(w), leaf(w)
+    dmid, d2 = torch.autograd.grad(hap_b200.linear8(mid, w2), [mid, w2], g.to(DEV))
+    (d1,) = torch.autograd.grad(hap_b200.linear8(xg.detach(), w1), [w1], dmid)
+    assert torch.equal(first[1], d1 + d2) or torch.equal(first[1], d2 + d1)
+
+
+def test_linear8_large_offsets():
+    """An output of more than 2^31 elements: the last rows and columns are where they belong."""
+    import hap_b200
+    from hap_b200 import block8
+    rows, fin, fout = 70000, 16, 33000
+    x = torch.zeros(rows, fin, dtype=BF, device=DEV)
+    w = torch.zeros(fout, fin, dtype=BF, device=DEV)
+    x[-300:] = torch.randn(300, fin, generator=gen(0)).to(BF).to(DEV)
+    w[-200:] = torch.randn(200, fin, generator=gen(1)).to(BF).to(DEV)
+    y = hap_b200.linear8(x, block8.quantize_weight(w))
+    assert y.numel() > 2 ** 31
+    xv, wv = B.fast_rows(x[-300:].cpu()), B.quantize(w.cpu()[32640:], True)[0]           # from a whole block of 128 weight rows on
+    close(y[-300:, 32640:], xv @ wv.t(), sum_slack(xv.abs() @ wv.abs().t(), fin))
+    assert float(y[:-300].abs().max()) == 0.0
 
 
 def test_linear8_refusals():
@@ -392,7 +432,8 @@ def norm_bounds(x, w, b, g, kept, want, rows):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("rows,E", [(1, 1), (1, 8), (5, 33), (3, 129), (591, 768), (130, 2048), (64, 1288), (33, 5000), (200, 127)])
+@pytest.mark.parametrize("rows,E", [(1, 1), (1, 8), (5, 33), (3, 129), (591, 768), (130, 2048), (64, 1288), (33, 5000), (200, 127), (2000, 256), (70, 400),
+                                    (9, 1000), (40, 4096), (5, 8192), (70, 9001), (3, 20000)])
 @pytest.mark.parametrize("affine", ["both", "weight", "none"])
 def test_layer_norm8(dtype, rows, E, affine):
     import hap_b200
@@ -433,7 +474,7 @@ def test_layer_norm8_gradient_against_differences():
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("shape", [(40, 3, 768), (9, 2, 65)])
+@pytest.mark.parametrize("shape", [(40, 3, 768), (9, 2, 65), (5, 2, 3000), (3, 2, 9001)])
 def test_layer_norm_fork8(dtype, shape):
     from hap_b200.norm import layer_norm8, layer_norm_fork8
     E, rows = shape[-1], shape[0] * shape[1]
