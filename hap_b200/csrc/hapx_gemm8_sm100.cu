@@ -5,17 +5,21 @@
 // The scales are applied by the tensor cores (tcgen05.mma kind::mxf8f6f4, which multiplies every 32 products by the two
 // scales of their row and column before adding them): the four 32-deep instructions of a block of 128 name the same
 // scale bytes.  So an accumulator runs over the whole contraction, as in the bfloat16 product (hapx_gemm_sm100.cu),
-// whose structure this kernel has: persistent, warp-specialised, two accumulators used alternately.
+// whose structure this kernel has: persistent, warp-specialised, accumulators in tensor memory.
 //   warp 0      : TMA producer (128 x 128 byte tiles, 128-byte swizzle; every fourth block also the scales of four blocks)
 //   warp 1      : allocates TMEM; one thread copies scales to tensor memory (tcgen05.cp) and issues tcgen05.mma
-//   the others  : epilogue, a warp per 32 rows x 64 columns: bias, one rounding, bulk stores through a staging tile
+//   the others  : epilogue, a warp per 32 rows x 64 columns (or two such pieces): bias, one rounding, bulk stores through a staging tile
 // (An earlier form kept one accumulator per block and the running sums in registers, adding block products with their
 // scales in the epilogue warps; it was bound by the chain commit -> wait -> read -> arrive of its two accumulators.)
 //
-// Pair kernel (M > 128): clusters of two CTAs, 256 x 192 tiles, cta_group::2; each CTA stages its 128 rows of A and half
-// of B's rows.  192 columns, because two accumulators of 192 leave tensor memory for the scales, and the model widths
-// (768, 2304) are whole numbers of such tiles.  Single kernel (M <= 128): 128 x 64 tiles, so that a narrow product still
-// spreads over the SMs.
+// Pair kernel (M > 128): clusters of two CTAs, cta_group::2; each CTA stages its 128 rows of A and half of B's rows.  Tiles
+// of 256 x 192 with two accumulators (which leave tensor memory for the scales, and divide widths of 768 and 2304), or of
+// 256 x 256 with one: unit_us chooses.  Single kernel (M <= 128): 128 x 64 tiles, so that a narrow product still spreads
+// over the SMs.
+//
+// 8192 x 8192 x 8192: 380 us = 2.9 PFLOP/s (the library's bfloat16 product 690 us); without its loads 4.1 PFLOP/s: bound by
+// what goes into shared memory and by power.  8192 x 33280 from 768: 205 us, of which 138 are what filling the 545 MB of
+// output takes.  8192 x 768 -> 2304 and back: 16, 15 and 20 us (forward, to the input, to the weight).
 //
 // Single kernel with X (a float type): the first operand comes as it is, bfloat16 or float32, and eight more warps make its
 // 8-bit tiles and scales in shared memory as the blocks go by, for themselves in every thread block: one launch for a few
@@ -53,7 +57,7 @@ struct Problem {
   void* D; long long ldd;
   const void* bias;          // N values of D's type, or null
   int out_f32, tma_store, bias_vec;
-  int m_tiles, n_tiles;
+  int m_tiles, n_tiles, band;
   int splits, kb_per_split;  // > 1: the blocks are cut into ranges; each writes a float32 partial tile to rows [split * m_pad, ...)
   long long m_pad;
   const float* colsum;       // null, or colsum_tiles x M floats whose column sums go to colsum_out (the bias gradient that
@@ -100,21 +104,25 @@ __device__ __forceinline__ void copy_scales(unsigned taddr, unsigned smem) {
   else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-template <bool PAIR, bool CONVERT = false>
+// BN: columns of the tile - 192 or 256 for the pair kernel, 64 for the single one.
+template <int BN_, bool CONVERT = false>
 struct Cfg {
-  static constexpr int BN = PAIR ? 192 : 64;                 // columns of the tile
+  static constexpr int BN = BN_;
+  static constexpr bool PAIR = BN > 64;
+  static constexpr int ACCS = 2 * BN + 64 <= 512 ? 2 : 1;    // accumulators in tensor memory, next to the scales
   static constexpr int PIECES = BN / 64;                     // 64 columns: 128 bytes of a bfloat16 row
-  static constexpr int EPI_WARPS = 4 * PIECES;               // one piece of 32 rows each
+  static constexpr int PARTS = BN == 256 ? 2 : PIECES;       // pieces that are worked on at a time, one of 32 rows per warp
+  static constexpr int EPI_WARPS = 4 * PARTS;
   static constexpr int CONVERT_WARPS = CONVERT ? 8 : 0;      // every eighth block each
   static constexpr int THREADS = 64 + 32 * (EPI_WARPS + CONVERT_WARPS);
-  static constexpr int STAGES = PAIR ? 6 : 7;
+  static constexpr int STAGES = BN == 256 ? 5 : PAIR ? 6 : 7;
   static constexpr int B_ATOMS = PAIR ? 2 : 1;               // 192 columns from a multiple of 64 on lie in two groups of 128
   static constexpr unsigned A_BYTES = BM * BK;
   static constexpr unsigned B_BYTES = (PAIR ? BN / 2 : BN) * BK;
   static constexpr unsigned STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr unsigned SCALE_BYTES = (1 + B_ATOMS) * kAtom;
   static constexpr unsigned STORE_BYTES = EPI_WARPS * 32 * 128;  // one 32-row x 128-byte staging tile per epilogue warp
-  static constexpr unsigned SF_COL = 2 * BN;                 // scales behind the accumulators, one set per stage
+  static constexpr unsigned SF_COL = ACCS * BN;              // scales behind the accumulators, one set per stage
   static constexpr unsigned SF_SET = 4 * (1 + B_ATOMS);
   static constexpr unsigned TMEM_COLS = PAIR ? 512 : 256;
   static_assert(SF_COL + STAGES * SF_SET <= TMEM_COLS, "tensor memory");
@@ -126,46 +134,34 @@ struct Cfg {
 };
 
 // One 128-byte row piece per thread, swizzled within the warp's staging tile (chunk ^ row % 8).
-template <bool OUT_F32>
-__device__ __forceinline__ void stage_row(unsigned char* row, int sw, const float* v) {
-  if constexpr (OUT_F32) {
+__device__ __forceinline__ void stage_row(unsigned char* row, int sw, const unsigned (&w)[32]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(row + ((j ^ sw) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      unsigned w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
-        w[e] = *reinterpret_cast<const unsigned*>(&h);
-      }
-      *reinterpret_cast<uint4*>(row + ((j ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
+  for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(row + ((j ^ sw) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
 // v[j] += bias[n + j] (float32) for the columns inside the matrix; `vec`: all are, and the bias lies on 16 bytes.
-__device__ __forceinline__ void add_bias(const Problem& p, int n, bool vec, float (&v)[32]) {
+__device__ __forceinline__ void add_bias(const Problem& p, int n, bool vec, unsigned (&v)[32]) {
   const float* bias = static_cast<const float*>(p.bias) + n;
+  auto add = [&](int j, float x) { v[j] = __float_as_uint(__uint_as_float(v[j]) + x); };
   if (vec) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float4 x = __ldg(reinterpret_cast<const float4*>(bias) + j);
-      v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+      add(4 * j, x.x); add(4 * j + 1, x.y); add(4 * j + 2, x.z); add(4 * j + 3, x.w);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (n + j < p.N) v[j] += bias[j];
+      if (n + j < p.N) add(j, bias[j]);
   }
 }
 
-template <bool PAIR, typename X>
-__global__ void __launch_bounds__(Cfg<PAIR, !std::is_void<X>::value>::THREADS, 1)
+template <int BN, typename X>
+__global__ void __launch_bounds__(Cfg<BN, !std::is_void<X>::value>::THREADS, 1)
 gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params params) {
   constexpr bool CONVERT = !std::is_void<X>::value;
-  using C = Cfg<PAIR, CONVERT>;
+  using C = Cfg<BN, CONVERT>;
+  constexpr bool PAIR = C::PAIR;
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -200,8 +196,16 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
     const Problem& p = params.pr[u.which];
     const int tile = unit / p.splits;
     u.split = unit - tile * p.splits;
-    u.m0 = (tile % p.m_tiles) * (PAIR ? 2 * BM : BM) + cta * BM;
-    u.n0 = (tile / p.m_tiles) * C::BN;
+    int row = tile, column, row0 = 0, rows = p.m_tiles;
+    if (p.band) {                                            // so many rows of tiles across all columns, then the next ones
+      const int band = tile / (p.band * p.n_tiles);
+      row0 = band * p.band;
+      row = tile - row0 * p.n_tiles;
+      rows = min(p.band, p.m_tiles - row0);
+    }
+    column = row / rows;
+    u.m0 = (row0 + row - column * rows) * (PAIR ? 2 * BM : BM) + cta * BM;
+    u.n0 = column * C::BN;
     u.kb0 = u.split * p.kb_per_split;
     u.kb1 = min(u.kb0 + p.kb_per_split, p.k_blocks);
     return true;
@@ -313,7 +317,7 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
       }
       if (!ok && lane == 0) atomicCAS(params.error, 0u, 2u);
     }
@@ -417,16 +421,14 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
           else static_cast<__nv_bfloat16*>(p.colsum_out)[row] = __float2bfloat16_rn(sum);
         }
       }
-      const int n0 = u.n0 + 64 * part, width = min(64, p.N - n0);   // this warp's columns inside the matrix (may be none)
-      const bool bias_vec = p.bias_vec && width == 64;
-      if (bias_vec && lane == 0) {                           // comes closer during the wait
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + (long long)n0 * (p.out_f32 ? 4 : 2)));
-        if (p.out_f32) asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + (long long)n0 * 4 + 128));
+      if (p.bias_vec && lane < C::PIECES / C::PARTS && u.n0 + 64 * (part + C::PARTS * lane) + 64 <= p.N) {   // comes closer during the wait
+        const long long n0 = u.n0 + 64 * (part + C::PARTS * lane);
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + n0 * (p.out_f32 ? 4 : 2)));
+        if (p.out_f32) asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + n0 * 4 + 128));
       }
       ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
       if (!ok) break;
       tc_fence_after();
-      const unsigned t = tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(acc * C::BN + 64 * part);
       const long long out_row0 = (long long)u.split * p.m_pad + u.m0 + q * 32;
       auto drained = [&] {                                   // this warp has read its part of the accumulator
         tc_fence_before();
@@ -436,15 +438,15 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
           else mbar_arrive(tempty_bar(acc));
         }
       };
-      // W columns from c on, staged as 128 bytes per row: out in one bulk store, or row by row for any pitch
-      auto send = [&](auto f32_tag, int c) {
+      // W columns from n0 on, `width` of them inside the matrix, staged as 128 bytes per row: out in one bulk store, or row by row for any pitch
+      auto send = [&](auto f32_tag, int n0, int width) {
         constexpr bool OUT_F32 = decltype(f32_tag)::value;
         constexpr int W = OUT_F32 ? 32 : 64;
         if (p.tma_store) {
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            tma_store_4d(&maps.d[u.which], tile_u32, n0 + c, (int)out_row0, 0, 0);
+            tma_store_4d(&maps.d[u.which], tile_u32, n0, (int)out_row0, 0, 0);
             bulk_commit_group();
           }
         } else {
@@ -455,9 +457,9 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
 #pragma unroll
           for (int h = 0; h < W / 32; ++h) {
             const int col = lane + 32 * h, byte = col * ES;
-            if (c + col >= width) continue;
+            if (col >= width) continue;
             const unsigned char* src = tile_gen + (byte & 15);
-            Bits* dst = static_cast<Bits*>(p.D) + out_row0 * p.ldd + n0 + c + col;
+            Bits* dst = static_cast<Bits*>(p.D) + out_row0 * p.ldd + n0 + col;
 #pragma unroll 1
             for (int i0 = 0; i0 < rows; i0 += 8) {           // eight rows in flight
               Bits v[8];
@@ -476,50 +478,68 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
         if (lane == 0) bulk_wait_read_0();
         __syncwarp();
       };
-      if (width <= 0) {
-        drained();
-      } else if (p.out_f32) {
+      const int n0 = u.n0 + 64 * part;                       // a warp's pieces of 64 columns lie 64 * PARTS apart
+      const unsigned t = tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(acc * C::BN + 64 * part);
+      constexpr int PER = C::PIECES / C::PARTS;
+      if (p.out_f32) {
 #pragma unroll 1
-        for (int c = 0; c < 64 && c < width; c += 32) {
+        for (int i = 0; i < 2 * PER; ++i) {
+          const int off = (i >> 1) * 64 * C::PARTS + (i & 1) * 32, n = n0 + off, width = min(32, p.N - n);
           unsigned r[32];
-          tmem_ld_32x32(t + (unsigned)c, r);
+          tmem_ld_32x32(t + (unsigned)off, r);
           tmem_ld_wait();
-          if (c + 32 >= width) drained();
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          if (p.bias) add_bias(p, n0 + c, bias_vec, v);
+          if (i == 2 * PER - 1) drained();
+          if (width <= 0) continue;
+          if (p.bias) add_bias(p, n, p.bias_vec && width == 32, r);
           staging_free();
-          stage_row<true>(tile_gen + lane * 128, lane & 7, v);
-          send(std::true_type{}, c);
+          stage_row(tile_gen + lane * 128, lane & 7, r);
+          send(std::true_type{}, n, width);
         }
       } else {
         unsigned r[64];
-        tmem_ld_32x32(t, reinterpret_cast<unsigned(&)[32]>(r[0]));
-        tmem_ld_32x32(t + 32, reinterpret_cast<unsigned(&)[32]>(r[32]));
-        tmem_ld_wait();
-        drained();
-        float v[64];
+        auto load = [&](int off) {
+          tmem_ld_32x32(t + (unsigned)off, reinterpret_cast<unsigned(&)[32]>(r[0]));
+          tmem_ld_32x32(t + (unsigned)off + 32, reinterpret_cast<unsigned(&)[32]>(r[32]));
+          tmem_ld_wait();
+        };
+        load(0);
+        if (PER == 1) drained();
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j]);
-        if (bias_vec) {
+        for (int i = 0; i < PER; ++i) {
+          const int n = n0 + i * 64 * C::PARTS, width = min(64, p.N - n);
+          float v[64];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + n0) + j);
-            const unsigned w[4] = {x.x, x.y, x.z, x.w};
+          for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j]);
+          if (p.bias_vec && width == 64) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { v[8 * j + 2 * e] += __uint_as_float(w[e] << 16); v[8 * j + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u); }
+            for (int j = 0; j < 8; ++j) {
+              const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.bias) + n) + j);
+              const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { v[8 * j + 2 * e] += __uint_as_float(w[e] << 16); v[8 * j + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u); }
+            }
+          } else if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (j < width) v[j] += __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n + j]);
           }
-        } else if (p.bias) {
+          staging_free();
+          unsigned w[32];
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (j < width) v[j] += __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n0 + j]);
+          for (int j = 0; j < 32; ++j) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const unsigned*>(&h);
+          }
+          if (i + 1 < PER) {                                 // the accumulator is let go before anything is stored
+            load((i + 1) * 64 * C::PARTS);
+            if (i + 2 == PER) drained();
+          }
+          if (width <= 0) continue;
+          stage_row(tile_gen + lane * 128, lane & 7, w);
+          send(std::false_type{}, n, width);
         }
-        staging_free();
-        stage_row<false>(tile_gen + lane * 128, lane & 7, v);
-        send(std::false_type{}, 0);
       }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) bulk_wait_all();
     if (!ok) atomicCAS(params.error, 0u, 3u);
@@ -584,13 +604,13 @@ static int make_map(CUtensorMap* map, const void* ptr, CUtensorMapDataType type,
   return HAPX_OK;
 }
 
-// How a product is cut: by the pair kernel or the single one, and into how many ranges of blocks.
-struct Plan { bool pair; int splits, kb_per_split; long long m_pad, tiles; int n_pad, blocks; };
+// How a product is cut: into tiles of 64 (single kernel), 192 or 256 columns, and into how many ranges of blocks.
+struct Plan { int bn, f32, splits, kb_per_split; long long m_pad, tiles; int n_pad, blocks; };
 
-static Plan plan_whole(long long M, long long N, long long K, bool pair) {
+static Plan plan_whole(long long M, long long N, long long K, int f32, int bn) {
   Plan pl;
-  pl.pair = pair;
-  const long long bm = pair ? 2 * BM : BM, bn = pair ? Cfg<true>::BN : Cfg<false>::BN, m_tiles = (M + bm - 1) / bm;
+  pl.bn = bn; pl.f32 = f32;
+  const long long bm = bn > 64 ? 2 * BM : BM, m_tiles = (M + bm - 1) / bm;
   pl.tiles = m_tiles * ((N + bn - 1) / bn);
   pl.blocks = (int)((K + BK - 1) / BK);
   pl.splits = 1; pl.kb_per_split = pl.blocks; pl.m_pad = m_tiles * bm; pl.n_pad = (int)((N + 3) / 4 * 4);
@@ -602,38 +622,52 @@ static bool cut(Plan& pl, int splits) {        // false where a range would be e
   pl.splits = splits; pl.kb_per_split = per;
   return true;
 }
-// Microseconds of one block of a tile (measured: 0.30 to 0.33 of a pair's 256 x 192, long contractions), and of a split:
-// its partial tiles written and read back at about 4 TB/s plus a launch.
-static double block_us(bool pair) { return pair ? 0.30 : 0.15; }
+// Microseconds of a tile's unit of so many blocks, fitted to measurements, and of a split: its partial tiles written and
+// read back at about 4 TB/s plus a launch.  A block of 256 x 256 is a third more work than one of 256 x 192 for a seventh
+// more bytes into shared memory, but its accumulator has no second one, so nothing hides its drain; and 256 columns may
+// divide a width better or worse.  (192 against 256: 4096 x 1024 from 8192 36.4 / 27.2 us, 8192^3 396 / 384,
+// 16384 x 4096 from 1024 65.5 / 62.7; 8192 x 768 from 2304 15.8 / 18.9, 4096 x 4096 from 1024 19.3 / 20.2.)
+// Twice as many bytes of float32 take 0.8 us longer to leave (8192 x 4096 from 1024 with its quantiser: 64.8 us in 256 columns, 59.1 in 192).
+static double unit_us(const Plan& pl) {
+  const int kb = pl.kb_per_split;
+  return pl.bn == 64 ? 0.15 * kb : pl.bn == 192 ? 0.29 * kb + 0.8 : 0.39 * kb + (pl.f32 || pl.splits > 1 ? 1.95 : 1.15);
+}
 static double split_us(const Plan& pl) { return pl.splits > 1 ? 3.0 + pl.splits * 8.0 * (double)pl.m_pad * pl.n_pad / 4e6 : 0.0; }
 
 // A long contraction over few tiles leaves SMs idle, or the last round of tiles nearly empty: cut the blocks into ranges
 // whose float32 partial tiles a second kernel adds in a fixed order, where that costs less by a clear margin.
-static Plan plan_of(long long M, long long N, long long K, int sm_count) {
-  Plan best = plan_whole(M, N, K, M > BM), pl = best;
-  const int workers = pl.pair ? sm_count / 2 : sm_count;
-  auto cost = [&](const Plan& q) { return (double)((q.tiles * q.splits + workers - 1) / workers) * q.kb_per_split * block_us(q.pair) + split_us(q); };
-  for (int sp = 2; sp <= 16; ++sp)
-    if (cut(pl, sp) && cost(pl) < 0.9 * cost(best)) best = pl;
-  return best;
+static Plan plan_of(long long M, long long N, long long K, int f32, int sm_count) {
+  auto cost = [&](const Plan& q) {
+    const int workers = q.bn > 64 ? sm_count / 2 : sm_count;
+    return (double)((q.tiles * q.splits + workers - 1) / workers) * unit_us(q) + split_us(q);
+  };
+  auto best_of = [&](int bn) {
+    Plan best = plan_whole(M, N, K, f32, bn), pl = best;
+    for (int sp = 2; sp <= 16; ++sp)
+      if (cut(pl, sp) && cost(pl) < 0.9 * cost(best)) best = pl;
+    return best;
+  };
+  if (M <= BM) return best_of(64);
+  const Plan a = best_of(192), b = best_of(256);
+  return cost(b) < cost(a) ? b : a;
 }
 
-// Blocks until the last worker is done with two products dealt out as the kernel does it, the longer units first; and
-// the number of rounds of the second product's units for all workers.
-static long long makespan(const Plan& a, const Plan& b, int workers, int* rounds) {
-  const long long ua = a.tiles * a.splits, ub = b.tiles * b.splits, la = a.kb_per_split, lb = b.kb_per_split;
-  const long long full = ua / workers, left = ua % workers;
+// Microseconds until the last worker is done with two products dealt out as the kernel does it, the longer units first;
+// and the number of rounds of the second product's units for all workers.
+static double makespan(const Plan& a, const Plan& b, int workers, int* rounds) {
+  const long long ua = a.tiles * a.splits, ub = b.tiles * b.splits, full = ua / workers, left = ua % workers, all = (ub + workers - 1) / workers;
+  const double la = unit_us(a), lb = unit_us(b);
   if (left == 0) {
-    *rounds = (int)((ub + workers - 1) / workers);
-    return full * la + *rounds * lb;
+    *rounds = (int)all;
+    return full * la + all * lb;
   }
-  const long long ideal = (ua * la + ub * lb + workers - 1) / workers, guess = std::max(0ll, (ideal - (full + 1) * la) / lb);
-  long long best = -1;
+  const double ideal = (ua * la + ub * lb) / workers;
+  const long long guess = (long long)std::max(0.0, (ideal - (full + 1) * la) / lb);
+  double best = -1.0;
   for (long long r = guess; r <= guess + 1; ++r) {
-    const long long all = std::min(r, (ub + workers - 1) / workers), rest = std::max(0ll, ub - all * workers);
-    const long long more = (rest + workers - left - 1) / (workers - left);
-    const long long t = std::max((full + 1) * la + (ub > 0 ? all : 0) * lb, full * la + (all + more) * lb);
-    if (best < 0 || t < best) { best = t; *rounds = (int)all; }
+    const long long some = std::min(r, all), rest = std::max(0ll, ub - some * workers), more = (rest + workers - left - 1) / (workers - left);
+    const double t = std::max((full + 1) * la + some * lb, full * la + (some + more) * lb);
+    if (best < 0.0 || t < best) { best = t; *rounds = (int)some; }
   }
   return best;
 }
@@ -641,19 +675,21 @@ static long long makespan(const Plan& a, const Plan& b, int workers, int* rounds
 // Two products in one launch of the pair kernel: which goes first, its cut, the other's.
 struct PairPlan { Plan pl[2]; int first, rounds; };
 static PairPlan plan_two(const Product& x, const Product& y, int sm_count) {
-  const Plan whole[2] = {plan_whole(x.m, x.n, x.k, true), plan_whole(y.m, y.n, y.k, true)};
   const int workers = sm_count / 2;
   PairPlan best;
   double best_us = -1.0;
-  for (int cx = 1; cx <= 16; cx = cx < 4 ? cx + 1 : cx * 2) {
-    for (int cy = 1; cy <= 16; cy = cy < 4 ? cy + 1 : cy * 2) {
-      if (cx > 1 && cy > 1) continue;                       // one of the two at most
-      PairPlan t;
-      t.pl[0] = whole[0]; t.pl[1] = whole[1];
-      if (!cut(t.pl[0], cx) || !cut(t.pl[1], cy)) continue;
-      t.first = t.pl[1].kb_per_split > t.pl[0].kb_per_split;
-      const double us = makespan(t.pl[t.first], t.pl[!t.first], workers, &t.rounds) * block_us(true) + split_us(t.pl[0]) + split_us(t.pl[1]);
-      if (best_us < 0.0 || us < 0.9 * best_us) { best = t; best_us = us; }
+  for (int bn = 192; bn <= 256; bn += 64) {
+    const Plan whole[2] = {plan_whole(x.m, x.n, x.k, x.out_f32, bn), plan_whole(y.m, y.n, y.k, y.out_f32, bn)};
+    for (int cx = 1; cx <= 16; cx = cx < 4 ? cx + 1 : cx * 2) {
+      for (int cy = 1; cy <= 16; cy = cy < 4 ? cy + 1 : cy * 2) {
+        if (cx > 1 && cy > 1) continue;                       // one of the two at most
+        PairPlan t;
+        t.pl[0] = whole[0]; t.pl[1] = whole[1];
+        if (!cut(t.pl[0], cx) || !cut(t.pl[1], cy)) continue;
+        t.first = t.pl[1].kb_per_split > t.pl[0].kb_per_split;
+        const double us = makespan(t.pl[t.first], t.pl[!t.first], workers, &t.rounds) + split_us(t.pl[0]) + split_us(t.pl[1]);
+        if (best_us < 0.0 || us < 0.95 * best_us) { best = t; best_us = us; }
+      }
     }
   }
   return best;
@@ -661,10 +697,11 @@ static PairPlan plan_two(const Product& x, const Product& y, int sm_count) {
 
 static long long partial_bytes(const Plan& pl) { return pl.splits > 1 ? pl.splits * pl.m_pad * pl.n_pad * 4 : 0; }
 
-template <bool PAIR, typename X>
+template <int BN, typename X>
 static int launch(const Maps& maps, const Params& p, int sm_count, cudaStream_t stream) {
-  using C = Cfg<PAIR, !std::is_void<X>::value>;
-  auto kernel = gemm8_kernel<PAIR, X>;
+  using C = Cfg<BN, !std::is_void<X>::value>;
+  constexpr bool PAIR = C::PAIR;
+  auto kernel = gemm8_kernel<BN, X>;
   static int limit_of[64] = {};             // per device: function attributes and occupancy belong to one
   static std::mutex mutex;
   int device = 0;
@@ -701,6 +738,12 @@ static int launch(const Maps& maps, const Params& p, int sm_count, cudaStream_t 
   return HAPX_OK;
 }
 
+static int launch_plan(const Plan& pl, const Maps& maps, const Params& p, int sm_count, cudaStream_t stream) {
+  if (pl.bn == 64) return launch<64, void>(maps, p, sm_count, stream);
+  if (pl.bn == 192) return launch<192, void>(maps, p, sm_count, stream);
+  return launch<256, void>(maps, p, sm_count, stream);
+}
+
 // The scales as (128 words of an atom, group of 128 rows, four blocks).
 static int make_scale_map(CUtensorMap* map, const void* ptr, long long rows, int k_blocks, int box_groups) {
   gemm::EncodeTiledFn fn = gemm::encode_fn();
@@ -716,17 +759,26 @@ static int make_scale_map(CUtensorMap* map, const void* ptr, long long rows, int
   return HAPX_OK;
 }
 
-long long workspace_bytes(long long m, long long n, long long k, int sm_count) { return partial_bytes(plan_of(m, n, k, sm_count)); }
+long long workspace_bytes(long long m, long long n, long long k, int sm_count) {      // for either type of the output
+  return std::max(partial_bytes(plan_of(m, n, k, 0, sm_count)), partial_bytes(plan_of(m, n, k, 1, sm_count)));
+}
+
+// Tiles are walked down the rows, so that the second operand comes from memory once; a first operand too long for half of
+// L2 next to what else is there is walked in bands of eight rows of tiles, and then it comes once.  (33280 x 768 from 8192:
+// 212 / 164 us without / with bands; 16384 x 4096 from 4096 207 / 190; of 16 MB no difference, but two more divisions.)
+constexpr long long kLongOperand = 32ll << 20;
+constexpr int kBand = 8;
 
 // One product as entry i of a launch; `partial`: where its partial tiles go.
 static int describe(const Product& pr, const Plan& pl, void* partial, int i, Maps* maps, Params* params) {
   const long long M = pr.m, N = pr.n, K = pr.k;
-  const int bm = pl.pair ? 2 * BM : BM, bn = pl.pair ? Cfg<true>::BN : Cfg<false>::BN;
+  const int bn = pl.bn, bm = bn > 64 ? 2 * BM : BM;
   Problem& p = params->pr[i];
   p = Problem();
   p.M = (int)M; p.N = (int)N; p.k_blocks = pl.blocks;
   p.splits = pl.splits; p.kb_per_split = pl.kb_per_split; p.m_pad = pl.m_pad;
   p.m_tiles = (p.M + bm - 1) / bm; p.n_tiles = (p.N + bn - 1) / bn;
+  p.band = M * K >= kLongOperand && p.m_tiles > kBand ? kBand : 0;
   if (pl.tiles * pl.splits > 0x3fffffff) return fail(HAPX_ERR_EXTENT, "block8_matmul: too many tiles");
   params->units[i] = (int)(pl.tiles * pl.splits);
   long long out_rows = M;
@@ -738,11 +790,11 @@ static int describe(const Product& pr, const Plan& pl, void* partial, int i, Map
   if (pr.a)
     if (int e = make_map(&maps->a[i], pr.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, pr.lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
-  if (int e = make_map(&maps->b[i], pr.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, pr.ldb, BK, pl.pair ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
+  if (int e = make_map(&maps->b[i], pr.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, pr.ldb, BK, bn > 64 ? bn / 2 : bn, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return e;
   if (pr.a)
     if (int e = make_scale_map(&maps->sa[i], pr.a_scale, M, p.k_blocks, 1)) return e;
-  if (int e = make_scale_map(&maps->sb[i], pr.b_scale, N, p.k_blocks, pl.pair ? Cfg<true>::B_ATOMS : Cfg<false>::B_ATOMS)) return e;
+  if (int e = make_scale_map(&maps->sb[i], pr.b_scale, N, p.k_blocks, bn > 64 ? 2 : 1)) return e;
   p.tma_store = (reinterpret_cast<uintptr_t>(p.D) & 15u) == 0 && (p.ldd * es) % 16 == 0;
   if (p.tma_store)
     return make_map(&maps->d[i], p.D, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, pl.splits > 1 ? pl.n_pad : N,
@@ -768,9 +820,9 @@ int run(const Product& pr, int sm_count, cudaStream_t stream) {
   Maps maps;
   std::memset(&maps, 0, sizeof(maps));
   if (int e = gemm::error_word(&params.error, nullptr)) return e;
-  const Plan pl = plan_of(pr.m, pr.n, pr.k, sm_count);
+  const Plan pl = plan_of(pr.m, pr.n, pr.k, pr.out_f32, sm_count);
   if (int e = describe(pr, pl, pr.workspace, 0, &maps, &params)) return e;
-  if (int e = pl.pair ? launch<true, void>(maps, params, sm_count, stream) : launch<false, void>(maps, params, sm_count, stream)) return e;
+  if (int e = launch_plan(pl, maps, params, sm_count, stream)) return e;
   return join(pr, pl, pr.workspace, sm_count, stream);
 }
 
@@ -783,17 +835,23 @@ int run_converting(const Product& pr, const void* x, int dtype, long long ldx, i
   Maps maps;
   std::memset(&maps, 0, sizeof(maps));
   if (int e = gemm::error_word(&params.error, nullptr)) return e;
-  const Plan pl = plan_of(pr.m, pr.n, pr.k, sm_count);
+  const Plan pl = plan_of(pr.m, pr.n, pr.k, pr.out_f32, sm_count);
   if (int e = describe(pr, pl, pr.workspace, 0, &maps, &params)) return e;
   params.x = x; params.ldx = ldx; params.K = (int)pr.k;
-  if (int e = dtype == HAPX_BF16 ? launch<false, __nv_bfloat16>(maps, params, sm_count, stream) : launch<false, float>(maps, params, sm_count, stream))
+  if (int e = dtype == HAPX_BF16 ? launch<64, __nv_bfloat16>(maps, params, sm_count, stream) : launch<64, float>(maps, params, sm_count, stream))
     return e;
   return join(pr, pl, pr.workspace, sm_count, stream);
 }
 
 long long workspace_bytes_two(const Product& x, const Product& y, int sm_count) {
-  const PairPlan t = plan_two(x, y, sm_count);
-  return partial_bytes(t.pl[0]) + partial_bytes(t.pl[1]);
+  long long most = 0;
+  for (int f32 = 0; f32 < 2; ++f32) {
+    Product a = x, b = y;
+    a.out_f32 = b.out_f32 = f32;
+    const PairPlan t = plan_two(a, b, sm_count);
+    most = std::max(most, partial_bytes(t.pl[0]) + partial_bytes(t.pl[1]));
+  }
+  return most;
 }
 
 int run_two(const Product& x, const Product& y, int sm_count, cudaStream_t stream) {
@@ -807,7 +865,7 @@ int run_two(const Product& x, const Product& y, int sm_count, cudaStream_t strea
   for (int i = 0; i < 2; ++i)
     if (int e = describe(*pr[i], t.pl[i], partial[i], i == t.first ? 0 : 1, &maps, &params)) return e;
   params.rounds = t.rounds;
-  if (int e = launch<true, void>(maps, params, sm_count, stream)) return e;
+  if (int e = launch_plan(t.pl[0], maps, params, sm_count, stream)) return e;
   for (int i = 0; i < 2; ++i)
     if (int e = join(*pr[i], t.pl[i], partial[i], sm_count, stream)) return e;
   return HAPX_OK;

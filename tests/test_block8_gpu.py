@@ -117,6 +117,19 @@ def test_matmul(out, square, m, n, k):
     assert torch.equal(got, block8.matmul(aq, bq, bias.to(DEV), out))          # the same bits every time
 
 
+@pytest.mark.parametrize("out", [BF, F32])
+@pytest.mark.parametrize("m,n,k", [(2600, 1000, 16384), (2305, 513, 16389), (40000, 300, 1000), (4096, 1024, 8192), (513, 2049, 2000), (8200, 1027, 4096)])
+def test_matmul_of_long_operands_is_exact(out, m, n, k):
+    """Whole numbers up to 6 quantise without error and their sums stay below 2^24: every order of addition gives the same."""
+    from hap_b200 import block8
+    a = torch.randint(-6, 7, (m, k), device=DEV, dtype=torch.int8).float()
+    b = torch.randint(-6, 7, (n, k), device=DEV, dtype=torch.int8).float()
+    bias = torch.randint(-500, 501, (n,), device=DEV).to(out)
+    want = (a.double() @ b.double().t() + bias.double()).to(out)
+    assert float(want.abs().max()) < 2 ** 24
+    assert torch.equal(block8.matmul(block8.quantize(a), block8.quantize(b), bias, out), want)
+
+
 def test_matmul_of_integers_is_exact_and_nan_stays_in_its_row():
     from hap_b200 import block8
     a = torch.randint(-8, 9, (200, 384), generator=gen(0)).float()
