@@ -115,7 +115,10 @@ struct Cfg {
   static constexpr int EPI_WARPS = 4 * PARTS;
   static constexpr int CONVERT_WARPS = CONVERT ? 8 : 0;      // every eighth block each
   static constexpr int THREADS = 64 + 32 * (EPI_WARPS + CONVERT_WARPS);
-  static constexpr int STAGES = BN == 256 ? 5 : PAIR ? 6 : 7;
+  static constexpr int STAGES = BN == 256 ? 5 : PAIR ? 6 : 8;
+  // A wait for a stage tells apart its last use and the one before, no more.  A converting warp that has seen block j - STAGES
+  // consumed knows nothing of the next one: its following turn may come a whole round of the stages later, not more.
+  static_assert(CONVERT_WARPS <= STAGES, "a converting warp's wait would take an older use of the stage for the last");
   static constexpr int B_ATOMS = PAIR ? 2 : 1;               // 192 columns from a multiple of 64 on lie in two groups of 128
   static constexpr unsigned A_BYTES = BM * BK;
   static constexpr unsigned B_BYTES = (PAIR ? BN / 2 : BN) * BK;

@@ -277,6 +277,25 @@ def test_linear8_few_tokens_prepared_weight(dtype, rows, fin, fout):
     assert bool(torch.isnan(y[bad]).all()) and bool(torch.isfinite(y[~bad]).all())
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [3, 4, 7, 32])
+def test_linear8_few_tokens_wide_weight(dtype, rows):
+    """Several tiles per thread block, whose first operand is converted far quicker than the weight arrives: the ring of
+    stages goes round often, and every call gives the same bits."""
+    import hap_b200
+    from hap_b200 import block8
+    x = torch.randint(-6, 7, (rows, 768), device=DEV).to(dtype)
+    w = torch.randint(-6, 7, (33280, 768), device=DEV).float()
+    want = (x.double() @ w.double().t()).to(dtype)
+    w8 = block8.quantize_weight(w)
+    flush = torch.empty(256 << 20, device=DEV, dtype=torch.uint8)
+    with torch.no_grad():
+        for i in range(60):
+            if i % 2:
+                flush.zero_()
+            assert torch.equal(hap_b200.linear8(x, w8), want)
+
+
 def test_linear8_uses_the_same_leaf_twice_and_keeps_its_graph():
     import hap_b200
     x, w, b, g = linear_inputs(60, 96, 96, F32)
