@@ -28,7 +28,9 @@ struct QuantJobs {
 // Two passes over the tile in registers, where the elements stay in their own type (32 registers for bfloat16, three
 // blocks per SM): the maxima of rows and columns, then - once all scales are known - both forms from one unpacking.  The
 // transposed bytes go through shared memory and leave as whole 128-byte rows.  What bounds it is the bytes in flight: a
-// block fetches its next tile into shared memory by one bulk tensor load while it works on and stores the present one.
+// block fetches its next tile into shared memory by one bulk tensor load while it works on and stores the present one; and,
+// close behind, the 18 instructions per element.  bfloat16, 8192 x 33280: 205 us for both forms (5.3 TB/s), 142 for one
+// (5.7); 8192 x 768, where the 384 tiles are one round of the SMs: 7.5 us (3.3 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const __grid_constant__ QuantJobs jobs, const __grid_constant__ CUtensorMap map0,
                                                                                const __grid_constant__ CUtensorMap map1) {
@@ -195,7 +197,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_kernel(c
   }
 }
 
-// out[c] = sum over the row tiles in a fixed order: warp w of 8 takes tiles w, w + 8, ...
+// out[c] = sum over the row tiles in a fixed order: warp w of 8 takes tiles w, w + 8, ...  A launch's length (3 us); where a
+// weight gradient is computed too, its product does this instead.
 template <typename T>
 __global__ void __launch_bounds__(256) colsum_join_kernel(const float* __restrict__ partial, int tiles, long long cols, T* __restrict__ out) {
   __shared__ float s_sum[8][32];
@@ -213,6 +216,7 @@ __global__ void __launch_bounds__(256) colsum_join_kernel(const float* __restric
   out[c] = from_f<T>(s);
 }
 
+// x~ = q s, one element per thread at a time: for inspection and tests, on no training path.
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned char* __restrict__ q, long long ldq, const unsigned char* __restrict__ s,
                                                          T* __restrict__ out, long long rows, long long cols) {
