@@ -882,7 +882,7 @@ using namespace hapx;
 extern "C" {
 
 int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0 || m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00) return 0;
   int n_sm = 0;
   return sm_count(&n_sm) ? 0 : gemm8::workspace_bytes(m, n, k, n_sm);
 }
@@ -890,8 +890,8 @@ int64_t hapx_block8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
 int hapx_block8_matmul(void* d, int out_dtype, const void* a, int64_t lda, const void* a_scale, const void* b, int64_t ldb, const void* b_scale,
                        const void* bias, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, hapx_stream stream) {
   if (out_dtype != HAPX_F32 && out_dtype != HAPX_BF16) return fail(HAPX_ERR_DTYPE, "block8_matmul: the output is float32 or bfloat16");
-  if (m < 0 || n < 0 || k < 1 || m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff)
-    return fail(HAPX_ERR_EXTENT, "block8_matmul: extents must lie below 2^31, the contraction at 1 or above");
+  if (m < 0 || n < 0 || k < 1 || m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00)
+    return fail(HAPX_ERR_EXTENT, "block8_matmul: extents must lie below 2^31 - 256, the contraction at 1 or above");
   if (m == 0 || n == 0) return HAPX_OK;
   if (!d || !a || !a_scale || !b || !b_scale) return fail(HAPX_ERR_ARGUMENT, "block8_matmul: null pointer");
   if (lda % 16 != 0 || ldb % 16 != 0 || lda < k || ldb < k || ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u))

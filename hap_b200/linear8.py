@@ -16,6 +16,7 @@ weight).  A weight that does not change (evaluation, frozen layers) is quantised
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Union
 
 import torch
@@ -25,25 +26,16 @@ from . import block8
 from .block8 import Block8, _CODES, _up
 from .comm import _launch, _on_device, _once
 
-_sizes = {}      # (device, shape, what is asked) -> workspace bytes
-
-
+@functools.lru_cache(maxsize=4096)
 def _forward_workspace(device, m, n, k, prepared, keep_x) -> int:
-    key = (device.index, m, n, k, prepared, keep_x)
-    size = _sizes.get(key)
-    if size is None:
-        with _on_device(device):
-            size = _sizes[key] = N.lib.hapx_linear8_forward_workspace(m, n, k, prepared, keep_x)
-    return size
+    with _on_device(device):
+        return N.lib.hapx_linear8_forward_workspace(m, n, k, prepared, keep_x)
 
 
+@functools.lru_cache(maxsize=4096)
 def _backward_workspace(device, m, n, k, dx, dw, db) -> int:
-    key = (device.index, m, n, k, dx, dw, db)
-    size = _sizes.get(key)
-    if size is None:
-        with _on_device(device):
-            size = _sizes[key] = N.lib.hapx_linear8_backward_workspace(m, n, k, dx, dw, db)
-    return size
+    with _on_device(device):
+        return N.lib.hapx_linear8_backward_workspace(m, n, k, dx, dw, db)
 
 
 def _kept_bytes(rows: int, cols: int):

@@ -8,6 +8,8 @@ torch's own CUDA implementation unchanged.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn.functional as F
 
@@ -153,6 +155,12 @@ def _norm8_save(ctx, x, weight, bias, eps):
     return y
 
 
+@functools.lru_cache(maxsize=4096)
+def _norm8_workspace(device, rows, E) -> int:
+    with _on_device(device):
+        return N.lib.hapx_layer_norm8_backward_workspace(rows, E)
+
+
 def _norm8_backward(ctx, dy, add):
     kept, w = ctx.saved_tensors
     E, device, dtype = dy.shape[-1], dy.device, dy.dtype
@@ -166,18 +174,10 @@ def _norm8_backward(ctx, dy, add):
     saved = kept.data_ptr()
     work = None
     if ctx.need_w or ctx.need_b:
-        key = (device.index, rows, E)
-        size = _work8.get(key)
-        if size is None:
-            with _on_device(device):
-                size = _work8[key] = N.lib.hapx_layer_norm8_backward_workspace(rows, E)
-        work = dy.new_empty(size, dtype=torch.uint8)
+        work = dy.new_empty(_norm8_workspace(device, rows, E), dtype=torch.uint8)
     _launch(device, N.lib.hapx_layer_norm8_backward, saved, pitch, saved + scales_at, dy.data_ptr(), _ptr(w), saved + stats_at,
             saved + stats_at + 4 * rows, _ptr(add), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work), _DTYPES[dtype], rows, E)
     return dx, dw, db, None
-
-
-_work8 = {}      # (device, rows, E) -> workspace bytes of the backward pass
 
 
 class _LayerNorm8(torch.autograd.Function):
