@@ -159,7 +159,15 @@ __device__ __forceinline__ void add_bias(const Problem& p, int n, bool vec, unsi
   }
 }
 
-template <int BN, typename X>
+// JOIN: the output is float32, and the accumulator runs over kChunk blocks at a time; the epilogue warps add the chunks in
+// registers, rounding to nearest.  The tensor cores cut what an addition shifts out, so an accumulator drifts towards zero
+// with every step: a float32 weight gradient over 12232 tokens of uneven size was off by 5e-6 where float32 sums of the
+// library are off by 5e-7, and is by 3e-7 now.  One chunk is added while the next runs (8192 x 8192 x 8192: 400 us without,
+// 426 in chunks of 8, 443 of 4; 8192 x 4096 from 1024: 45 us either way).  A bfloat16 output rounds by a thousand times as
+// much and does not pay for it.
+constexpr int kChunk = 4;
+
+template <int BN, typename X, bool JOIN>
 __global__ void __launch_bounds__(Cfg<BN, !std::is_void<X>::value>::THREADS, 1)
 gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params params) {
   constexpr bool CONVERT = !std::is_void<X>::value;
@@ -287,11 +295,15 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
       const unsigned long long desc_a = make_desc(base, 16u, 1024u), desc_b = make_desc(base + C::A_BYTES, 16u, 1024u);
       Unit u;
       for (int step = 0; ok && next_unit(step, u); ++step) {
-        const unsigned d = tmem_base + (unsigned)(acc * C::BN), shift = (unsigned)(u.n0 >> 5) & 3u;   // B's rows start inside a group of 128
-        unsigned sf = 0;
-        ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), acc_phase ^ 1u));
-        if (!ok) break;
+        const unsigned shift = (unsigned)(u.n0 >> 5) & 3u;   // B's rows start inside a group of 128
+        unsigned sf = 0, d = 0;
         for (int kb = u.kb0; kb < u.kb1; ++kb) {
+          const bool first = kb == u.kb0 || (JOIN && (kb - u.kb0) % kChunk == 0), last = kb + 1 == u.kb1 || (JOIN && (kb + 1 - u.kb0) % kChunk == 0);
+          if (first) {
+            ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), acc_phase ^ 1u));
+            if (!ok) break;
+            d = tmem_base + (unsigned)(acc * C::BN);
+          }
           ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase));
           if (!ok) break;
           tc_fence_after();
@@ -308,19 +320,18 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
             const unsigned long long da = desc_a + (unsigned)(stage * (C::STAGE_BYTES >> 4)), db = desc_b + (unsigned)(stage * (C::STAGE_BYTES >> 4));
             const unsigned idesc = C::IDESC | ((unsigned)(kb & 3) << 4) | ((unsigned)(kb & 3) << 29);
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k) umma8<PAIR>(d, da + 2 * k, db + 2 * k, idesc, sf, sf + 4 + shift, kb != u.kb0 || k != 0);
+            for (int k = 0; k < BK / UMMA_K; ++k) umma8<PAIR>(d, da + 2 * k, db + 2 * k, idesc, sf, sf + 4 + shift, !first || k != 0);
             if (PAIR) umma2_commit_both(empty_bar(stage));
             else umma_commit(empty_bar(stage));
-            if (kb + 1 == u.kb1) {                           // the accumulator is complete
+            if (last) {                                      // the accumulator is complete
               if (PAIR) umma2_commit_both(tfull_bar(acc));
               else umma_commit(tfull_bar(acc));
             }
           }
           __syncwarp();
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+          if (last && ++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
         }
-        if (!ok) break;
-        if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
       }
       if (!ok && lane == 0) atomicCAS(params.error, 0u, 2u);
     }
@@ -429,9 +440,11 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
         asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + n0 * (p.out_f32 ? 4 : 2)));
         if (p.out_f32) asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.bias) + n0 * 4 + 128));
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
-      if (!ok) break;
-      tc_fence_after();
+      if constexpr (!JOIN) {
+        ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
+        if (!ok) break;
+        tc_fence_after();
+      }
       const long long out_row0 = (long long)u.split * p.m_pad + u.m0 + q * 32;
       auto drained = [&] {                                   // this warp has read its part of the accumulator
         tc_fence_before();
@@ -482,7 +495,40 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
         __syncwarp();
       };
       const int n0 = u.n0 + 64 * part;                       // a warp's pieces of 64 columns lie 64 * PARTS apart
-      const unsigned t = tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(acc * C::BN + 64 * part);
+      auto piece = [&] { return tmem_base + ((unsigned)(q * 32) << 16) + (unsigned)(acc * C::BN + 64 * part); };
+      if constexpr (JOIN) {
+        float sum[2][32] = {};
+        for (int kb = u.kb0; kb < u.kb1; kb += kChunk) {
+          ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            unsigned r[32];
+            tmem_ld_32x32(piece() + 32u * h, r);
+            tmem_ld_wait();
+            if (h == 1) drained();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[h][j] += __uint_as_float(r[j]);
+          }
+          if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int n = n0 + 32 * h, width = min(32, p.N - n);
+          if (width <= 0) continue;
+          unsigned r[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(sum[h][j]);
+          if (p.bias) add_bias(p, n, p.bias_vec && width == 32, r);
+          staging_free();
+          stage_row(tile_gen + lane * 128, lane & 7, r);
+          send(std::true_type{}, n, width);
+        }
+        continue;
+      }
+      const unsigned t = piece();
       constexpr int PER = C::PIECES / C::PARTS;
       if (p.out_f32) {
 #pragma unroll 1
@@ -630,10 +676,11 @@ static bool cut(Plan& pl, int splits) {        // false where a range would be e
 // more bytes into shared memory, but its accumulator has no second one, so nothing hides its drain; and 256 columns may
 // divide a width better or worse.  (192 against 256: 4096 x 1024 from 8192 36.4 / 27.2 us, 8192^3 396 / 384,
 // 16384 x 4096 from 1024 65.5 / 62.7; 8192 x 768 from 2304 15.8 / 18.9, 4096 x 4096 from 1024 19.3 / 20.2.)
-// Twice as many bytes of float32 take 0.8 us longer to leave (8192 x 4096 from 1024 with its quantiser: 64.8 us in 256 columns, 59.1 in 192).
+// Twice as many bytes of float32 take 0.8 us longer to leave (8192 x 4096 from 1024 with its quantiser: 64.8 us in 256
+// columns, 59.1 in 192).  Whole float32 outputs, whose accumulators change hands every kChunk blocks, need two.
 static double unit_us(const Plan& pl) {
   const int kb = pl.kb_per_split;
-  return pl.bn == 64 ? 0.15 * kb : pl.bn == 192 ? 0.29 * kb + 0.8 : 0.39 * kb + (pl.f32 || pl.splits > 1 ? 1.95 : 1.15);
+  return pl.bn == 64 ? 0.15 * kb : pl.bn == 192 ? 0.29 * kb + 0.8 : 0.39 * kb + (pl.splits > 1 ? 1.95 : 1.15);
 }
 static double split_us(const Plan& pl) { return pl.splits > 1 ? 3.0 + pl.splits * 8.0 * (double)pl.m_pad * pl.n_pad / 4e6 : 0.0; }
 
@@ -651,7 +698,9 @@ static Plan plan_of(long long M, long long N, long long K, int f32, int sm_count
     return best;
   };
   if (M <= BM) return best_of(64);
-  const Plan a = best_of(192), b = best_of(256);
+  const Plan a = best_of(192);
+  if (f32) return a;
+  const Plan b = best_of(256);
   return cost(b) < cost(a) ? b : a;
 }
 
@@ -681,7 +730,7 @@ static PairPlan plan_two(const Product& x, const Product& y, int sm_count) {
   const int workers = sm_count / 2;
   PairPlan best;
   double best_us = -1.0;
-  for (int bn = 192; bn <= 256; bn += 64) {
+  for (int bn = 192; bn <= (x.out_f32 ? 192 : 256); bn += 64) {
     const Plan whole[2] = {plan_whole(x.m, x.n, x.k, x.out_f32, bn), plan_whole(y.m, y.n, y.k, y.out_f32, bn)};
     for (int cx = 1; cx <= 16; cx = cx < 4 ? cx + 1 : cx * 2) {
       for (int cy = 1; cy <= 16; cy = cy < 4 ? cy + 1 : cy * 2) {
@@ -700,11 +749,11 @@ static PairPlan plan_two(const Product& x, const Product& y, int sm_count) {
 
 static long long partial_bytes(const Plan& pl) { return pl.splits > 1 ? pl.splits * pl.m_pad * pl.n_pad * 4 : 0; }
 
-template <int BN, typename X>
+template <int BN, typename X, bool JOIN>
 static int launch(const Maps& maps, const Params& p, int sm_count, cudaStream_t stream) {
   using C = Cfg<BN, !std::is_void<X>::value>;
   constexpr bool PAIR = C::PAIR;
-  auto kernel = gemm8_kernel<BN, X>;
+  auto kernel = gemm8_kernel<BN, X, JOIN>;
   static int limit_of[64] = {};             // per device: function attributes and occupancy belong to one
   static std::mutex mutex;
   int device = 0;
@@ -742,9 +791,9 @@ static int launch(const Maps& maps, const Params& p, int sm_count, cudaStream_t 
 }
 
 static int launch_plan(const Plan& pl, const Maps& maps, const Params& p, int sm_count, cudaStream_t stream) {
-  if (pl.bn == 64) return launch<64, void>(maps, p, sm_count, stream);
-  if (pl.bn == 192) return launch<192, void>(maps, p, sm_count, stream);
-  return launch<256, void>(maps, p, sm_count, stream);
+  if (pl.bn == 64) return pl.f32 ? launch<64, void, true>(maps, p, sm_count, stream) : launch<64, void, false>(maps, p, sm_count, stream);
+  if (pl.bn == 192) return pl.f32 ? launch<192, void, true>(maps, p, sm_count, stream) : launch<192, void, false>(maps, p, sm_count, stream);
+  return launch<256, void, false>(maps, p, sm_count, stream);
 }
 
 // The scales as (128 words of an atom, group of 128 rows, four blocks).
@@ -841,7 +890,7 @@ int run_converting(const Product& pr, const void* x, int dtype, long long ldx, i
   const Plan pl = plan_of(pr.m, pr.n, pr.k, pr.out_f32, sm_count);
   if (int e = describe(pr, pl, pr.workspace, 0, &maps, &params)) return e;
   params.x = x; params.ldx = ldx; params.K = (int)pr.k;
-  if (int e = dtype == HAPX_BF16 ? launch<64, __nv_bfloat16>(maps, params, sm_count, stream) : launch<64, float>(maps, params, sm_count, stream))
+  if (int e = dtype == HAPX_BF16 ? launch<64, __nv_bfloat16, false>(maps, params, sm_count, stream) : launch<64, float, true>(maps, params, sm_count, stream))
     return e;
   return join(pr, pl, pr.workspace, sm_count, stream);
 }

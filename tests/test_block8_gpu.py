@@ -130,6 +130,31 @@ def test_matmul_of_long_operands_is_exact(out, m, n, k):
     assert torch.equal(block8.matmul(block8.quantize(a), block8.quantize(b), bias, out), want)
 
 
+@pytest.mark.parametrize("m", [100, 300])
+def test_long_float32_sums_do_not_drift(m):
+    """Positive terms, so that every step that cuts instead of rounding errs in the same direction.  Accumulators run over
+    512 terms (16 steps of 32, each off by 2^-22 of the sum at most: one cut where the terms are aligned, one of the
+    result); their sums are added rounding to nearest, 2^-24 each."""
+    from hap_b200 import block8
+    k = 16384
+    a, b = (block8.quantize(torch.rand(rows, k, generator=gen(rows)).to(DEV) + 0.1) for rows in (m, 48))
+    want = a.dequantize().double() @ b.dequantize().double().t()
+    got = block8.matmul(a, b, None, F32).double()
+    assert float(((got - want).abs() / want).max()) <= 16 * 2.0 ** -22 + k / 512 * 2.0 ** -24
+
+
+def test_float32_weight_gradient_over_many_tokens():
+    """The same bound through linear8's backward pass."""
+    import hap_b200
+    from hap_b200 import block8
+    t = 16384
+    x, g = (torch.rand(t, n, generator=gen(n)).to(DEV) + 0.1 for n in (64, 300))
+    w = leaf(torch.rand(300, 64, generator=gen(1)))
+    (dw,) = torch.autograd.grad(hap_b200.linear8(x, w), w, g)
+    want = block8.quantize(g, False, True).dequantize().double() @ block8.quantize(x, False, True).dequantize().double().t()
+    assert float(((dw.double() - want).abs() / want).max()) <= 16 * 2.0 ** -22 + t / 512 * 2.0 ** -24
+
+
 def test_matmul_of_integers_is_exact_and_nan_stays_in_its_row():
     from hap_b200 import block8
     a = torch.randint(-8, 9, (200, 384), generator=gen(0)).float()
