@@ -17,8 +17,8 @@
 // 256 x 256 with one: unit_us chooses.  Single kernel (M <= 128): 128 x 64 tiles, so that a narrow product still spreads
 // over the SMs.
 //
-// 8192 x 8192 x 8192: 380 us = 2.9 PFLOP/s (the library's bfloat16 product 690 us); without its loads 4.1 PFLOP/s: bound by
-// what goes into shared memory and by power.  8192 x 33280 from 768: 205 us, of which 138 are what filling the 545 MB of
+// 8192 x 8192 x 8192: 380 us = 2.9 PFLOP/s (the library's bfloat16 product 690 us), the tensor pipe 90 % of the time active: bound
+// by it and by the clock that power leaves.  8192 x 33280 from 768: 205 us, of which 138 are what filling the 545 MB of
 // output takes.  8192 x 768 -> 2304 and back: 16, 15 and 20 us (forward, to the input, to the weight).
 //
 // Single kernel with X (a float type): the first operand comes as it is, bfloat16 or float32, and eight more warps make its
