@@ -51,7 +51,7 @@ def _block8(rows, cols):
 
 def test_scale_matrix_decodes_the_order_of_the_tensor_cores():
     b = _block8(300, 700)                                               # 3 groups of rows, 6 blocks of columns in 2 groups of 4
-    assert b.scales.numel() == N.lib.hapx_block8_scale_bytes(300, 700) == 2 * 3 * 512 and b.nbytes == 300 * 704 + 3072
+    assert b.scales.numel() == N.lib.hapx_block8_scale_bytes(300, 700) == 2 * 3 * 512 and b.nbytes == 300 * 704 + 6 * 512
     for r, kb in ((0, 0), (31, 1), (32, 2), (127, 3), (128, 4), (299, 5), (170, 3)):
         b.scales.fill_(127)
         b.scales[((kb // 4) * 3 + r // 128) * 512 + (r % 32) * 16 + (r // 32 % 4) * 4 + kb % 4] = 130
