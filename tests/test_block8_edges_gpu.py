@@ -1,0 +1,41 @@
+"""The 8-bit operators at the ends of what they accept: the largest extents, scales far apart, values near the largest
+float32 number, NaN and infinities, forward-mode differentiation, operands that do not fit together; and whole steps
+replayed from CUDA graphs."""
+import pytest
+import torch
+
+from tests.test_block8_gpu import BF, DEV, F32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """A kernel whose bounded wait ran out raises a flag; its output may look whole all the same."""
+    import hap_b200
+    yield
+    hap_b200.linear_ops.gemm_status()
+
+
+@pytest.mark.parametrize("rows", [1, 2])
+def test_prepared_weight_with_the_most_output_features(rows):
+    """out_features 2^31 - 256, where a row number plus the grid's stride is above 2^31 - 1.  in_features 1: y = x w."""
+    import hap_b200
+    from hap_b200 import block8
+    n = 2 ** 31 - 256
+    last = torch.arange(1, 9, dtype=F32)
+    raw = torch.zeros(n, 16, dtype=torch.uint8, device=DEV)                                               # 34 GB
+    raw[:, 0] = 0x38                                                                                      # 1.0
+    raw[-8:, 0] = last.to(torch.float8_e4m3fn).view(torch.uint8).to(DEV)
+    raw[2 ** 30, 0] = 0xC4                                                                                # -3.0
+    scales = torch.full((-(-n // 128) * 512,), 127, dtype=torch.uint8, device=DEV)                        # 2^0 everywhere
+    x = torch.tensor([[2.0], [-4.0]], dtype=BF, device=DEV)[:rows]
+    y = hap_b200.linear8(x, block8.Block8(raw.view(torch.float8_e4m3fn), scales, n, 1))
+    del raw, scales
+    assert y.shape == (rows, n)
+    for r in range(rows):
+        xr = float(x[r, 0])
+        assert torch.equal(y[r, -8:].float().cpu(), xr * last) and float(y[r, 2 ** 30]) == -3.0 * xr
+        y[r, -8:] = y[r, 2 ** 30] = xr
+        low, high = torch.aminmax(y[r])
+        assert float(low) == float(high) == xr
