@@ -31,6 +31,10 @@ def _blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
 
 
+def _scale_bytes(rows: int, cols: int) -> int:
+    return _up(cols, 512) // 512 * _blocks(rows) * 512
+
+
 class Block8:
     """``rows x cols`` e4m3 values (``values``, float8_e4m3fn, rows padded to a multiple of 16 bytes) and one
     power-of-two scale per 128 columns of a row (``scales``, bytes in the order the tensor cores read them;
@@ -40,6 +44,19 @@ class Block8:
     __slots__ = ("values", "scales", "rows", "cols", "transposed")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, transposed: Optional["Block8"] = None):
+        # the kernels take extents and pitch from here: what does not hold them is refused, not read past its end
+        if rows < 0 or cols < 1:
+            raise ValueError(f"Block8: {rows} x {cols} is no matrix")
+        if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8:
+            raise TypeError(f"Block8: values are float8_e4m3fn and scales uint8, got {values.dtype} and {scales.dtype}")
+        if values.dim() != 2 or values.shape[0] != rows or values.shape[1] < cols or values.shape[1] % 16 or not values.is_contiguous():
+            raise ValueError(f"Block8: the values of {rows} x {cols} are {rows} rows of a multiple of 16 bytes, contiguous; got {tuple(values.shape)}")
+        if scales.numel() != _scale_bytes(rows, cols) or not scales.is_contiguous():
+            raise ValueError(f"Block8: the scales of {rows} x {cols} are {_scale_bytes(rows, cols)} contiguous bytes, got {tuple(scales.shape)}")
+        if scales.device != values.device:
+            raise ValueError(f"Block8: values are on {values.device}, scales on {scales.device}")
+        if transposed is not None and (transposed.rows != cols or transposed.cols != rows or transposed.device != values.device):
+            raise ValueError(f"Block8: {transposed} is not the transposed form of {rows} x {cols} on {values.device}")
         self.values, self.scales, self.rows, self.cols, self.transposed = values, scales, rows, cols, transposed
 
     @property
@@ -89,10 +106,10 @@ def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     return x
 
 
-def _empty(rows: int, cols: int, device) -> Block8:
+def _empty(rows: int, cols: int, device, transposed: Optional[Block8] = None) -> Block8:
     values = torch.empty((rows, _up(cols, 16)), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty(_up(cols, 512) // 512 * _blocks(rows) * 512, dtype=torch.uint8, device=device)
-    return Block8(values, scales, rows, cols)
+    scales = torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device)
+    return Block8(values, scales, rows, cols, transposed)
 
 
 def _run(x: torch.Tensor, square: bool, q: Optional[Block8], qt: Optional[Block8], colsum: Optional[torch.Tensor] = None) -> None:
@@ -128,10 +145,9 @@ def quantize_weight(w: torch.Tensor, transposed: bool = False) -> Block8:
     w = _matrix(w, "block8.quantize_weight")
     if w.shape[0] < 1:
         raise ValueError("block8.quantize_weight: rows of at least one element are expected")
-    q = _empty(w.shape[0], w.shape[1], w.device)
     qt = _empty(w.shape[1], w.shape[0], w.device) if transposed else None
+    q = _empty(w.shape[0], w.shape[1], w.device, qt)
     _run(w, True, q, qt)
-    q.transposed = qt
     return q
 
 

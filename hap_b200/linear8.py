@@ -22,7 +22,6 @@ from typing import Optional, Union
 import torch
 
 from . import _native as N
-from . import block8
 from .block8 import Block8, _CODES, _up
 from .comm import _launch, _on_device, _once
 
@@ -127,6 +126,21 @@ class _Linear8(torch.autograd.Function):
         return dx, dw, db, None
 
 
+def _check_prepared(w8: Block8, transposed: bool) -> None:
+    """The kernels take a prepared weight's pitch as its row rounded up to 16 bytes, as ``quantize_weight`` makes it."""
+    forms = [w8]
+    if transposed:
+        t = w8.transposed
+        if t is None:
+            raise ValueError("linear8: the input's gradient needs the weight's transposed form: block8.quantize_weight(w, transposed=True)")
+        if t.rows != w8.cols or t.cols != w8.rows:
+            raise ValueError(f"linear8: {t} is not the transposed form of {w8}")
+        forms.append(t)
+    for q in forms:
+        if q.values.shape[1] != _up(q.cols, 16):
+            raise ValueError(f"linear8: the weight's rows lie {q.values.shape[1]} bytes apart, {_up(q.cols, 16)} are expected")
+
+
 def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``F.linear(input, weight, bias)`` on CUDA bfloat16 or float32 tensors of any extents, with the products in 8-bit
     floating point (see the module).  ``weight``: a tensor of the input's type, or a :class:`hap_b200.block8.Block8`
@@ -142,8 +156,7 @@ def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Opti
     prepared = None
     if isinstance(weight, Block8):
         prepared, weight = weight, None
-        if prepared.transposed is None and input.requires_grad and torch.is_grad_enabled():
-            raise ValueError("linear8: the input's gradient needs the weight's transposed form: block8.quantize_weight(w, transposed=True)")
+        _check_prepared(prepared, input.requires_grad and torch.is_grad_enabled())
         fout, fin, device = prepared.rows, prepared.cols, prepared.device
     else:
         if weight.dim() != 2 or weight.shape[0] < 1:

@@ -1,0 +1,38 @@
+"""The 8-bit operators without a GPU: operands that do not fit together, derivatives that are not there."""
+import pytest
+import torch
+
+from hap_b200 import block8
+from tests.test_block8 import _block8
+
+
+def test_blocks_that_do_not_hold_their_matrix_are_refused():
+    values, scales = torch.zeros(40, 48, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.full((512,), 127, dtype=torch.uint8)
+    good = block8.Block8(values, scales, 40, 40)
+    assert block8.Block8(values, scales, 40, 33).shape == (40, 33)                          # a pitch above the row's need
+    for args, err in (((values, scales, 41, 40), ValueError), ((values, scales, 40, 49), ValueError), ((values, scales, 40, 0), ValueError),
+                      ((values, scales, -1, 40), ValueError), ((values[:, :40], scales, 40, 40), ValueError), ((values[0], scales, 1, 40), ValueError),
+                      ((values.view(torch.uint8)[:, :40].contiguous().view(torch.float8_e4m3fn), scales, 40, 40), ValueError),      # pitch not of 16 bytes
+                      ((values.view(torch.uint8), scales, 40, 40), TypeError), ((values, scales.float(), 40, 40), TypeError),
+                      ((values, scales[:511], 40, 40), ValueError), ((values, scales.repeat(2)[::2], 40, 40), ValueError),
+                      ((values, scales.to("meta"), 40, 40), ValueError), ((values, scales, 40, 40, _block8(40, 41)), ValueError)):
+        with pytest.raises(err, match="Block8"):
+            block8.Block8(*args)
+    assert block8.Block8(values, scales, 40, 40, good).transposed is good
+
+
+def test_prepared_weights_of_another_pitch_are_refused():
+    from hap_b200.linear8 import _check_prepared
+    wide = block8.Block8(torch.zeros(40, 64, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.full((512,), 127, dtype=torch.uint8), 40, 40)
+    square = _block8(40, 40)
+    _check_prepared(square, False)
+    with pytest.raises(ValueError, match="64 bytes apart, 48"):
+        _check_prepared(wide, False)
+    with pytest.raises(ValueError, match="transposed form"):
+        _check_prepared(square, True)
+    with pytest.raises(ValueError, match="64 bytes apart, 48"):
+        _check_prepared(block8.Block8(square.values, square.scales, 40, 40, wide), True)
+    odd = _block8(40, 40)
+    odd.transposed = _block8(40, 41)
+    with pytest.raises(ValueError, match="not the transposed form"):
+        _check_prepared(odd, True)
