@@ -22,6 +22,7 @@ import os
 from typing import List, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -64,6 +65,14 @@ def _launch(device, entry, *args) -> None:
             code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     if code:
         N.check(code)
+
+
+def _differentiated(*tensors) -> bool:
+    """Whether an operator has to go through its autograd function: a gradient is asked for, or forward-mode
+    differentiation is on - its tensors carry tangents without ``requires_grad``, and the function refuses them."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _once(backward):

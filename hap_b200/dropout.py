@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .comm import _launch, _on_device, _once, _stream
+from .comm import _differentiated, _launch, _on_device, _once, _stream
 
 _next_call_id = 0
 
@@ -223,7 +223,7 @@ def act_dropout8(x: torch.Tensor, act: str, p: float, training: bool = True) -> 
         raise ValueError(f"act_dropout8: the activation is \"relu\" or \"gelu\", got {act!r}")
     p = float(p) if training else 0.0
     call_id = new_call_id() if p > 0.0 else 0
-    if x.requires_grad and torch.is_grad_enabled():
+    if _differentiated(x):
         return _ActDropout8.apply(x, _ACTS[act], p, call_id)
     return _act8(x, _ACTS[act], p, call_id, False)[0]
 

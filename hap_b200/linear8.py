@@ -23,7 +23,8 @@ import torch
 
 from . import _native as N
 from .block8 import Block8, _CODES, _up
-from .comm import _launch, _on_device, _once
+from .comm import _differentiated, _launch, _on_device, _once
+
 
 @functools.lru_cache(maxsize=4096)
 def _forward_workspace(device, m, n, k, prepared, keep_x) -> int:
@@ -173,7 +174,6 @@ def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Opti
             raise TypeError(f"linear8: mixed operand dtypes {dtype} and {bias.dtype}")
         if bias.shape != (fout,) or bias.device != device:
             raise ValueError(f"linear8: the bias must be ({fout},) on {device}, got {tuple(bias.shape)} on {bias.device}")
-    if torch.is_grad_enabled() and (input.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _differentiated(input, weight, bias):
         return _Linear8.apply(input, weight, bias, prepared)
     return _forward(input, weight, bias, prepared, False, False)[0]

@@ -14,7 +14,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native as N
-from .comm import _launch, _on_device, _once
+from .comm import _differentiated, _launch, _on_device, _once
 
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16}
 
@@ -205,10 +205,6 @@ class _LayerNormFork8(torch.autograd.Function):
         return _norm8_backward(ctx, dy, d_residual)
 
 
-def _wants_grad(x, w, b) -> bool:
-    return torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad) or (b is not None and b.requires_grad))
-
-
 def _check8(what, input, shape, weight, bias):
     if not input.is_cuda:
         raise RuntimeError(f"{what}: hap_b200 has no CPU path; tensor is on {input.device}")
@@ -228,7 +224,7 @@ def layer_norm8(input: torch.Tensor, normalized_shape, weight=None, bias=None, e
     statistics of the input itself."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     _check8("layer_norm8", input, shape, weight, bias)
-    if _wants_grad(input, weight, bias):
+    if _differentiated(input, weight, bias):
         return _LayerNorm8.apply(input, weight, bias, eps)
     return _norm8_forward(input, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), eps, False)[0]
 
@@ -238,6 +234,6 @@ def layer_norm_fork8(input: torch.Tensor, normalized_shape, weight=None, bias=No
     gradient added inside the normalisation's backward kernel."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     _check8("layer_norm_fork8", input, shape, weight, bias)
-    if _wants_grad(input, weight, bias):
+    if _differentiated(input, weight, bias):
         return _LayerNormFork8.apply(input, weight, bias, eps)
     return input, layer_norm8(input, shape, weight, bias, eps)

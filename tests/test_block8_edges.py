@@ -1,4 +1,6 @@
 """The 8-bit operators without a GPU: operands that do not fit together, derivatives that are not there."""
+import sys
+
 import pytest
 import torch
 
@@ -36,3 +38,39 @@ def test_prepared_weights_of_another_pitch_are_refused():
     odd.transposed = _block8(40, 41)
     with pytest.raises(ValueError, match="not the transposed form"):
         _check_prepared(odd, True)
+
+
+class _OnGpu(torch.Tensor):
+    """A host tensor that passes for one on the GPU, for what happens before any launch."""
+    is_cuda = True
+
+
+def _operators(monkeypatch):
+    """The four operators with their launches left out, as functions of one input and one parameter vector."""
+    from hap_b200 import dropout, norm
+    modules = [sys.modules[f"hap_b200.{m}"] for m in ("linear8", "dropout", "norm")]
+    for m in modules:
+        monkeypatch.setattr(m, "_launch", lambda *args: None)
+    monkeypatch.setattr(modules[0], "_forward_workspace", lambda *args: 0)
+    w, w8 = torch.ones(4, 8).as_subclass(_OnGpu), _block8(4, 8)
+    linear8 = modules[0].linear8
+    return {"linear8": lambda x, v: linear8(x, w, v[:4]), "linear8 of a prepared weight": lambda x, v: linear8(x, w8, v[:4]),
+            "act_dropout8": lambda x, v: dropout.act_dropout8(x * v, "gelu", 0.0), "layer_norm8": lambda x, v: norm.layer_norm8(x, 8, v),
+            "layer_norm_fork8": lambda x, v: norm.layer_norm_fork8(x, 8, v)}
+
+
+@pytest.mark.parametrize("which", ["linear8", "linear8 of a prepared weight", "act_dropout8", "layer_norm8", "layer_norm_fork8"])
+def test_tangents_are_refused(monkeypatch, which):
+    """Forward-mode differentiation: a dual tensor has requires_grad False; a result without a tangent would read as a zero
+    derivative."""
+    from torch.autograd import forward_ad
+    f = _operators(monkeypatch)[which]
+    x, v = torch.ones(2, 8).as_subclass(_OnGpu), torch.ones(8).as_subclass(_OnGpu)
+    f(x, v)
+    with forward_ad.dual_level():
+        f(x, v)                                                    # no tangent, nothing to refuse
+        for args in ((forward_ad.make_dual(x, x), v), (x, forward_ad.make_dual(v, v))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="jvp"):
+                    f(*args)
+    f(x, v)
