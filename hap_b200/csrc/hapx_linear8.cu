@@ -56,10 +56,9 @@ __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long
   __syncthreads();
   // ROWS rows of w at a time: their loads in flight together, x read from shared memory once for all of them
   const long long groups = ((long long)N + kBlock - 1) / kBlock;
-  // (counted in groups of ROWS: N may come within 256 of 2^31, where a row number plus the stride leaves 32 bits)
-  const int row_groups = (N + ROWS - 1) / ROWS;
-  for (int group = blockIdx.x * 8 + warp; group < row_groups; group += gridDim.x * 8) {
-    const int n0 = group * ROWS;
+  // (unsigned: N may come within 256 of 2^31, where a row number plus the stride leaves 31 bits)
+  for (unsigned first = (blockIdx.x * 8 + warp) * ROWS; first < (unsigned)N; first += gridDim.x * 8 * ROWS) {
+    const int n0 = (int)first;
     float acc[ROWS][MT];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
