@@ -28,6 +28,9 @@ constexpr int kThinElements = 24 * 1024;    // tokens x in_features that fit sha
 // warp multiplies ROWS rows of w, whose loads are in flight together, with all tokens from registers; the values multiplied
 // are those of the other path.  One token, 768 -> 2304: 3.5 us, 768 -> 33280: 10.8 us = 2.4 TB/s (of L2), where its blocks are
 // too many for one round of the SMs.
+// A sum of 16 products of e4m3 numbers is 0 or lies in [2^-18, 2^22): with a weight's scale in [2^-108, 2^105] it stays a
+// normal number, and the token's scale then rounds it once at most.
+constexpr int kNearLow = 127 - 108, kNearHigh = 127 + 105;
 // MT: tokens, rounded up to a power of two.
 template <typename T, int MT, int ROWS>
 __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long long ldx, const unsigned char* __restrict__ w, long long ldw,
@@ -36,7 +39,7 @@ __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long
   extern __shared__ float4 s_mem[];
   const int kpad = (K + kBlock - 1) / kBlock * kBlock, blocks = kpad / kBlock;
   float* s_x = reinterpret_cast<float*>(s_mem);          // [token][kpad] e4m3 values, unscaled
-  float* s_s = s_x + (long long)M * kpad;                // [token][block] scales
+  int* s_e = reinterpret_cast<int*>(s_x + (long long)M * kpad);      // [token][block] exponents of the scales
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool vec = (ldx & 3) == 0 && (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
   for (int i = warp; i < M * blocks; i += 8) {
@@ -51,7 +54,7 @@ __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long
     const unsigned q = pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
     const float2 lo = unpack2(q & 0xffffu), hi = unpack2(q >> 16);
     *reinterpret_cast<float4*>(s_x + (long long)m * kpad + k) = make_float4(lo.x, lo.y, hi.x, hi.y);
-    if (lane == 0) s_s[m * blocks + kb] = pow2(e);
+    if (lane == 0) s_e[m * blocks + kb] = e;
   }
   __syncthreads();
   // ROWS rows of w at a time: their loads in flight together, x read from shared memory once for all of them
@@ -74,6 +77,9 @@ __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long
         raw[r] = __ldg(reinterpret_cast<const uint4*>(w + (long long)n * ldw + k));
         e[r] = ws[scale_at(n, kb, groups)];
       }
+      bool far = false;                                  // a scale that may carry a sum of 16 products out of float32 by itself
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) far |= (unsigned)(e[r] - kNearLow) > (unsigned)(kNearHigh - kNearLow);
       float part[ROWS][MT];
 #pragma unroll
       for (int r = 0; r < ROWS; ++r)
@@ -97,9 +103,17 @@ __global__ void __launch_bounds__(256) thin_kernel(const T* __restrict__ x, long
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const float sx = s_s[min(m, M - 1) * blocks + kb];
+        const int ex = s_e[min(m, M - 1) * blocks + kb];
+        if (!far) {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) acc[r][m] = fmaf(part[r][m] * pow2(e[r] - 127), sx, acc[r][m]);
+          for (int r = 0; r < ROWS; ++r) acc[r][m] = fmaf(part[r][m] * pow2(e[r] - 127), pow2(ex), acc[r][m]);
+        } else {                                         // rare: both scales as one power of two, in halves that are normal numbers
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            const int both = e[r] - 127 + ex, half = both >> 1;
+            acc[r][m] = fmaf(part[r][m] * pow2(half), pow2(both - half), acc[r][m]);
+          }
+        }
       }
     }
 #pragma unroll

@@ -4,7 +4,8 @@ replayed from CUDA graphs."""
 import pytest
 import torch
 
-from tests.test_block8_gpu import BF, DEV, F32
+from oracle import block8_math as B
+from tests.test_block8_gpu import BF, DEV, F32, close, gen, sum_slack
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,18 @@ def test_prepared_weight_with_the_most_output_features(rows):
         y[r, -8:] = y[r, 2 ** 30] = xr
         low, high = torch.aminmax(y[r])
         assert float(low) == float(high) == xr
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 33, 200])
+@pytest.mark.parametrize("ex,ew", [(-120, 120), (115, -110), (-118, 125), (100, -120), (-60, -60), (10, 100)])
+def test_scales_far_apart(rows, ex, ew):
+    """Either operand's scale alone takes the sums out of float32, both together do not: every path by which tokens reach a
+    prepared weight multiplies them as one power of two."""
+    import hap_b200
+    from hap_b200 import block8
+    k, n = 300, 40
+    x, w = (torch.randint(-448, 449, shape, generator=gen(sum(shape))).double() / 64 for shape in ((rows, k), (n, k)))
+    x, w = (x * 2.0 ** ex).float(), (w * 2.0 ** ew).float()                    # exact: 10 bits, normal numbers
+    xv, wv = B.fast_rows(x), B.quantize(w, square=True)[0]
+    y = hap_b200.linear8(x.to(DEV), block8.quantize_weight(w.to(DEV)))
+    close(y, xv @ wv.t(), sum_slack(xv.abs() @ wv.abs().t(), k))
