@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(256) act_forward_kernel(const T* __restrict__ 
   for (; piece < pieces; piece += stride) work(piece, std::false_type{});
 }
 
-// The same split and the same look-ahead; reads the incoming gradient and the 8-bit input (or the bit).
+// The same split and the same look-ahead; reads the incoming gradient and the 8-bit input (or the bit).  A scale of 2^120
+// (inputs above 2^127) is taken as 2^119: 256 * 2^120 is no float32 number, and the slope is 0 or 1 at either.
 template <typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__ dy, const unsigned char* __restrict__ saved,
                                                            const float* __restrict__ scales, T* __restrict__ dx, long long n,
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
       next_s[u] = 0.f;
       if (valid > 0) {
         if (ACT == ACT_RELU) next_w[u].x = sp[32 * u];
-        else { next_w[u] = *reinterpret_cast<const uint2*>(sp + 256 * u); next_s[u] = cp[2 * u]; }
+        else { next_w[u] = *reinterpret_cast<const uint2*>(sp + 256 * u); next_s[u] = fminf(cp[2 * u], 0x1p119f); }
       }
     }
   };

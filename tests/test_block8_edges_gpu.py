@@ -55,3 +55,15 @@ def test_scales_far_apart(rows, ex, ew):
     xv, wv = B.fast_rows(x), B.quantize(w, square=True)[0]
     y = hap_b200.linear8(x.to(DEV), block8.quantize_weight(w.to(DEV)))
     close(y, xv @ wv.t(), sum_slack(xv.abs() @ wv.abs().t(), k))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gelu_gradient_of_the_largest_numbers(dtype):
+    """From 248 * 2^120 on the kept value is 256 * 2^120, which float32 does not hold; the slope there is 1 (or 0) all the same."""
+    from hap_b200 import dropout as D
+    x = torch.tensor([3.2e38, 3.3e38, 3.38e38, torch.finfo(dtype).max, 1.0, 0.0, 3e37, 2.0 ** 111]).to(dtype).repeat(20)
+    for sign in (1.0, -1.0):
+        xg = (sign * x).to(DEV).requires_grad_(True)
+        g = torch.full_like(x, 0.75)
+        D.act_dropout8(xg, "gelu", 0.0).backward(g.to(DEV))
+        close(xg.grad, 0.75 * B.gelu_slope(B.runs(sign * x)), torch.full(x.shape, 2.0 ** -20, dtype=torch.float64))
