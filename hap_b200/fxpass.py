@@ -268,6 +268,35 @@ def fuse_residual_norm(graph: torch.fx.Graph) -> int:
     return changed
 
 
+def _known_dtype(value):
+    """The type of a node's value where the graph tells it, else None."""
+    if not isinstance(value, torch.fx.Node):
+        return getattr(value, "dtype", None)
+    for key in ("val", "tensor_meta"):
+        dtype = getattr(value.meta.get(key), "dtype", None)
+        if dtype is not None:
+            return dtype
+    if value.op == "get_attr" and value.graph.owning_module is not None:
+        found = value.graph.owning_module
+        for part in value.target.split("."):
+            found = getattr(found, part, None)
+        return getattr(found, "dtype", None)
+    return None
+
+
+def _norm8_takes(node) -> bool:
+    """Whether a layer_norm node is one for ``layer_norm8``, as far as the graph tells."""
+    names = ("input", "normalized_shape", "weight", "bias")
+    args = dict(zip(names, node.args), **{k: v for k, v in node.kwargs.items() if k in names})
+    shape = args.get("normalized_shape")
+    if isinstance(shape, (tuple, list)) and len(shape) == 1:
+        (shape,) = shape
+    if not isinstance(shape, int) or not 1 <= shape <= 1 << 20:
+        return False
+    known = {_known_dtype(args.get(k)) for k in ("input", "weight", "bias")} - {None}
+    return len(known) <= 1 and known <= {torch.float32, torch.bfloat16}
+
+
 def use_block8(graph: torch.fx.Graph, products: bool = True, saved: bool = True, skip=None) -> Dict[str, int]:
     """Move a program onto the 8-bit operators; rewrites ``graph`` in place and returns how many nodes of each kind
     were changed.  Run it last, after the passes that fuse nodes.
@@ -277,6 +306,11 @@ def use_block8(graph: torch.fx.Graph, products: bool = True, saved: bool = True,
       inputs kept for the backward pass in 8 bits;
     * ``saved``: ``act_dropout`` -> :func:`hap_b200.dropout.act_dropout8`, ``layer_norm`` / ``layer_norm_fork`` ->
       :func:`hap_b200.norm.layer_norm8` / ``layer_norm_fork8``: the same forward results, inputs kept in 8 bits.
+
+    Nodes that the 8-bit form does not take and ``layer_norm`` hands to torch stay as they are and are not counted: a
+    normalised shape of several dimensions, of more than 2^20 elements or not known before the program runs, and types
+    other than float32 and bfloat16 as far as the graph tells them (``node.meta`` of a shape propagation, parameters of
+    the graph's module).
 
     ``skip(node)``: true for a node to leave as it is (a vocabulary projection, say).  Unlike the other passes this
     one changes what the program computes: by the rounding of the products' operands and of the kept inputs."""
@@ -296,6 +330,8 @@ def use_block8(graph: torch.fx.Graph, products: bool = True, saved: bool = True,
             continue
         for old, new in moves:
             if _is(node.target, old):
+                if _is(old, layer_norm, layer_norm_fork) and not _norm8_takes(node):
+                    break
                 node.target = new
                 changed[old.__name__] += 1
                 break

@@ -74,3 +74,30 @@ def test_tangents_are_refused(monkeypatch, which):
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="jvp"):
                     f(*args)
     f(x, v)
+
+
+def test_use_block8_leaves_norms_that_layer_norm_hands_to_torch():
+    from hap_b200 import fxpass
+    from hap_b200.norm import layer_norm, layer_norm8, layer_norm_fork, layer_norm_fork8
+    root = torch.nn.Module()
+    for name, dtype in (("p16", torch.float16), ("p64", torch.float64), ("pb16", torch.bfloat16), ("p32", torch.float32)):
+        root.register_parameter(name, torch.nn.Parameter(torch.ones(8, dtype=dtype)))
+    graph = torch.fx.Graph(root)
+    x, n = graph.placeholder("x"), graph.placeholder("n")
+    p = {name: graph.get_attr(name) for name, _ in root.named_parameters()}
+    typed = graph.call_function(torch.relu, (x,))
+    typed.meta["val"] = torch.empty(2, 8, dtype=torch.float16)
+    stay = [graph.call_function(layer_norm, (x, (4, 8))), graph.call_function(layer_norm, (x, [4, 8], None, None)),
+            graph.call_function(layer_norm_fork, (x,), {"normalized_shape": (4, 8)}), graph.call_function(layer_norm, (x, (1 << 20) + 1)),
+            graph.call_function(layer_norm, (x, ())), graph.call_function(layer_norm, (x, (0,))), graph.call_function(layer_norm, (x, n)),
+            graph.call_function(layer_norm, (x, (n,))), graph.call_function(layer_norm, (x, (8,), p["p16"])),
+            graph.call_function(layer_norm, (x, (8,)), {"bias": p["p64"]}), graph.call_function(layer_norm, (x, (8,), p["p32"], p["pb16"])),
+            graph.call_function(layer_norm, (typed, (8,))), graph.call_function(layer_norm_fork, (typed, 8))]
+    move = [graph.call_function(layer_norm, (x, (8,))), graph.call_function(layer_norm, (x, 8, p["pb16"], p["pb16"])),
+            graph.call_function(layer_norm, (x,), {"normalized_shape": [1 << 20], "weight": p["p32"], "eps": 1e-6}),
+            graph.call_function(layer_norm_fork, (x, torch.Size([8]), p["p32"]))]
+    graph.output(tuple(stay + move))
+    before = [node.target for node in stay]
+    assert fxpass.use_block8(graph, products=False) == {"act_dropout": 0, "layer_norm": 3, "layer_norm_fork": 1}
+    assert [node.target for node in stay] == before
+    assert [node.target for node in move] == [layer_norm8, layer_norm8, layer_norm8, layer_norm_fork8]
