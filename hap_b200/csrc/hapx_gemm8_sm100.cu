@@ -410,7 +410,7 @@ gemm8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok && lane == 0) atomicCAS(params.error, 0u, 4u);
+      if (!ok && lane == 0) atomicCAS(params.error, 0u, 5u);
     }
   } else {
     // ---------------- epilogue: 32 rows x 64 columns of the tile per warp ----------------

@@ -1221,7 +1221,7 @@ int hapx_gemm_status(void) {
   if (code != 0) {
     HAPX_CUDA(cudaMemset(dev->error, 0, sizeof(unsigned)));
     return fail(HAPX_ERR_PEER_TIMEOUT, "a GEMM kernel gave up waiting on a barrier (role " + std::to_string(code) +
-                                           ": 1 = TMA producer, 2 = MMA issuer, 3 = epilogue, 4 = block quantiser)");
+                                           ": 1 = TMA producer, 2 = MMA issuer, 3 = epilogue, 4 = block quantiser, 5 = converting warps of the 8-bit product)");
   }
   return HAPX_OK;
 }

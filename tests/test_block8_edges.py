@@ -101,3 +101,16 @@ def test_use_block8_leaves_norms_that_layer_norm_hands_to_torch():
     assert fxpass.use_block8(graph, products=False) == {"act_dropout": 0, "layer_norm": 3, "layer_norm_fork": 1}
     assert [node.target for node in stay] == before
     assert [node.target for node in move] == [layer_norm8, layer_norm8, layer_norm8, layer_norm_fork8]
+
+
+def test_every_bounded_wait_has_a_code_of_its_own():
+    """hapx_gemm_status names the role that gave up: the quantiser and the product's own quantising warps are two."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(block8.__file__), "csrc")
+    text = {name: open(os.path.join(csrc, name)).read() for name in ("hapx_block8.cu", "hapx_gemm8_sm100.cu", "hapx_gemm_sm100.cu")}
+    codes = {name: re.findall(r"atomicCAS\(\w+\.error, 0u, (\d+)u\)", t) for name, t in text.items()}
+    assert codes["hapx_block8.cu"] == ["4"] and sorted(codes["hapx_gemm8_sm100.cu"]) == ["1", "2", "3", "5"]
+    message = text["hapx_gemm_sm100.cu"].split("gave up waiting on a barrier (role ")[1].split(";")[0]
+    for code in sum(codes.values(), []):
+        assert re.search(rf"\b{code} = ", message), f"role {code} is not named"
