@@ -112,15 +112,15 @@ def _empty(rows: int, cols: int, device, transposed: Optional[Block8] = None) ->
     return Block8(values, scales, rows, cols, transposed)
 
 
-def _run(x: torch.Tensor, square: bool, q: Optional[Block8], qt: Optional[Block8], colsum: Optional[torch.Tensor] = None) -> None:
+def _run(x: torch.Tensor, square: bool, q: Optional[Block8], qt: Optional[Block8]) -> None:
     """One pass of the quantiser over ``x`` into ``q`` (as it stands) and / or ``qt`` (transposed)."""
     rows, cols = x.shape
     ldx = x.stride(0) if rows > 1 else cols
     a = (q.values.data_ptr(), q.values.shape[1], q.scales.data_ptr()) if q is not None else (None, 0, None)
     b = (qt.values.data_ptr(), qt.values.shape[1], qt.scales.data_ptr()) if qt is not None else (None, 0, None)
     with _on_device(x.device):
-        N.check(N.lib.hapx_block8_quantize(x.data_ptr(), _CODES[x.dtype], rows, cols, ldx, int(square), *a, *b,
-                                           colsum.data_ptr() if colsum is not None else None, _stream(x.device)))
+        N.check(N.lib.hapx_block8_quantize(x.data_ptr(), _CODES[x.dtype], rows, cols, ldx, int(square), *a, *b, None,
+                                           _stream(x.device)))
 
 
 def quantize(x: torch.Tensor, rows: bool = True, columns: bool = False):
