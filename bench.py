@@ -946,6 +946,23 @@ def run_lm_cpu(world, batch_per_rank, layers):
             "step_s": r["s"]}
 
 
+def step_roofline(fwd, core, ms, peaks, peak_kind, block8):
+    """The ``roofline`` of a training step that took ``ms``: the GEMM flops of the busiest rank (largest batch share), 3 x
+    forward, 2*M*N*K each.  ``core``: those of ``fwd`` that are no linear products (attention core, expert FFNs) and stay in
+    bf16 when ``block8`` moves the linear ones to 8 bits.  ``peak`` is then the rate of both at theirs, one after the other."""
+    achieved = 3 * fwd / (ms * 1e-3) / 1e12
+    bf16 = peaks.get("bf16_tflops_sustained") or peaks["bf16_tflops"]
+    kernel, peak = "gemm2_bf16_kernel (all linear / attention contractions of the busiest rank)", bf16
+    kind = peak_kind + " (sustained: the kernels run inside a long step)"
+    if block8:
+        kernel = "gemm8_kernel (linear products of the busiest rank, e4m3), bf16 kernels (its other contractions)"
+        peak = fwd / ((fwd - core) / (2 * bf16) + core / bf16)
+        kind += "; 8-bit products at twice the bf16 rate (nominal ratio: no 8-bit rate was measured)"
+    return {"bound": "tensor", "kernel": kernel, "achieved": achieved, "peak": peak, "unit": "TFLOP/s", "frac": achieved / peak,
+            "peak_kind": kind, "traffic": None,
+            "note": "whole-step time, so this fraction also pays for every non-GEMM op of the step"}
+
+
 def lm_step(args, job, kind, plan, use_graph, dropout_p, block8=False):
     """Time the training step of one program (``kind``: lm / vit / moe) at job.n_gpus GPUs: device time per
     step (CUDA events, max over ranks) and the end-to-end time with the inputs coming from pinned host memory
@@ -972,14 +989,16 @@ def lm_step(args, job, kind, plan, use_graph, dropout_p, block8=False):
         emit = lambda m, r: P.emit_lm(m, plan, ratios, r, B, dropout_p=dropout_p)
         in_h = (torch.randint(0, 33278, (B, 256), generator=g), torch.randint(0, 33278, (B, 256), generator=g))
         M = bmax * 256
-        fwd = L * (2.0 * M * 768 * (2304 + 768 + 3072 + 3072) + 2 * 2.0 * bmax * 12 * 256 * 256 * 64) + 2.0 * M * 768 * 33280
+        core = L * 2 * 2.0 * bmax * 12 * 256 * 256 * 64
+        fwd = L * 2.0 * M * 768 * (2304 + 768 + 3072 + 3072) + 2.0 * M * 768 * 33280 + core
         desc = f"Transformer LM training step ({L} layers, d_model 768, 12 heads, FFN 3072, pre-LN, vocab 33280, seq 256, dropout {dropout_p}), plan {plan}"
     elif kind == "vit":
         model = P.ViT(nlayers=L)
         emit = lambda m, r: P.emit_vit(m, plan, ratios, r, B, dropout_p=dropout_p)
         in_h = (torch.randn(B, 3, 224, 224, generator=g).to(torch.bfloat16), torch.randint(0, 1000, (B,), generator=g))
         M = bmax * 197
-        fwd = L * (2.0 * M * 768 * (2304 + 768 + 3072 + 3072) + 2 * 2.0 * bmax * 12 * 197 * 197 * 64) + 2.0 * bmax * 196 * 768 * 768
+        core = L * 2 * 2.0 * bmax * 12 * 197 * 197 * 64
+        fwd = L * 2.0 * M * 768 * (2304 + 768 + 3072 + 3072) + 2.0 * bmax * 196 * 768 * 768 + core
         desc = f"ViT-B/16 training step ({L} layers, d 768, 12 heads, MLP 3072, 224x224x3 images, 1000 classes, dropout {dropout_p}), plan {plan}"
     else:
         model = P.MoETransformerLM(nlayers=L)
@@ -987,8 +1006,8 @@ def lm_step(args, job, kind, plan, use_graph, dropout_p, block8=False):
         in_h = (torch.randint(0, 33278, (B, 512), generator=g), torch.randint(0, 33278, (B, 512), generator=g))
         M = bmax * 512
         e_max = max(hap_b200.sharding_round(32, ratios))
-        fwd = L * (2.0 * M * 1024 * (3072 + 1024) + 2 * 2.0 * bmax * 16 * 512 * 512 * 64        # attention projections + core
-                   + 2 * 2.0 * B * e_max * 20 * 1024 * 4096) + 2.0 * M * 1024 * 33280           # expert FFNs of the busiest rank
+        core = L * (2 * 2.0 * bmax * 16 * 512 * 512 * 64 + 2 * 2.0 * B * e_max * 20 * 1024 * 4096)     # attention core, expert FFNs of the busiest rank
+        fwd = L * 2.0 * M * 1024 * (3072 + 1024) + 2.0 * M * 1024 * 33280 + core
         desc = (f"MoE Transformer training step ({L} layers, d_model 1024, 16 heads, 32 experts FFN 4096, top-2 gating, capacity 20, "
                 f"vocab 33280, seq 512, dropout {dropout_p}), expert parallel, experts per rank {hap_b200.sharding_round(32, ratios)}")
     model = model.to(torch.bfloat16).to(dev)
@@ -1100,9 +1119,6 @@ def lm_step(args, job, kind, plan, use_graph, dropout_p, block8=False):
     comm.check()
     hap_b200.linear_ops.gemm_status()
     peaks, peak_kind = measured_peaks()
-    # GEMM flops of one step on the busiest rank (largest batch share): 3 x forward, 2*M*N*K each
-    achieved = 3 * fwd / (ms * 1e-3) / 1e12
-    peak = peaks.get("bf16_tflops_sustained") or peaks["bf16_tflops"]
     result = {
         "metric": "spmd_step_samples_per_s", "value": B / (ms * 1e-3), "unit": "samples/s", "n_gpus": n_gpus, "steps": args.steps,
         "warmup": max(args.warmup, 3), "ms_per_step": ms, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
@@ -1110,10 +1126,7 @@ def lm_step(args, job, kind, plan, use_graph, dropout_p, block8=False):
         "config": {"workload": f"{desc}{', 8-bit blocks' if block8 else ''}, global batch {B} split {lb}", "parameters": n_params, "plan": plan, "batch_split": lb,
                    "executor": "CUDA graph of the whole iteration" if use_graph else "eager fx GraphModule",
                    "l2": "activations and weights of a step exceed L2 by far", "loss": losses[-1]},
-        "roofline": {"bound": "tensor", "kernel": "gemm2_bf16_kernel (all linear / attention contractions of the busiest rank)",
-                     "achieved": achieved, "peak": peak, "unit": "TFLOP/s", "frac": achieved / peak,
-                     "peak_kind": peak_kind + " (sustained: the kernels run inside a long step)", "traffic": None,
-                     "note": "whole-step time, so this fraction also pays for every non-GEMM op of the step"},
+        "roofline": step_roofline(fwd, core, ms, peaks, peak_kind, block8),
         "e2e": {"value": B / (e2e_ms * 1e-3), "unit": "samples/s",
                 "h2d_bytes_per_step": int(tok_h.numel() * tok_h.element_size() + tgt_h.numel() * tgt_h.element_size()) * n_gpus,
                 "d2h_bytes_per_step": 4 * n_gpus, "ms_per_step": e2e_ms, "host_wall_ms_per_step": wall_ms, "steps": e2e_steps,
