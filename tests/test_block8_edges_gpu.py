@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import block8_math as B
-from tests.test_block8_gpu import BF, DEV, F32, close, gen, sum_slack
+from tests.test_block8_gpu import BF, DEV, F32, close, gen, leaf, linear_inputs, lm_worker, sum_slack
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,80 @@ def test_gelu_gradient_of_the_largest_numbers(dtype):
         g = torch.full_like(x, 0.75)
         D.act_dropout8(xg, "gelu", 0.0).backward(g.to(DEV))
         close(xg.grad, 0.75 * B.gelu_slope(B.runs(sign * x)), torch.full(x.shape, 2.0 ** -20, dtype=torch.float64))
+
+
+def test_replayed_steps_train_like_eager_ones():
+    """Three steps of the 8-bit program, eager and replayed from a graph, from the same parameters and optimizer state: the
+    losses, every updated parameter and both moments have the same bits."""
+    import hap_b200
+    g = gen(0)
+    batches = [tuple(torch.randint(0, 520, (5, 40), generator=g).to(DEV) for _ in range(2)) for _ in range(3)]
+    runs = []
+    for captured in (False, False, True):
+        model, worker = lm_worker()
+        opt, step = worker.optimizer, worker.step
+        state = [*model.parameters(), *opt.exp_avg, *opt.exp_avg_sq, opt.state]
+        if captured:
+            start = [t.detach().clone() for t in state]
+            step = worker.capture(*batches[0])
+            with torch.no_grad():
+                for t, s in zip(state, start):
+                    t.copy_(s)
+        hap_b200.dropout.manual_seed(1)
+        losses = [float(step(*b)) for b in batches]
+        # every parameter had a gradient (a norm's weight of 1 may not move: a step of 1e-3 is below 2^-9, half its rounding)
+        assert all(float(m.float().abs().max()) > 0 for m in opt.exp_avg)
+        runs.append((losses, [t.detach().clone() for t in state]))
+        del step, worker
+    for losses, state in runs[1:]:
+        assert losses == runs[0][0]
+        for a, b in zip(state, runs[0][1]):
+            assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["gelu", "relu", "fork", "linear"])
+def test_two_graphs_of_each_operator_replayed_beside_an_eager_call(which):
+    """Forward and backward (dropout on) captured twice and replayed on two streams at once, with an eager call beside them."""
+    import hap_b200
+    from hap_b200 import block8
+    from hap_b200 import dropout as D
+    from hap_b200.norm import layer_norm_fork8
+    x, w, b, g = (t.to(DEV) for t in linear_inputs(700, 520, 264, BF))
+    gx, wv, bv = x.flip(0), w[0].clone(), w[1].clone()
+    w8 = block8.quantize_weight(w, transposed=True)
+
+    def step(v):
+        v, lw, lb = (t.detach().requires_grad_(True) for t in (v, wv, bv))
+        if which == "fork":
+            res, y = layer_norm_fork8(v, (520,), lw, lb)
+            return (y.detach(), *torch.autograd.grad([res, y], (v, lw, lb), [gx, gx]))
+        if which == "linear":
+            y = hap_b200.linear8(v, w8, b)
+            return (y.detach(), *torch.autograd.grad(y, v, g))
+        y = D._ActDropout8.apply(v, D._ACTS[which], 0.25, 7)             # the same call id, so the same mask, in every call
+        return (y.detach(), *torch.autograd.grad(y, v, gx))
+    xs = [x, x * 2]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [[t.clone() for t in step(v)] for v in xs]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(float(t.float().abs().max()) > 0 for t in want[0])
+    graphs, outs = [], []
+    for v in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(v))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        eager = step(x)
+    torch.cuda.synchronize()
+    for got, ref in ((outs[0], want[0]), (outs[1], want[1]), (eager, want[0])):
+        for a, c in zip(got, ref):
+            assert torch.equal(a, c)
