@@ -36,7 +36,7 @@ def _scale_bytes(rows: int, cols: int) -> int:
 
 
 class Block8:
-    """``rows x cols`` e4m3 values (``values``, float8_e4m3fn, rows padded to a multiple of 16 bytes) and one
+    """``rows x cols`` e4m3 values (``values``, float8_e4m3fn, contiguous, rows padded to a multiple of 16 bytes) and one
     power-of-two scale per 128 columns of a row (``scales``, bytes in the order the tensor cores read them;
     :meth:`scale_matrix` decodes them).  ``transposed`` is the same matrix with rows and columns exchanged, where the
     maker was asked for both."""
@@ -78,7 +78,8 @@ class Block8:
         return torch.ldexp(torch.ones(s.shape, device=s.device), s.to(torch.int32) - 127)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """The matrix as it is represented (exact in bfloat16 too: e4m3 has four significant bits)."""
+        """The matrix as it is represented (exact in bfloat16 too, as e4m3 has four significant bits; what a scale of 2^120 or
+        one near 2^-126 takes out of the type's range is rounded there)."""
         if dtype not in _CODES:
             raise TypeError(f"block8: bfloat16 or float32 only, got {dtype}")
         out = torch.empty((self.rows, self.cols), dtype=dtype, device=self.device)

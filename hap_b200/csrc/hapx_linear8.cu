@@ -4,8 +4,8 @@
 // transposed, for the input gradient), both in one launch, then the product.  Backward: g likewise in both forms from one
 // read, with the partial sums of the bias gradient, then the two products in one launch, which joins those sums.
 //
-// 8192 x 768 -> 2304 (bfloat16), forward and both gradients: 76 us (28 + 48: quantisers 12 + 19, products 16 + 28); with
-// bfloat16 products 104.  -> 33280: 233 + 520 us against 1150.
+// 8192 x 768 -> 2304 (bfloat16), forward and both gradients: 80 us (28 + 48 one direction at a time: quantisers 12 + 19,
+// products 16 + 28); with bfloat16 products 104.  -> 33280: 765 us (234 + 525) against 1130.
 //
 // Up to 32 tokens through a weight that is already in 8 bits take one launch: the product's, which converts x by itself.
 #include <algorithm>
@@ -20,13 +20,13 @@ namespace linear8 {
 
 using namespace block8;
 
-constexpr int kThinTokens = 2;              // 2 x 768 -> 2304 takes 4.7 us here, 2 x 768 -> 33280 14.6; 4 tokens on the tensor cores 6.2 and 12.8
+constexpr int kThinTokens = 2;              // 2 x 768 -> 2304 takes 4.1 us here, 2 x 768 -> 33280 14.4; 4 tokens on the tensor cores 5.7 and 12.7
 constexpr int kThinElements = 24 * 1024;    // tokens x in_features that fit shared memory as float32 (96 KiB)
 
 // One or two tokens: y[m, n] = sum over blocks of s_x s_w sum of q_x q_w, + bias.  No tensor cores: the time is that of the
 // launch and of reading the weight (bytes N K).  Every thread block makes the 8-bit form of x for itself in shared memory, a
 // warp multiplies ROWS rows of w, whose loads are in flight together, with all tokens from registers; the values multiplied
-// are those of the other path.  One token, 768 -> 2304: 3.5 us, 768 -> 33280: 10.8 us = 2.4 TB/s (of L2), where its blocks are
+// are those of the other path.  One token, 768 -> 2304: 3.0 us, 768 -> 33280: 11.0 us = 2.3 TB/s (of L2), where its blocks are
 // too many for one round of the SMs.
 // A sum of 16 products of e4m3 numbers is 0 or lies in [2^-18, 2^22): with a weight's scale in [2^-108, 2^105] it stays a
 // normal number, and the token's scale then rounds it once at most.

@@ -8,7 +8,8 @@
 //   layer_norm y = (x - mean) rstd w + b  z = (x~ - mean) rstd,  g = dy w,  dx = rstd (g - mean(g) - z mean(g z)) [+ add],
 //                                         dw = sum dy z,  db = sum dy      (mean and rstd of x itself, in float32)
 //
-// x~ is x to half a step of 3 fraction bits; forward results are those of the operators that keep x.
+// x~ is x to half a step of 3 fraction bits; forward results are those of the operators that keep x, to rounding (gelu has a
+// distribution function of its own here, layer_norm adds in another order).
 #include <algorithm>
 #include <mutex>
 #include <set>
@@ -29,8 +30,10 @@ enum Act { ACT_RELU = 1, ACT_GELU = 2 };
 
 // Phi(v) = erfc(-v / sqrt 2) / 2 and e = exp(-v^2 / 2) = 2^(-u^2), u = |v| sqrt(log2(e) / 2).  For v < 0 it is the tail
 // e t P(t) with t = 1 / (1 + 0.36 u): P is a least-maximum fit to erfcx(|v| / sqrt 2) / (2 t) over |v| <= 13, so the tail
-// keeps its relative accuracy, which y = v Phi(v) needs, and shares its exponential with the density.  Degree 7 for
-// float32 tensors (relative error 1.0e-7), degree 5 for bfloat16 ones (4.1e-6, a 950th of their rounding).
+// keeps most of its relative accuracy, which y = v Phi(v) needs, and shares its exponential with the density.  Degree 7 for
+// float32 tensors (the fit is off by 1.0e-7 of itself), degree 5 for bfloat16 ones (4.1e-6, a 950th of their rounding).  The
+// rounding of u and u^2 comes on top, which the exponential turns into (2 v^2 + 16) 2^-24 of the tail at most: measured in
+// float32 5e-7 on [-1, 0], 2.6e-6 on [-5, -3], 4.8e-6 on [-8, -5], 1.3e-5 at -12.9.
 template <bool WIDE>
 __device__ __forceinline__ float normal_cdf(float v, float& e) {
   const float u = fabsf(v) * 0.84932180028801907f;
@@ -311,7 +314,8 @@ __device__ __forceinline__ int valid_of(int E, int c) { return VEC ? (c < E ? 8 
 
 // A team of W warps holds a row in registers (a lane's eight columns, NG groups of them) and has the next row's loads in
 // flight; mean, then the mean of squared distances, then y and the blocks of x from the same registers.  By its bytes
-// HBM-bound; measured it is the chain of a row's two sums and sixteen-lane maxima: bfloat16 8192 x 768 9.4 us = 3.4 TB/s,
+// HBM-bound; measured it is the chain of a row's two sums and sixteen-lane maxima with few warps to hide it (three groups of
+// 256 columns take all 128 registers that two blocks per SM leave: 16 warps): bfloat16 8192 x 768 9.4 us = 3.4 TB/s,
 // 2048 x 8192 20.5, float32 4000 x 2040 16.1 = 4.6 TB/s.
 template <typename T, int W, int NG, bool VEC>
 __global__ void __launch_bounds__(256, 2) norm_forward_team_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b,
@@ -399,8 +403,9 @@ __global__ void __launch_bounds__(256, 2) norm_forward_team_kernel(const T* __re
 
 // dx of the rows, and partial[block][0][c] = sum dy z, partial[block][1][c] = sum dy over the rows the thread block took.  The
 // running sums of a warp's columns lie in shared memory, owned by the warp: in registers, next to the prefetched row, they
-// would leave half of the warps.  Bound by the row's chain and by adding to those sums (with the join of the partials 8192 x
-// 768 takes 15.2 us = 2.1 TB/s, with the residual's gradient 16.1; float32 4000 x 2040 25.0 = 2.9 TB/s).
+// would leave half of the warps.  Bound by the row's chain, again with 16 warps per SM (bfloat16 rows of 513 to 768 columns and
+// of more than 4096 spill a few registers even so), and by adding to those sums (with the join of the partials 8192 x 768
+// takes 15.2 us = 2.1 TB/s, with the residual's gradient 16.1; float32 4000 x 2040 25.0 = 2.9 TB/s).
 template <typename T, int W, int NG, bool VEC>
 __global__ void __launch_bounds__(256, 2) norm_backward_team_kernel(const unsigned char* __restrict__ q, long long ldq, const float* __restrict__ s,
                                                                     const T* __restrict__ dy, const T* __restrict__ w,

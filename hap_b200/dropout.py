@@ -216,8 +216,11 @@ class _ActDropout8(torch.autograd.Function):
 
 def act_dropout8(x: torch.Tensor, act: str, p: float, training: bool = True) -> torch.Tensor:
     """:func:`act_dropout` that keeps one byte (gelu) or one bit (relu) per element for the backward pass instead of a
-    whole tensor.  The result is the same; relu's gradient too, gelu's slope is taken at the input rounded to e4m3
-    (blocks of 128 consecutive elements, :mod:`hap_b200.block8`)."""
+    whole tensor.  relu's result and gradient have the same bits (but a NaN passes, as in torch, where act_dropout gives 0);
+    gelu's result differs by at most 2^-20 |x| (float32) or 2^-18 |x| (bfloat16), scaled as the kept elements are, and the
+    rounding - most far below zero, where this form keeps its relative accuracy - and its slope is taken at the input
+    rounded to e4m3 (blocks of 128 consecutive elements, :mod:`hap_b200.block8`).  No forward-mode derivative: a tangent is
+    refused."""
     _check(x, "act_dropout8", p)
     if act not in _ACTS:
         raise ValueError(f"act_dropout8: the activation is \"relu\" or \"gelu\", got {act!r}")

@@ -305,7 +305,7 @@ def use_block8(graph: torch.fx.Graph, products: bool = True, saved: bool = True,
       :func:`hap_b200.attention.multi_head_attention_forward8` (its two projections): products in 8-bit floating point,
       inputs kept for the backward pass in 8 bits;
     * ``saved``: ``act_dropout`` -> :func:`hap_b200.dropout.act_dropout8`, ``layer_norm`` / ``layer_norm_fork`` ->
-      :func:`hap_b200.norm.layer_norm8` / ``layer_norm_fork8``: the same forward results, inputs kept in 8 bits.
+      :func:`hap_b200.norm.layer_norm8` / ``layer_norm_fork8``: the same forward results to rounding, inputs kept in 8 bits.
 
     Nodes that the 8-bit form does not take and ``layer_norm`` hands to torch stay as they are and are not counted: a
     normalised shape of several dimensions, of more than 2^20 elements or not known before the program runs, and types

@@ -13,6 +13,10 @@ x8t is written by the pass that makes x8 and is all the forward pass keeps of x:
 per 128 instead of two or four bytes per element.  The weight's 8-bit transposed form is kept too (one byte per
 weight).  A weight that does not change (evaluation, frozen layers) is quantised once with
 :func:`hap_b200.block8.quantize_weight` and passed as it is.
+
+Blocks start where the tensor starts.  So a shard of a weight that is not cut at multiples of 128 is rounded otherwise
+than the whole weight, and so are x and g where the cut runs through their contraction; y and dx of a token do not depend
+on how the batch is cut, dW does (by the roundings of x8t and g8t).
 """
 from __future__ import annotations
 
@@ -146,7 +150,8 @@ def linear8(input: torch.Tensor, weight: Union[torch.Tensor, Block8], bias: Opti
     """``F.linear(input, weight, bias)`` on CUDA bfloat16 or float32 tensors of any extents, with the products in 8-bit
     floating point (see the module).  ``weight``: a tensor of the input's type, or a :class:`hap_b200.block8.Block8`
     from :func:`hap_b200.block8.quantize_weight` - then nothing is computed for a weight gradient, and a gradient of
-    the input needs the weight's transposed form (``quantize_weight(w, transposed=True)``)."""
+    the input needs the weight's transposed form (``quantize_weight(w, transposed=True)``).  No forward-mode derivative: a
+    tangent is refused."""
     if not input.is_cuda:
         raise RuntimeError(f"linear8: hap_b200 has no CPU path; tensor is on {input.device}")
     dtype, shape = input.dtype, input.shape

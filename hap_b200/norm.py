@@ -218,10 +218,10 @@ def _check8(what, input, shape, weight, bias):
 
 
 def layer_norm8(input: torch.Tensor, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
-    """:func:`layer_norm` over the last dimension (of any extent) that keeps its input for the backward pass as e4m3
-    values with one scale per 128 columns (:mod:`hap_b200.block8`) and two floats per row, instead of the input
-    itself.  The result is layer_norm's; the gradients are layer_norm's at the rounded input, normalised with the
-    statistics of the input itself."""
+    """:func:`layer_norm` over the last dimension (of any extent up to 2^20) that keeps its input for the backward pass as
+    e4m3 values with one scale per 128 columns (:mod:`hap_b200.block8`) and two floats per row, instead of the input
+    itself.  The result is layer_norm's to the order of its float32 sums; the gradients are layer_norm's at the rounded
+    input, normalised with the statistics of the input itself.  No forward-mode derivative: a tangent is refused."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     _check8("layer_norm8", input, shape, weight, bias)
     if _differentiated(input, weight, bias):
