@@ -40,6 +40,8 @@ def test_prepared_weight_with_the_most_output_features(rows):
         y[r, -8:] = y[r, 2 ** 30] = xr
         low, high = torch.aminmax(y[r])
         assert float(low) == float(high) == xr
+    del y
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("rows", [1, 2, 3, 33, 200])
